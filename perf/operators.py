@@ -403,11 +403,13 @@ def _run_compact(s):
     count = cu[1:] - cu[:-1]
     seq = torch.repeat_interleave(torch.arange(n, device=dev), count)
     j = torch.arange(keep.shape[1], device=dev) - cu[seq]
-    # pages at the front whose tokens all stay where they are keep their blocks (all pages, where all tokens do)
+    # full pages at the front whose tokens all stay where they are keep their blocks (a sequence that keeps
+    # every token keeps every page)
     moved = torch.where(keep != j, j, count[seq]).to(torch.int64)
     first = torch.full((L, n), 1 << 40, device=dev).scatter_reduce_(1, seq.expand(L, -1), moved, "amin")
     pages = (count + BLOCK - 1) // BLOCK
-    lead = torch.where(first == count, pages, first // BLOCK)
+    whole = (first == count) & (count == s["ntok"][:, s["src"].long()])
+    lead = torch.where(whole, pages, first.minimum(count) // BLOCK)
     # fresh blocks, popped sequence by sequence, layer by layer, page by page
     page = torch.arange(s["tables"].shape[2], device=dev)
     mine = page < pages.view(n, 1, 1)
@@ -632,7 +634,7 @@ def _exact_compact(c, s):
             stay = 0
             while stay < len(kept) and kept[stay] == stay:
                 stay += 1
-            if stay == len(kept):
+            if stay == len(kept) == int(s["ntok"][layer, i]):
                 continue
             begin = stay // BLOCK * BLOCK
             to = np.arange(begin, len(kept))
