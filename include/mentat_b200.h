@@ -36,6 +36,10 @@ extern "C" {
 #define MENTAT_DEV_PLAN_OVERFLOW 4   /* decode plan exceeded its workspace */
 #define MENTAT_DEV_TABLE_OVERFLOW 5  /* a sequence outgrew max_blocks_per_seq */
 #define MENTAT_DEV_DECODE_TIMEOUT 6  /* a bounded wait in a decode kernel gave up; that call's output is invalid */
+#define MENTAT_DEV_BAD_SLOT 8    /* a batch of sequences names a slot outside [0, max_seqs), one twice, or a
+                                    destination in use (ctrl[ERRARG] = the slot); the call changes nothing */
+#define MENTAT_DEV_BAD_TOKEN 9   /* a kept position outside its sequence (ctrl[ERRARG] = the position); the
+                                    call changes nothing */
 #define MENTAT_DEV_BAD_BLOCK 7       /* a block table entry outside [0, num_blocks) (ctrl[ERRARG] = the entry),
                                         which the decode and gather kernels do not read; that call's output is
                                         invalid.  The reference asserts on bad block ids at paged_kv_cache.py:59,63 */
@@ -305,6 +309,150 @@ int mentat_gate_step(const void* logits, int32_t dtype, int32_t n, int32_t vocab
 int mentat_prune_similar(const void* sim, int32_t dtype, int64_t sim_stride, const int32_t* group_off,
                          int32_t ngroups, int32_t max_group, const int64_t* parent_key, const double* logp,
                          float threshold, uint8_t* prune_out, cudaStream_t s);
+
+/*
+ * Rotary positions.  No counterpart in the reference, which leaves them to the
+ * model's own modules (qwen3_adapter.py:71-93, :195-221).  Dimensions offset ..
+ * offset + 2 pairs of every head are taken as pairs (i, i + pairs), or
+ * (2i, 2i + 1) if interleaved, and pair i is turned by position * inv_freq[i]
+ * (by its negative if inverse) and multiplied by scale; the other dimensions
+ * are copied.  Angles are reduced to one turn in 64 bits, so positions may be
+ * any int64 (negative ones turn backwards); the pairs are turned in 32 bits and
+ * rounded once.
+ */
+typedef struct mentat_rotary {
+    const double* inv_freq;      /* device [pairs], radians per position */
+    int32_t pairs;               /* 2 * pairs + offset <= head_dim */
+    int32_t offset;
+    int32_t interleaved;
+    int32_t inverse;
+    float scale;
+} mentat_rotary;
+
+/* rows of a [tokens][heads][head_dim] tensor, head_dim contiguous, strides in elements */
+typedef struct mentat_rows {
+    void* ptr;
+    int64_t token_stride;
+    int64_t head_stride;
+    int32_t heads;
+} mentat_rows;
+
+/* Turns q and k (either may have 0 heads) of n tokens at positions (device
+ * int64[n]) into q_out and k_out, which may be q and k themselves (in place)
+ * but must not overlap them otherwise. */
+int mentat_rotary_apply(int32_t dtype, int32_t head_dim, int32_t n, const mentat_rows* q, const mentat_rows* q_out,
+                        const mentat_rows* k, const mentat_rows* k_out, const int64_t* positions,
+                        const mentat_rotary* r, cudaStream_t s);
+
+/* The same with k's rows and v's written into the cache: token i goes to row
+ * rows[i] = block * block_size + offset of layer `layer` (device int64[n],
+ * distinct; -1 writes no row, for padding).  A row outside the pool is recorded
+ * as MENTAT_DEV_BAD_BLOCK and not written.  q may have 0 heads. */
+int mentat_rotary_append(const mentat_kv_cache* c, int32_t layer, int32_t n, const int64_t* rows, const mentat_rows* q,
+                         const mentat_rows* q_out, const mentat_rows* k, const mentat_rows* v,
+                         const int64_t* positions, const mentat_rotary* r, cudaStream_t s);
+
+/* mentat_kv_append_batched (one token for each of n sequences) and
+ * mentat_kv_append (n tokens of one sequence) with q and k turned on the way:
+ * a token's position is its index in its sequence, plus nothing else, unless
+ * positions (device int64[n]) is given.  q_out as in mentat_rotary_apply; a
+ * padding entry (slot -1) is turned as at position 0.  If the call records an
+ * error, q_out is not written. */
+int mentat_kv_append_rotated_batched(const mentat_kv_cache* c, int32_t layer, const int32_t* slots, int32_t n,
+                                     const mentat_rows* q, const mentat_rows* q_out, const mentat_rows* k,
+                                     const mentat_rows* v, const int64_t* positions, const mentat_rotary* r,
+                                     cudaStream_t s);
+int mentat_kv_append_rotated(const mentat_kv_cache* c, int32_t layer, int32_t slot, int32_t n, const mentat_rows* q,
+                             const mentat_rows* q_out, const mentat_rows* k, const mentat_rows* v,
+                             const int64_t* positions, const mentat_rotary* r, cudaStream_t s);
+
+/*
+ * Pages of several sequences at once.  The slots are device int32[n], n <= 1024.
+ * A batch that names a slot outside [0, max_seqs), or one that must be distinct
+ * twice, changes nothing and records MENTAT_DEV_BAD_SLOT.
+ */
+/* fork_sequence (paged_kv_cache.py:152-170) of parents[i] into children[i].
+ * The children are distinct and none is also a parent; a parent may have
+ * several.  max_nblocks is the longest parent's table (a launch-size hint). */
+int mentat_kv_fork_batched(const mentat_kv_cache* c, const int32_t* parents, const int32_t* children, int32_t n,
+                           int32_t max_nblocks, cudaStream_t s);
+
+/* free_sequence (paged_kv_cache.py:172-176) of distinct slots, with the state
+ * that freeing them one after another leaves, the free list's order included.
+ * workspace: mentat_pages_workspace_bytes(c, n) bytes. */
+int64_t mentat_pages_workspace_bytes(const mentat_kv_cache* c, int32_t n);
+int mentat_kv_free_batched(const mentat_kv_cache* c, const int32_t* slots, int32_t n, int32_t max_nblocks,
+                           void* workspace, int64_t workspace_bytes, cudaStream_t s);
+
+/* Compaction to kept tokens.  No counterpart in the reference (trim_to_window,
+ * paged_kv_cache.py:370-417, keeps a window of one sequence).  Sequence i keeps
+ * the positions keep[layer * keep_layer_stride + cu[i] .. cu[i + 1]) of
+ * src[i], in that order (any order; a position may repeat), as its positions 0,
+ * 1, ...; keep_layer_stride 0 keeps the same ones in every layer.  max_keep is
+ * the longest list, max_nblocks the longest source table (launch-size hints:
+ * larger is safe).  Full pages at the front whose tokens all stay in place (all
+ * pages, if the sequence keeps every token) are not copied; the others are written
+ * to fresh blocks, popped sequence by sequence, layer by layer.  With dst NULL the
+ * sequences are compacted in place (src distinct) and the pages they no longer
+ * hold are released in that order; the fresh blocks are taken before.  Otherwise
+ * dst[i], distinct and empty, becomes a new sequence that shares the pages at the
+ * front, and src[i] stays as it is.  With a rotary the keys of copied rows are
+ * turned from their old position to the new one (scale is not applied again).
+ * workspace as above. */
+int mentat_kv_compact(const mentat_kv_cache* c, const int32_t* src, const int32_t* dst, int32_t n,
+                      const int32_t* keep, int64_t keep_layer_stride, const int32_t* cu, int32_t max_keep,
+                      int32_t max_nblocks, const mentat_rotary* r, void* workspace, int64_t workspace_bytes,
+                      cudaStream_t s);
+
+/*
+ * Page index: for each block and KV head the bounds of its keys in every
+ * channel, 8 bits with one power of two: bounds [layers][blocks][kv_heads][2]
+ * [head_dim] (lowest values rounded down, then highest rounded up, in units of
+ * 2^exps), exps [layers][blocks][kv_heads], the least e with every |key| <=
+ * 127 * 2^e, within -50 .. 50 (larger keys saturate at 127).  A page with a NaN
+ * or an infinity among its keys has exps 127.  No counterpart in the reference.
+ */
+typedef struct mentat_page_index {
+    int8_t* bounds;
+    int8_t* exps;
+} mentat_page_index;
+
+/* Indexes the n blocks (device int32[n]) of layer `layer`, every row of each. */
+int mentat_page_index_blocks(const mentat_kv_cache* c, int32_t layer, const int32_t* blocks, int32_t n,
+                             const mentat_page_index* x, cudaStream_t s);
+
+/* Indexes the full pages first_page .. first_page + max_pages of n sequences
+ * (slots, device int32[n]; -1 is skipped) in layer `layer`, or in every layer if
+ * layer is -1; first_page -1 means each one's last page alone, if it is full. */
+int mentat_page_index_seqs(const mentat_kv_cache* c, int32_t layer, const int32_t* slots, int32_t n,
+                           int32_t first_page, int32_t max_pages, const mentat_page_index* x, cudaStream_t s);
+
+/* What the index holds for n blocks, as the values it stands for: low and high
+ * float [n][kv_heads][head_dim], and a copy of their exponents [n][kv_heads]. */
+int mentat_page_bounds(const mentat_kv_cache* c, int32_t layer, const int32_t* blocks, int32_t n,
+                       const mentat_page_index* x, float* low, float* high, int8_t* exps, cudaStream_t s);
+
+/*
+ * Sparse decode: one query per sequence, each KV head of which attends to at
+ * most `budget` of the sequence's pages.  Its first `sink` and last `recent`
+ * (>= 1) pages are always among them; the others are those with the highest
+ * scores, ties to the lowest page.  The score of a page is the maximum over the
+ * KV head's query heads of an upper bound of their products with the page's
+ * keys: the query rounded to 8 bits (nearest, ties to even, in units of the
+ * least power of two 2^e with |q| <= 127 * 2^e, e within -50 .. 50; NaN and infinities count as 0)
+ * times, in every channel, the bound that makes the product larger.  It is a
+ * whole number times a power of two, so no order of summation changes it.
+ * Pages with exps 127 come before all scores.  The softmax and the sums over
+ * the chosen pages are those of mentat_paged_decode.
+ * slots, q, out, scale as in mentat_paged_decode; sink + recent <= budget <= 8192;
+ * the pages before a sequence's last one must be indexed.  max_len: the longest
+ * sequence (a longer one gets zeros and MENTAT_DEV_PLAN_OVERFLOW).  pages, if not
+ * NULL: device int32 [n][kv_heads][budget], the chosen pages in rising order,
+ * then -1.  GQA groups up to 16, head_dim 64 or 128. */
+int mentat_sparse_decode(const mentat_kv_cache* c, int32_t layer, const mentat_page_index* x, const int32_t* slots,
+                         int32_t n, const void* q, int64_t q_stride, int32_t num_q_heads, void* out,
+                         int64_t out_stride, float scale, int32_t max_len, int32_t budget, int32_t sink,
+                         int32_t recent, int32_t* pages, cudaStream_t s);
 
 #ifdef __cplusplus
 }

@@ -18,7 +18,7 @@ MENTAT_F32, MENTAT_BF16, MENTAT_F16 = 0, 1, 2
 CTRL_HEAD, CTRL_TAIL, CTRL_PEAK, CTRL_ERROR, CTRL_ERRARG, CTRL_ALLOCS, CTRL_COWS = range(7)
 CTRL_WORDS = 16
 DEV_OUT_OF_BLOCKS, DEV_REF_FREE, DEV_RELEASE_FREE, DEV_PLAN_OVERFLOW, DEV_TABLE_OVERFLOW = 1, 2, 3, 4, 5
-DEV_DECODE_TIMEOUT, DEV_BAD_BLOCK = 6, 7
+DEV_DECODE_TIMEOUT, DEV_BAD_BLOCK, DEV_BAD_SLOT, DEV_BAD_TOKEN = 6, 7, 8, 9
 GATE_MAXK = 8
 GATE_SKIP_PEN_ENTROPY, GATE_FLOAT_LOGSUM = 1, 2
 NOALLOC_SCRATCH_BYTES = 16 * 1024 * 1024
@@ -54,8 +54,24 @@ class GateOut(C.Structure):
     ]
 
 
+class Rotary(C.Structure):
+    _fields_ = [
+        ("inv_freq", C.c_void_p), ("pairs", C.c_int32), ("offset", C.c_int32), ("interleaved", C.c_int32),
+        ("inverse", C.c_int32), ("scale", C.c_float),
+    ]
+
+
+class Rows(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64), ("heads", C.c_int32)]
+
+
+class PageIndex(C.Structure):
+    _fields_ = [("bounds", C.c_void_p), ("exps", C.c_void_p)]
+
+
 _P, _I32, _I64, _F = C.c_void_p, C.c_int32, C.c_int64, C.c_float
 _KV = C.POINTER(KVCache)
+_ROT, _ROWS, _IDX = C.POINTER(Rotary), C.POINTER(Rows), C.POINTER(PageIndex)
 # (name, restype, argtypes) for every entry point of include/mentat_b200.h
 SIGNATURES = [
     ("mentat_abi_version", C.c_int, []),
@@ -84,6 +100,19 @@ SIGNATURES = [
     ("mentat_kernel_launch_count", C.c_int64, []),
     ("mentat_gate_step", C.c_int, [_P, _I32, _I32, _I32, _I64, _P, _P, _P, C.POINTER(GateParams), _P, _P]),
     ("mentat_prune_similar", C.c_int, [_P, _I32, _I64, _P, _I32, _I32, _P, _P, _F, _P, _P]),
+    ("mentat_rotary_apply", C.c_int, [_I32, _I32, _I32, _ROWS, _ROWS, _ROWS, _ROWS, _P, _ROT, _P]),
+    ("mentat_rotary_append", C.c_int, [_KV, _I32, _I32, _P, _ROWS, _ROWS, _ROWS, _ROWS, _P, _ROT, _P]),
+    ("mentat_kv_append_rotated_batched", C.c_int, [_KV, _I32, _P, _I32, _ROWS, _ROWS, _ROWS, _ROWS, _P, _ROT, _P]),
+    ("mentat_kv_append_rotated", C.c_int, [_KV, _I32, _I32, _I32, _ROWS, _ROWS, _ROWS, _ROWS, _P, _ROT, _P]),
+    ("mentat_kv_fork_batched", C.c_int, [_KV, _P, _P, _I32, _I32, _P]),
+    ("mentat_pages_workspace_bytes", _I64, [_KV, _I32]),
+    ("mentat_kv_free_batched", C.c_int, [_KV, _P, _I32, _I32, _P, _I64, _P]),
+    ("mentat_kv_compact", C.c_int, [_KV, _P, _P, _I32, _P, _I64, _P, _I32, _I32, _ROT, _P, _I64, _P]),
+    ("mentat_page_index_blocks", C.c_int, [_KV, _I32, _P, _I32, _IDX, _P]),
+    ("mentat_page_index_seqs", C.c_int, [_KV, _I32, _P, _I32, _I32, _I32, _IDX, _P]),
+    ("mentat_page_bounds", C.c_int, [_KV, _I32, _P, _I32, _IDX, _P, _P, _P, _P]),
+    ("mentat_sparse_decode", C.c_int,
+     [_KV, _I32, _IDX, _P, _I32, _P, _I64, _I32, _P, _I64, _F, _I32, _I32, _I32, _I32, _P, _P]),
 ]
 
 _lib = None

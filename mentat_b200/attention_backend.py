@@ -58,6 +58,35 @@ def attn_decode(q: torch.Tensor, k, v, cu_seqlens_q: torch.Tensor = None, cu_seq
     return out
 
 
+def attn_decode_sparse(q: torch.Tensor, k, v, budget: int, *, sink: int = 1, recent: int = 1,
+                       softmax_scale: Optional[float] = None, return_pages: bool = False):
+    """``attn_decode`` over at most ``budget`` pages of each sequence, chosen for each KV
+    head by the scores of the cache's page index (``enable_page_index``): its first
+    ``sink`` and last ``recent`` pages, then those whose keys can have the largest
+    products with the head's queries.  Where a sequence has no more pages than that
+    it is ``attn_decode``.  No counterpart in the reference.
+
+    q: (N, num_heads, head_dim); k, v: the PagedKV handles of one
+    ``build_packed_kv`` call.  Returns (N, num_heads, head_dim), with
+    ``return_pages`` also the chosen pages (``ops.sparse_decode``)."""
+    if not isinstance(k, PagedKV) or not isinstance(v, PagedKV):
+        raise TypeError("mentat_b200.attn_decode_sparse reads KV blocks in place: pass the handles returned by "
+                        "mentat_b200.PagedKVCacheManager.build_packed_kv")
+    mgr = k.cache
+    if q.shape[0] != len(k.lens):
+        raise ValueError(f"q has {q.shape[0]} sequences, the KV handle has {len(k.lens)}")
+    scale = 1.0 / math.sqrt(q.shape[2]) if softmax_scale is None else float(softmax_scale)
+    longest = max(k.lens, default=0)
+    if return_pages:
+        out = ops.sparse_decode(ops._index_of(mgr), k.layer, k.slots, q, longest, budget, sink=sink, recent=recent,
+                                scale=scale, return_pages=True)
+    else:
+        out = ops.paged_sparse_decode(q, k.slots, longest, mgr._op_id, k.layer, scale, budget, sink, recent)
+    if mgr.strict:
+        mgr.check()
+    return out
+
+
 _DENSE_INDEX: dict = {}
 
 

@@ -62,6 +62,16 @@ static cudaError_t launch(bool pdl, void (*kernel)(KArgs...), dim3 grid, dim3 bl
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// launch(...) within an entry point: counted, and an error returned as its status
+#define MENTAT_LAUNCH(...)                                               \
+    do {                                                                 \
+        if (mentat::launch(mentat::pdl_enabled(), __VA_ARGS__) != cudaSuccess) { \
+            (void)cudaGetLastError();                                    \
+            return MENTAT_ERR_CUDA;                                      \
+        }                                                                \
+        MENTAT_CHECK_LAUNCH();                                           \
+    } while (0)
+
 // device timeline of one call (trace builds only): nanosecond stamps, first and
 // last over the CTAs of a kernel
 #ifdef MENTAT_TC_TRACE
@@ -134,6 +144,12 @@ template <> struct Elem<__half> {
 };
 
 __host__ __device__ inline int dtype_bytes(int dtype) { return dtype == MENTAT_F32 ? 4 : 2; }
+
+// VEC elements moved by one access
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+    T v[VEC];
+};
 
 // ---------------------------------------------------------------------------
 // cache indexing

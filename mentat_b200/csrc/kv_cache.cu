@@ -6,7 +6,7 @@
 // in device memory so that a decode step needs no host round trip; errors go
 // to ctrl[MENTAT_CTRL_ERROR] and every kernel becomes a no-op once it is set.
 
-#include "common.cuh"
+#include "rotary.cuh"
 
 namespace mentat {
 
@@ -141,17 +141,19 @@ __device__ __forceinline__ void release_one(const mentat_kv_cache& c, int b) {
 }
 
 // scratch of the batched append: [0] mode (0 parallel, 1 sequential, 2 skip),
-// then dst block, dst slot and CoW source (-1: none) per batch entry
+// then dst block, dst slot, CoW source (-1: none) and position per batch entry
 struct AppendScratch {
     int32_t* mode;
     int32_t* dst_blk;
     int32_t* dst_slot;
     int32_t* cow_src;
+    int32_t* pos;
     __device__ AppendScratch(const mentat_kv_cache& c) {
         mode = c.scratch;
         dst_blk = c.scratch + 8;
         dst_slot = dst_blk + c.max_seqs;
         cow_src = dst_slot + c.max_seqs;
+        pos = cow_src + c.max_seqs;
     }
 };
 
@@ -185,6 +187,7 @@ __device__ void append_one_seq(const mentat_kv_cache& c, int layer, int slot, Ap
     }
     sc.dst_blk[i] = t;
     sc.dst_slot[i] = tf;
+    sc.pos[i] = c.ntok[si];
     c.tail[si] = tf + 1;
     c.ntok[si] += 1;
 }
@@ -219,6 +222,7 @@ __global__ void __launch_bounds__(1024) k_append_plan(mentat_kv_cache c, int lay
         s_slot[i] = -1;
         s_tblk[i] = -1;
         sc.dst_blk[i] = -1;
+        sc.pos[i] = 0;
     }
     if (valid) {
         slot = slots[i];
@@ -297,6 +301,7 @@ __global__ void __launch_bounds__(1024) k_append_plan(mentat_kv_cache c, int lay
         sc.dst_blk[i] = dst;
         sc.dst_slot[i] = dslot;
         sc.cow_src[i] = src;
+        sc.pos[i] = c.ntok[si];
         c.tail[si] = dslot + 1;
         c.ntok[si] += 1;
     }
@@ -336,6 +341,55 @@ __global__ void k_append_data(mentat_kv_cache c, int layer, int n, const uint8_t
         }
         block_copy_bytes(kp + pool_row(c, layer, dst, slot) * esz, k + i * k_sb, row_bytes);
         block_copy_bytes(vp + pool_row(c, layer, dst, slot) * esz, v + i * v_sb, row_bytes);
+        __syncthreads();
+    }
+}
+
+// The same with q and k turned on the way (rotary.cuh): the positions are the
+// entries' own unless given.  One CTA per entry; a repeated slot (mode 1) is walked
+// in order by CTA 0, as above.
+struct AppendRotaryArgs {
+    mentat_rotary r;
+    mentat_rows q, qo, k, v;
+    const int64_t* positions;
+};
+
+template <typename T, int VEC, bool IL>
+__global__ void __launch_bounds__(256) k_append_rotary_data(mentat_kv_cache c, int layer, int n, AppendRotaryArgs a) {
+    extern __shared__ float cs[];
+    griddep_wait();
+    griddep_launch();
+    AppendScratch sc(c);
+    const int mode = sc.mode[0];
+    if (mode == 2) return;
+    const int D = c.head_dim, H = c.num_kv_heads;
+    const int64_t blk_bytes = (int64_t)H * D * c.block_size * sizeof(T);
+    T* kp = reinterpret_cast<T*>(c.k_pool);
+    T* vp = reinterpret_cast<T*>(c.v_pool);
+    int lo = blockIdx.x, hi = blockIdx.x + 1;
+    if (mode == 1) {
+        if (blockIdx.x != 0) return;
+        lo = 0;
+        hi = n;
+    }
+    for (int i = lo; i < hi; ++i) {
+        const int dst = sc.dst_blk[i];
+        rotary_table(a.r, a.positions ? a.positions[i] : (int64_t)sc.pos[i], cs);
+        if (dst >= 0 && sc.cow_src[i] >= 0) {
+            const int64_t to = pool_row(c, layer, dst, 0), from = pool_row(c, layer, sc.cow_src[i], 0);
+            block_copy_bytes(kp + to, kp + from, blk_bytes);
+            block_copy_bytes(vp + to, vp + from, blk_bytes);
+        }
+        __syncthreads();
+        if (a.q.heads)
+            rotate_heads<T, VEC, IL>((const T*)a.q.ptr + i * a.q.token_stride, a.q.head_stride,
+                                     (T*)a.qo.ptr + i * a.qo.token_stride, a.qo.head_stride, a.q.heads, D, a.r, cs);
+        if (dst >= 0) {  // not a padding entry
+            const int64_t at = pool_row(c, layer, dst, sc.dst_slot[i]);
+            rotate_heads<T, VEC, IL>((const T*)a.k.ptr + i * a.k.token_stride, a.k.head_stride, kp + at, D, H, D, a.r,
+                                     cs);
+            copy_heads<T, VEC>((const T*)a.v.ptr + i * a.v.token_stride, a.v.head_stride, vp + at, D, H, D);
+        }
         __syncthreads();
     }
 }
@@ -449,6 +503,40 @@ __global__ void k_append_multi_data(mentat_kv_cache c, int layer, int slot, int 
     }
 }
 
+// the same with q and k turned on the way
+template <typename T, int VEC, bool IL>
+__global__ void __launch_bounds__(256) k_append_multi_rotary_data(mentat_kv_cache c, int layer, int slot, int n,
+                                                                  AppendRotaryArgs a) {
+    extern __shared__ float cs[];
+    const int32_t* sc = c.scratch;
+    if (sc[0] == 2) return;
+    const int D = c.head_dim, H = c.num_kv_heads, bs = c.block_size;
+    T* kp = reinterpret_cast<T*>(c.k_pool);
+    T* vp = reinterpret_cast<T*>(c.v_pool);
+    const int32_t* row = table_row(c, layer, slot);
+    const int cow_src = sc[1], cow_dst = sc[2], p0 = sc[3], first_n = sc[4];
+    const int copier = cow_src >= 0 ? 1 : 0;
+    int w = blockIdx.x < copier ? 0 : first_n + (int)blockIdx.x - copier;
+    const int end = blockIdx.x < copier ? first_n : n, step = blockIdx.x < copier ? 1 : (int)gridDim.x - copier;
+    if (blockIdx.x < copier) {
+        const int64_t to = pool_row(c, layer, cow_dst, 0), from = pool_row(c, layer, cow_src, 0);
+        block_copy_bytes(kp + to, kp + from, (int64_t)H * D * bs * sizeof(T));
+        block_copy_bytes(vp + to, vp + from, (int64_t)H * D * bs * sizeof(T));
+    }
+    for (; w < end; w += step) {
+        const int p = p0 + w;
+        rotary_table(a.r, a.positions ? a.positions[w] : (int64_t)p, cs);
+        __syncthreads();
+        if (a.q.heads)
+            rotate_heads<T, VEC, IL>((const T*)a.q.ptr + w * a.q.token_stride, a.q.head_stride,
+                                     (T*)a.qo.ptr + w * a.qo.token_stride, a.qo.head_stride, a.q.heads, D, a.r, cs);
+        const int64_t at = pool_row(c, layer, row[p / bs], p % bs);
+        rotate_heads<T, VEC, IL>((const T*)a.k.ptr + w * a.k.token_stride, a.k.head_stride, kp + at, D, H, D, a.r, cs);
+        copy_heads<T, VEC>((const T*)a.v.ptr + w * a.v.token_stride, a.v.head_stride, vp + at, D, H, D);
+        __syncthreads();
+    }
+}
+
 // ---------------------------------------------------------------------------
 // trim_to_window (paged_kv_cache.py:370-417), one CTA, rare
 // ---------------------------------------------------------------------------
@@ -548,6 +636,41 @@ static bool bad_cache(const mentat_kv_cache* c) {
            !c->nblocks || !c->ntok || !c->tail || !c->scratch;
 }
 
+static bool append_rotary_args(const mentat_kv_cache* c, const mentat_rows* q, const mentat_rows* qo,
+                               const mentat_rows* k, const mentat_rows* v, const int64_t* positions,
+                               const mentat_rotary* r, AppendRotaryArgs* a, bool* wide) {
+    const int D = c->head_dim;
+    if (!rotary_ok(r, D) || !rows_ok(q, true) || !rows_ok(qo, true) || !rows_ok(k, false) ||
+        !rows_ok(v, false) || qo->heads != q->heads || k->heads != c->num_kv_heads || v->heads != c->num_kv_heads)
+        return false;
+    *a = AppendRotaryArgs{*r, *q, *qo, *k, *v, positions};
+    const int esz = dtype_bytes(c->dtype), vec = 16 / esz;
+    *wide = rotary_aligned(r, D, vec) && rows_aligned(q, vec, esz) && rows_aligned(qo, vec, esz) &&
+            rows_aligned(k, vec, esz) && rows_aligned(v, vec, esz) &&
+            ((uintptr_t)c->k_pool | (uintptr_t)c->v_pool) % 16 == 0;
+    return true;
+}
+
+namespace {
+struct LaunchAppendRotary {
+    const mentat_kv_cache& c;
+    int layer, slot, n;  // slot -1: a batch of sequences
+    const AppendRotaryArgs& a;
+    cudaStream_t s;
+    template <typename T, int VEC, bool IL>
+    int operator()() {
+        const size_t smem = 2 * a.r.pairs * sizeof(float);
+        if (slot >= 0) {
+            k_append_multi_rotary_data<T, VEC, IL><<<n < 1184 ? n + 1 : 1185, 256, smem, s>>>(c, layer, slot, n, a);
+            MENTAT_CHECK_LAUNCH();
+        } else {
+            MENTAT_LAUNCH(k_append_rotary_data<T, VEC, IL>, dim3(n), dim3(256), smem, s, c, layer, n, a);
+        }
+        return MENTAT_OK;
+    }
+};
+}  // namespace
+
 extern "C" {
 
 int64_t mentat_kernel_launch_count(void) { return (int64_t)mentat::g_kernel_launches.load(std::memory_order_relaxed); }
@@ -568,12 +691,14 @@ const char* mentat_status_string(int s) {
         case MENTAT_DEV_PLAN_OVERFLOW: return "decode plan workspace overflow";
         case MENTAT_DEV_TABLE_OVERFLOW: return "sequence table overflow";
         case MENTAT_DEV_DECODE_TIMEOUT: return "a bounded wait in a decode kernel gave up";
+        case MENTAT_DEV_BAD_SLOT: return "slot out of range, named twice or in use";
+        case MENTAT_DEV_BAD_TOKEN: return "kept position outside its sequence";
         case MENTAT_DEV_BAD_BLOCK: return "block table entry outside the pool";
         default: return "unknown status";
     }
 }
 
-int64_t mentat_kv_scratch_ints(int32_t max_seqs) { return 8 + 3 * (int64_t)max_seqs + 8; }
+int64_t mentat_kv_scratch_ints(int32_t max_seqs) { return 8 + 4 * (int64_t)max_seqs + 8; }
 
 int mentat_kv_init(const mentat_kv_cache* c, const int32_t* order, cudaStream_t s) {
     if (bad_cache(c)) return MENTAT_ERR_ARG;
@@ -647,6 +772,36 @@ int mentat_kv_append(const mentat_kv_cache* c, int32_t layer, int32_t slot, int3
                                             (const uint8_t*)v, v_stride * esz);
     MENTAT_CHECK_LAUNCH();
     return MENTAT_OK;
+}
+
+int mentat_kv_append_rotated_batched(const mentat_kv_cache* c, int32_t layer, const int32_t* slots, int32_t n,
+                                     const mentat_rows* q, const mentat_rows* qo, const mentat_rows* k,
+                                     const mentat_rows* v, const int64_t* positions, const mentat_rotary* r,
+                                     cudaStream_t s) {
+    AppendRotaryArgs a;
+    bool wide;
+    if (bad_cache(c) || layer < 0 || layer >= c->num_layers || n < 0 || n > 1024 || n > c->max_seqs ||
+        (n > 0 && !slots) || !c->k_pool || !c->v_pool || !append_rotary_args(c, q, qo, k, v, positions, r, &a, &wide))
+        return MENTAT_ERR_ARG;
+    if (c->dtype != MENTAT_F32 && c->dtype != MENTAT_BF16 && c->dtype != MENTAT_F16) return MENTAT_ERR_UNSUPPORTED;
+    if (n == 0) return MENTAT_OK;
+    MENTAT_LAUNCH(k_append_plan, dim3(1), dim3(((n + 31) / 32) * 32), 2 * n * sizeof(int), s, *c, layer, slots, n);
+    return rotary_dispatch(c->dtype, wide, r->interleaved != 0, LaunchAppendRotary{*c, layer, -1, n, a, s});
+}
+
+int mentat_kv_append_rotated(const mentat_kv_cache* c, int32_t layer, int32_t slot, int32_t n, const mentat_rows* q,
+                             const mentat_rows* qo, const mentat_rows* k, const mentat_rows* v,
+                             const int64_t* positions, const mentat_rotary* r, cudaStream_t s) {
+    AppendRotaryArgs a;
+    bool wide;
+    if (bad_cache(c) || layer < 0 || layer >= c->num_layers || slot < 0 || slot >= c->max_seqs || n < 0 ||
+        !c->k_pool || !c->v_pool || !append_rotary_args(c, q, qo, k, v, positions, r, &a, &wide))
+        return MENTAT_ERR_ARG;
+    if (c->dtype != MENTAT_F32 && c->dtype != MENTAT_BF16 && c->dtype != MENTAT_F16) return MENTAT_ERR_UNSUPPORTED;
+    if (n == 0) return MENTAT_OK;
+    k_append_multi_plan<<<1, MULTI_PLAN_THREADS, 0, s>>>(*c, layer, slot, n);
+    MENTAT_CHECK_LAUNCH();
+    return rotary_dispatch(c->dtype, wide, r->interleaved != 0, LaunchAppendRotary{*c, layer, slot, n, a, s});
 }
 
 int mentat_kv_trim(const mentat_kv_cache* c, int32_t slot, int32_t window, cudaStream_t s) {

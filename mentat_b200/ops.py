@@ -20,6 +20,7 @@ import ctypes as C
 import itertools
 import math
 import weakref
+from typing import Optional
 
 import torch
 
@@ -96,6 +97,8 @@ def _append_batched(k_pool: torch.Tensor, v_pool: torch.Tensor, slots: torch.Ten
             mgr._descp, layer, slots.data_ptr() + 4 * a, b - a,
             k.data_ptr() + a * ks * k.element_size(), ks,
             v.data_ptr() + a * vs * v.element_size(), vs, stream), "append_tokens_batched")
+    if mgr.page_index is not None:
+        _index_tails(mgr, layer, slots, n)
 
 
 append_batched_op = torch.library.custom_op("mentat_b200::append_batched", mutates_args=("k_pool", "v_pool"),
@@ -208,3 +211,333 @@ def prune_similar(sim: torch.Tensor, group_off: torch.Tensor, parent_key: torch.
                                         group_off.numel() - 1, max_group, parent_key.data_ptr(), logp.data_ptr(),
                                         thr, out.data_ptr(), stream), "mentat_prune_similar")
     return out
+
+
+# ---------------------------------------------------------------------------
+# rotary positions, pages, sparse decode
+# ---------------------------------------------------------------------------
+def _call(device, what: str, fn, *args) -> None:
+    """``fn(*args, stream)`` on the device's current torch stream, with the device current."""
+    if device.type != "cuda":
+        raise RuntimeError("mentat_b200 runs on CUDA devices only")
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+    else:
+        _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+
+
+_NO_ROWS = C.byref(_lib.Rows())
+
+
+def _row_ref(t: torch.Tensor):
+    return C.byref(_lib.Rows(t.data_ptr(), t.stride(0), t.stride(1), t.shape[1]))
+
+
+def _check_rows(name: str, t: torch.Tensor, n: int, d: int, dtype, device) -> torch.Tensor:
+    if t.dim() != 3 or t.shape[0] != n or t.shape[2] != d:
+        raise ValueError(f"{name} {tuple(t.shape)} is not ({n}, heads, {d})")
+    if t.dtype != dtype or dtype not in _DT:
+        raise TypeError(f"{name} has dtype {t.dtype}, {dtype if dtype in _DT else 'float32, bfloat16 or float16'} expected")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, {device} expected")
+    return t if t.stride(2) == 1 or d == 1 else t.contiguous()
+
+
+def _out_rows(name: str, out: Optional[torch.Tensor], x: torch.Tensor) -> torch.Tensor:
+    """``out`` checked as the result of a row operation on ``x``: its own rows distinct, and
+    either ``x`` itself or apart from it; a new tensor if None."""
+    if out is None:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    n, h, d = x.shape
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise ValueError(f"{name} must have the input's shape, dtype and device")
+    if x.numel() == 0:
+        return out
+    s0, s1 = out.stride(0), out.stride(1)
+    if (d > 1 and out.stride(2) != 1) or not (
+            ((h == 1 or s1 >= d) and (n == 1 or s0 >= (h - 1) * s1 * (h > 1) + d)) or
+            ((n == 1 or s0 >= d) and (h == 1 or s1 >= (n - 1) * s0 * (n > 1) + d))):
+        raise ValueError(f"{name} must hold rows of its own, each contiguous")
+    if out.data_ptr() == x.data_ptr() and out.stride() == x.stride():
+        return out
+
+    def span(t):
+        a = t.data_ptr()
+        return a, a + t.element_size() * (sum((m - 1) * s for m, s in zip(t.shape, t.stride())) + 1)
+    (a0, a1), (b0, b1) = span(out), span(x)
+    if a0 < b1 and b0 < a1:
+        raise ValueError(f"{name} must be the input itself or not overlap it")
+    return out
+
+
+def _check_positions(positions: torch.Tensor, n: int, device) -> torch.Tensor:
+    if positions.shape != (n,) or positions.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"positions must be {n} int64 or int32 values")
+    if positions.device != device:
+        raise ValueError(f"positions are on {positions.device}, {device} expected")
+    return positions.to(torch.int64).contiguous()
+
+
+def _check_rotary(rotary, d: int, device) -> None:
+    if rotary.head_dim != d:
+        raise ValueError(f"the rotary is for heads of {rotary.head_dim}, not {d}")
+    if rotary.device != device:
+        raise ValueError(f"the rotary is on {rotary.device}, {device} expected")
+
+
+def _check_ids(name: str, t: torch.Tensor, device, n: Optional[int] = None, limit: Optional[int] = None) -> torch.Tensor:
+    if t.dim() != 1 or t.dtype != torch.int32 or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{name} must be a vector of {'' if n is None else str(n) + ' '}int32 values")
+    if t.device != device:
+        raise ValueError(f"{name} are on {t.device}, {device} expected")
+    if limit is not None and t.shape[0] > limit:
+        raise ValueError(f"{name}: {t.shape[0]} in one call, at most {limit}")
+    return t.contiguous()
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, rotary, *, inverse: bool = False,
+           q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None) -> tuple:
+    """Turns ``q`` (N, Hq, D) and ``k`` (N, Hkv, D; may be None) to ``positions`` (N,)
+    (``Rotary``); ``inverse`` turns back, which is also the gradient of the turn.
+    Returns (q, k): new tensors, or ``q_out`` / ``k_out``, which may be the inputs
+    themselves.  Any token and head strides; wraps ``mentat_rotary_apply``."""
+    n, _, d = q.shape
+    q = _check_rows("q", q, n, d, q.dtype, q.device)
+    _check_rotary(rotary, d, q.device)
+    positions = _check_positions(positions, n, q.device)
+    qo = _out_rows("q_out", q_out, q)
+    ko = None
+    if k is not None:
+        k = _check_rows("k", k, n, d, q.dtype, q.device)
+        ko = _out_rows("k_out", k_out, k)
+    if n:
+        _call(q.device, "mentat_rotary_apply", _lib.load().mentat_rotary_apply, _DT[q.dtype], d, n, _row_ref(q),
+              _row_ref(qo), _NO_ROWS if k is None else _row_ref(k), _NO_ROWS if k is None else _row_ref(ko),
+              positions.data_ptr(), rotary._refs[bool(inverse)])
+    return qo, ko
+
+
+def rotary_append(cache, layer: int, rows: torch.Tensor, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
+                  positions: torch.Tensor, rotary, *, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Turns ``q`` (N, Hq, D; may be None) and ``k`` (N, Hkv, D) to ``positions`` (N,) and
+    writes the keys and ``v`` into rows ``rows`` (N,) int64 of layer ``layer``
+    of ``cache`` (a manager or a ``KVCacheView``): block * block_size + offset,
+    distinct; -1 writes none.  Returns the turned queries.  The tables and lengths
+    are not touched; ``PagedKVCacheManager.append_rotated`` keeps them.  Wraps
+    ``mentat_rotary_append``."""
+    n, _, d = k.shape
+    dev = cache.device
+    if d != cache.head_dim or k.shape[1] != cache.num_key_value_heads or v.shape[1] != k.shape[1]:
+        raise ValueError("k or v shape does not match the cache geometry")
+    if not 0 <= layer < cache.num_layers:
+        raise ValueError(f"layer {layer} is not within 0 .. {cache.num_layers - 1}")
+    k, v = _check_rows("k", k, n, d, cache.dtype, dev), _check_rows("v", v, n, d, cache.dtype, dev)
+    _check_rotary(rotary, d, dev)
+    positions = _check_positions(positions, n, dev)
+    if rows.shape != (n,) or rows.dtype != torch.int64 or rows.device != dev:
+        raise ValueError(f"rows must be {n} int64 values on {dev}")
+    rows = rows.contiguous()
+    qo = None
+    if q is not None:
+        q = _check_rows("q", q, n, d, cache.dtype, dev)
+        qo = _out_rows("q_out", q_out, q)
+    if n:
+        _call(dev, "mentat_rotary_append", _lib.load().mentat_rotary_append, cache._descp, layer, n, rows.data_ptr(),
+              _NO_ROWS if q is None else _row_ref(q), _NO_ROWS if q is None else _row_ref(qo), _row_ref(k), _row_ref(v),
+              positions.data_ptr(), rotary._refs[0])
+    return qo
+
+
+def _append_rotated(k_pool: torch.Tensor, v_pool: torch.Tensor, slots: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                    v: torch.Tensor, cache: int, layer: int, rotary: int) -> torch.Tensor:
+    """``append_batched`` with ``q`` (N, Hq, D) and ``k`` turned to the index of their
+    token in its sequence; returns the turned queries.  ``rotary`` is the id that
+    ``register_cache`` gave a ``Rotary``.  Wraps ``mentat_kv_append_rotated_batched``."""
+    mgr, rot = _cache(cache), _cache(rotary)
+    lib = _lib.load()
+    n, d = k.shape[0], k.shape[2]
+    dev = mgr.device
+    q, k, v = (_check_rows(name, t, n, d, mgr.dtype, dev) for name, t in (("q", q), ("k", k), ("v", v)))
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    for a in range(0, n, 1024):
+        b = min(n, a + 1024)
+        _call(dev, "append_rotated_batched", lib.mentat_kv_append_rotated_batched, mgr._descp, layer,
+              slots.data_ptr() + 4 * a, b - a, _row_ref(q[a:b]), _row_ref(qo[a:b]), _row_ref(k[a:b]), _row_ref(v[a:b]),
+              None, rot._refs[0])
+    if mgr.page_index is not None:
+        _index_tails(mgr, layer, slots, n)
+    return qo
+
+
+append_rotated_op = torch.library.custom_op("mentat_b200::append_rotated", mutates_args=("k_pool", "v_pool"),
+                                            device_types="cuda")(_append_rotated)
+
+
+@append_rotated_op.register_fake
+def _append_rotated_fake(k_pool, v_pool, slots, q, k, v, cache, layer, rotary):
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
+def append_rotated(k_pool, v_pool, slots, q, k, v, cache, layer, rotary):
+    if torch.compiler.is_compiling():
+        return torch.ops.mentat_b200.append_rotated(k_pool, v_pool, slots, q, k, v, cache, layer, rotary)
+    return _append_rotated(k_pool, v_pool, slots, q, k, v, cache, layer, rotary)
+
+
+def _index_tails(mgr, layer: int, slots: torch.Tensor, n: int) -> None:
+    """Indexes each sequence's last page, if it is full (after a batched append)."""
+    _call(mgr.device, "mentat_page_index_seqs", _lib.load().mentat_page_index_seqs, mgr._descp, layer, slots.data_ptr(),
+          n, -1, 1, mgr.page_index._ref)
+
+
+def index_sequences(mgr, slots: torch.Tensor, first_page: int, max_pages: int, layer: int = -1) -> None:
+    """Indexes the full pages ``first_page .. first_page + max_pages`` of the slots' sequences
+    in ``layer`` (-1: every layer) into the cache's index.  Wraps ``mentat_page_index_seqs``."""
+    step = max(1, 0x7fffffff // max(1, max_pages))
+    for a in range(0, slots.shape[0], step):
+        part = slots[a: a + step]
+        _call(mgr.device, "mentat_page_index_seqs", _lib.load().mentat_page_index_seqs, mgr._descp, layer,
+              part.data_ptr(), part.shape[0], first_page, max_pages, mgr.page_index._ref)
+
+
+def _workspace(cache, n: int) -> tuple:
+    size = int(_lib.load().mentat_pages_workspace_bytes(cache._descp, n))
+    return torch.empty(size, dtype=torch.uint8, device=cache.device), size
+
+
+MAX_SEQS_PER_PAGES_CALL = 1024
+
+
+def fork_pages(cache, parents: torch.Tensor, children: torch.Tensor, max_blocks: Optional[int] = None) -> None:
+    """Every layer's table of slot ``parents[i]`` into slot ``children[i]``, with a
+    reference on each page (int32 slots on the device; the children distinct, empty
+    and no parents).  ``max_blocks``: the longest parent's table, a launch-size hint.
+    ``PagedKVCacheManager.fork_sequences`` keeps the host's mirror too.  Wraps
+    ``mentat_kv_fork_batched``."""
+    dev = cache.device
+    parents = _check_ids("parents", parents, dev, limit=MAX_SEQS_PER_PAGES_CALL)
+    children = _check_ids("children", children, dev, parents.shape[0])
+    hint = cache.table_capacity if max_blocks is None else max_blocks
+    _call(dev, "fork_pages", _lib.load().mentat_kv_fork_batched, cache._descp, parents.data_ptr(), children.data_ptr(),
+          parents.shape[0], hint)
+
+
+def free_pages(cache, slots: torch.Tensor, max_blocks: Optional[int] = None) -> None:
+    """Releases every page of the (distinct) slots, as freeing them one after another
+    would, the order of the free list included.  Wraps ``mentat_kv_free_batched``."""
+    dev = cache.device
+    slots = _check_ids("slots", slots, dev, limit=MAX_SEQS_PER_PAGES_CALL)
+    hint = cache.table_capacity if max_blocks is None else max_blocks
+    ws, size = _workspace(cache, slots.shape[0])
+    _call(dev, "free_pages", _lib.load().mentat_kv_free_batched, cache._descp, slots.data_ptr(), slots.shape[0], hint,
+          ws.data_ptr(), size)
+
+
+def compact_pages(cache, src: torch.Tensor, dst: Optional[torch.Tensor], keep: torch.Tensor, cu: torch.Tensor,
+                  max_keep: int, *, rotary=None, max_blocks: Optional[int] = None) -> None:
+    """Sequence ``src[i]`` reduced to its positions ``keep[cu[i]:cu[i + 1]]``, which become
+    positions 0, 1, ...: in place if ``dst`` is None, else as a new sequence in the
+    empty slot ``dst[i]`` that shares the full pages at the front whose tokens stay
+    where they are.  ``keep`` (total,) int32, or (layers, total) with a choice for each
+    layer; ``cu`` (n + 1,) int32; ``max_keep`` the longest list.  With ``rotary``
+    the keys are turned from their old position to the new one.
+    ``PagedKVCacheManager.compact_sequences`` keeps the host's mirror too.  Wraps
+    ``mentat_kv_compact``."""
+    dev = cache.device
+    src = _check_ids("src", src, dev, limit=MAX_SEQS_PER_PAGES_CALL)
+    n = src.shape[0]
+    dst = None if dst is None else _check_ids("dst", dst, dev, n)
+    cu = _check_ids("cu", cu, dev, n + 1)
+    if keep.dtype != torch.int32 or keep.device != dev or keep.dim() not in (1, 2) or \
+            (keep.dim() == 2 and keep.shape[0] not in (1, cache.num_layers)):
+        raise ValueError(f"keep must be int32 on {dev}, (total,) or (layers, total)")
+    if keep.stride(-1) != 1:
+        keep = keep.contiguous()
+    per_layer = keep.dim() == 2 and keep.shape[0] > 1
+    if rotary is not None:
+        _check_rotary(rotary, cache.head_dim, dev)
+    hint = cache.table_capacity if max_blocks is None else max_blocks
+    ws, size = _workspace(cache, n)
+    _call(dev, "compact_pages", _lib.load().mentat_kv_compact, cache._descp, src.data_ptr(),
+          None if dst is None else dst.data_ptr(), n, keep.data_ptr(), keep.stride(0) if per_layer else 0,
+          cu.data_ptr(), max_keep, hint, None if rotary is None else rotary._refs[0], ws.data_ptr(), size)
+
+
+def page_index(index, layer: int, blocks: torch.Tensor) -> None:
+    """Indexes ``blocks`` (n,) int32 of layer ``layer`` from every row of each.  A
+    manager's own index (``enable_page_index``) is kept by its appends.  Wraps
+    ``mentat_page_index_blocks``."""
+    c = index.cache
+    blocks = _check_ids("blocks", blocks, c.device)
+    _call(c.device, "page_index", _lib.load().mentat_page_index_blocks, c._descp, layer, blocks.data_ptr(),
+          blocks.shape[0], index._ref)
+
+
+def page_bounds(index, layer: int, blocks: torch.Tensor) -> tuple:
+    """What the index holds for ``blocks`` (n,): ``(low, high, exps)``, the bounds of their
+    keys as float32 (n, Hkv, D) and their exponents int8 (n, Hkv).  Wraps
+    ``mentat_page_bounds``."""
+    c = index.cache
+    blocks = _check_ids("blocks", blocks, c.device)
+    n, h, d = blocks.shape[0], c.num_key_value_heads, c.head_dim
+    both = torch.empty((2, n, h, d), device=c.device)
+    exps = torch.empty((n, h), dtype=torch.int8, device=c.device)
+    _call(c.device, "page_bounds", _lib.load().mentat_page_bounds, c._descp, layer, blocks.data_ptr(), n, index._ref,
+          both[0].data_ptr(), both[1].data_ptr(), exps.data_ptr())
+    return both[0], both[1], exps
+
+
+def sparse_decode(index, layer: int, slots: torch.Tensor, q: torch.Tensor, max_len: int, budget: int, *, sink: int = 1,
+                  recent: int = 1, scale: Optional[float] = None, return_pages: bool = False):
+    """Decode attention of ``q`` (N, Hq, D) over at most ``budget`` pages of each of the
+    sequences in ``slots`` (N,) int32, chosen for each KV head by the scores of
+    ``index`` (``PageIndex``): the first ``sink`` and last ``recent`` always, then the
+    highest.  ``max_len``: the longest of the lengths.  Returns (N, Hq, D), with
+    ``return_pages`` also the chosen pages, int32 (N, Hkv, budget), rising, then -1.
+    Wraps ``mentat_sparse_decode``."""
+    c = index.cache
+    n, hq, d = q.shape
+    if d != c.head_dim or hq % c.num_key_value_heads:
+        raise ValueError("q shape does not match the cache geometry")
+    q = _check_rows("q", q, n, d, c.dtype, c.device)
+    if q.stride(1) != d:
+        q = q.contiguous()
+    slots = _check_ids("slots", slots, c.device, n)
+    if recent < 1 or sink < 0 or sink + recent > budget:
+        raise ValueError(f"sink {sink} >= 0 and recent {recent} >= 1 pages must fit in the budget of {budget}")
+    out = torch.empty((n, hq, d), device=q.device, dtype=q.dtype)
+    pages = torch.empty((n, c.num_key_value_heads, budget), dtype=torch.int32, device=q.device) if return_pages else None
+    if n:
+        _call(c.device, "mentat_sparse_decode", _lib.load().mentat_sparse_decode, c._descp, layer, index._ref,
+              slots.data_ptr(), n, q.data_ptr(), q.stride(0), hq, out.data_ptr(), out.stride(0),
+              default_scale(d) if scale is None else scale, max_len, budget, sink, recent,
+              None if pages is None else pages.data_ptr())
+    return (out, pages) if return_pages else out
+
+
+def _paged_sparse_decode(q: torch.Tensor, slots: torch.Tensor, max_len: int, cache: int, layer: int, scale: float,
+                         budget: int, sink: int, recent: int) -> torch.Tensor:
+    """``sparse_decode`` over a manager's own index, the cache given by its id."""
+    return sparse_decode(_index_of(_cache(cache)), layer, slots, q, max_len, budget, sink=sink, recent=recent, scale=scale)
+
+
+def _index_of(mgr):
+    if mgr.page_index is None:
+        raise RuntimeError("the cache has no page index: call enable_page_index() first")
+    return mgr.page_index
+
+
+paged_sparse_decode_op = torch.library.custom_op("mentat_b200::paged_sparse_decode", mutates_args=(),
+                                                 device_types="cuda")(_paged_sparse_decode)
+
+
+@paged_sparse_decode_op.register_fake
+def _paged_sparse_decode_fake(q, slots, max_len, cache, layer, scale, budget, sink, recent):
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
+def paged_sparse_decode(q, slots, max_len, cache, layer, scale, budget, sink, recent):
+    if torch.compiler.is_compiling():
+        return torch.ops.mentat_b200.paged_sparse_decode(q, slots, max_len, cache, layer, scale, budget, sink, recent)
+    return _paged_sparse_decode(q, slots, max_len, cache, layer, scale, budget, sink, recent)

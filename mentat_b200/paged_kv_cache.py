@@ -172,6 +172,116 @@ class _PinnedRing:
         return dev
 
 
+def raise_device_error(err: int, arg: int, max_blocks: int, max_blocks_per_seq: int) -> None:
+    """The exception of a recorded device error (reference exception types)."""
+    if err == 0:
+        return
+    if err == _lib.DEV_OUT_OF_BLOCKS:
+        raise RuntimeError(OUT_OF_BLOCKS_MSG.format(n=max_blocks))
+    if err == _lib.DEV_REF_FREE:
+        raise AssertionError(f"ref() on free block {arg}")
+    if err == _lib.DEV_RELEASE_FREE:
+        raise AssertionError(f"release() on free block {arg}")
+    if err == _lib.DEV_TABLE_OVERFLOW:
+        raise RuntimeError(f"PagedKVCache: sequence table overflow (slot {arg}, "
+                           f"max_blocks_per_seq={max_blocks_per_seq})")
+    if err == _lib.DEV_PLAN_OVERFLOW:
+        raise RuntimeError("mentat_b200: decode plan workspace overflow")
+    if err == _lib.DEV_BAD_BLOCK:
+        raise AssertionError(f"block table entry {arg} outside the pool (max_blocks={max_blocks})")
+    if err == _lib.DEV_BAD_SLOT:
+        raise ValueError(f"sequence slot {arg} is out of range, named twice in one call or in use")
+    if err == _lib.DEV_BAD_TOKEN:
+        raise IndexError(f"kept position {arg} is outside its sequence")
+    if err == _lib.DEV_DECODE_TIMEOUT:
+        raise RuntimeError(f"mentat_b200: a decode kernel's bounded wait gave up (stage {arg}); "
+                           "that call's output is invalid")
+    raise RuntimeError(f"mentat_b200 device error {err} ({arg})")
+
+
+class KVCacheView:
+    """A paged cache over tensors that the caller owns, for the functions of
+    ``mentat_b200.ops`` that take a cache: ``k_pool`` and ``v_pool`` (layers, blocks,
+    block_size, Hkv, D), ``tables`` (layers, sequences, capacity) int32 block ids and
+    ``ntok`` (layers, sequences) int32 lengths; for the functions that allocate or
+    release pages also ``nblocks`` and ``tail`` (as ``ntok``), ``refcounts`` and
+    ``free_ring`` (blocks,) int32 and the allocator's control words ``ctrl`` (16,)
+    int64.  What is not given is made (control words, for errors) or absent
+    (``tables`` and ``ntok``; a function that needs them refuses)."""
+
+    def __init__(self, k_pool: torch.Tensor, v_pool: torch.Tensor, tables: torch.Tensor | None = None,
+                 ntok: torch.Tensor | None = None, *, nblocks=None, tail=None, refcounts=None, free_ring=None,
+                 ctrl=None):
+        if k_pool.dim() != 5 or v_pool.shape != k_pool.shape or v_pool.dtype != k_pool.dtype or \
+                not (k_pool.is_contiguous() and v_pool.is_contiguous()):
+            raise ValueError("k_pool and v_pool must be contiguous (layers, blocks, block_size, Hkv, D) of one shape and dtype")
+        if k_pool.dtype not in _DTYPES:
+            raise TypeError(f"unsupported cache dtype {k_pool.dtype}")
+        if k_pool.device.type != "cuda" or v_pool.device != k_pool.device:
+            raise ValueError("k_pool and v_pool must be on one CUDA device")
+        self.device, self.dtype = k_pool.device, k_pool.dtype
+        self.num_layers, self.max_blocks, self.block_size, self.num_key_value_heads, self.head_dim = k_pool.shape
+        if ctrl is None:
+            ctrl = torch.zeros(_lib.CTRL_WORDS, dtype=torch.int64, device=self.device)
+        if (tables is None) != (ntok is None):
+            raise ValueError("tables and ntok go together")
+        per_seq = None if ntok is None else tuple(ntok.shape)
+        shapes = {"tables": None, "ntok": per_seq, "nblocks": per_seq, "tail": per_seq,
+                  "refcounts": (self.max_blocks,), "free_ring": (self.max_blocks,), "ctrl": (_lib.CTRL_WORDS,)}
+        given = {"tables": tables, "ntok": ntok, "nblocks": nblocks, "tail": tail, "refcounts": refcounts,
+                 "free_ring": free_ring, "ctrl": ctrl}
+        for name, t in given.items():
+            if t is None:
+                continue
+            want = torch.int64 if name == "ctrl" else torch.int32
+            if t.dtype != want or t.device != self.device or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous {want} on {self.device}")
+            if shapes[name] is not None and tuple(t.shape) != shapes[name]:
+                raise ValueError(f"{name} {tuple(t.shape)} must be {shapes[name]}")
+            if name in ("nblocks", "tail") and per_seq is None:
+                raise ValueError(f"{name} needs tables and ntok")
+        if tables is not None and (tables.dim() != 3 or tables.shape[0] != self.num_layers or
+                                   tuple(tables.shape[:2]) != per_seq):
+            raise ValueError("tables must be (layers, sequences, capacity) and ntok (layers, sequences)")
+        self._tensors = dict(given, k_pool=k_pool, v_pool=v_pool)  # keeps them alive
+        self.max_seqs, self.table_capacity = (0, 0) if tables is None else tuple(tables.shape[1:])
+        d = _lib.KVCache()
+        d.num_layers, d.num_blocks, d.block_size = self.num_layers, self.max_blocks, self.block_size
+        d.num_kv_heads, d.head_dim, d.dtype = self.num_key_value_heads, self.head_dim, _DTYPES[self.dtype]
+        d.max_seqs, d.max_blocks_per_seq = self.max_seqs, self.table_capacity
+        for name, t in self._tensors.items():
+            setattr(d, name, None if t is None else t.data_ptr())
+        self._desc, self._descp = d, C.byref(d)
+        self.page_index = None
+
+    def check(self) -> None:
+        """Raise the first error the device recorded (waits for the device)."""
+        c = self._tensors["ctrl"].tolist()
+        raise_device_error(c[_lib.CTRL_ERROR], c[_lib.CTRL_ERRARG], self.max_blocks, self.table_capacity)
+
+
+class PageIndex:
+    """Bounds of every page's keys in 8 bits, from which ``ops.sparse_decode`` and
+    ``attention_backend.attn_decode_sparse`` choose pages: ``bounds`` int8 (layers,
+    blocks, Hkv, 2, D), lowest and highest key of each channel in units of 2**exps,
+    and ``exps`` int8 (layers, blocks, Hkv).  A page that was never indexed is chosen
+    before all others."""
+
+    def __init__(self, cache, *, bounds: torch.Tensor | None = None, exps: torch.Tensor | None = None):
+        shape = (cache.num_layers, cache.max_blocks, cache.num_key_value_heads)
+        dev = cache.device
+        if bounds is None:
+            bounds = torch.zeros(shape + (2, cache.head_dim), dtype=torch.int8, device=dev)
+        if exps is None:
+            exps = torch.full(shape, 127, dtype=torch.int8, device=dev)
+        for name, t, want in (("bounds", bounds, shape + (2, cache.head_dim)), ("exps", exps, shape)):
+            if tuple(t.shape) != want or t.dtype != torch.int8 or t.device != dev or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous int8 {want} on {dev}")
+        self.cache, self.bounds, self.exps = cache, bounds, exps
+        self._desc = _lib.PageIndex(bounds.data_ptr(), exps.data_ptr())
+        self._ref = C.byref(self._desc)
+
+
 class PagedKVCacheManager:
     """``PagedKVCacheManager`` (``core/paged_kv_cache.py:102-455``) on the device."""
 
@@ -247,8 +357,13 @@ class PagedKVCacheManager:
         self._uploads = _PinnedRing(self.device)
         self._op_id = ops.register_cache(self)
         self._ws_bytes = 0
+        self.page_index: PageIndex | None = None
 
     # ------------------------------------------------------------------ util
+    @property
+    def table_capacity(self) -> int:
+        return self._table_stride
+
     def _s(self) -> int:
         return _stream(self.device)
 
@@ -261,25 +376,7 @@ class PagedKVCacheManager:
         """Raise the first error the device recorded (reference exception types)."""
         c = self._ctrl_host()
         err, arg = int(c[_lib.CTRL_ERROR]), int(c[_lib.CTRL_ERRARG])
-        if err == 0:
-            return
-        if err == _lib.DEV_OUT_OF_BLOCKS:
-            raise RuntimeError(OUT_OF_BLOCKS_MSG.format(n=self.max_blocks))
-        if err == _lib.DEV_REF_FREE:
-            raise AssertionError(f"ref() on free block {arg}")
-        if err == _lib.DEV_RELEASE_FREE:
-            raise AssertionError(f"release() on free block {arg}")
-        if err == _lib.DEV_TABLE_OVERFLOW:
-            raise RuntimeError(f"PagedKVCache: sequence table overflow (slot {arg}, "
-                               f"max_blocks_per_seq={self.max_blocks_per_seq})")
-        if err == _lib.DEV_PLAN_OVERFLOW:
-            raise RuntimeError("mentat_b200: decode plan workspace overflow")
-        if err == _lib.DEV_BAD_BLOCK:
-            raise AssertionError(f"block table entry {arg} outside the pool (max_blocks={self.max_blocks})")
-        if err == _lib.DEV_DECODE_TIMEOUT:
-            raise RuntimeError(f"mentat_b200: a decode kernel's bounded wait gave up (stage {arg}); "
-                               "that call's output is invalid")
-        raise RuntimeError(f"mentat_b200 device error {err} ({arg})")
+        raise_device_error(err, arg, self.max_blocks, self.max_blocks_per_seq)
 
     def clear_error(self) -> None:
         """Forget the recorded device error (after the caller has handled it)."""
@@ -344,6 +441,143 @@ class PagedKVCacheManager:
         self._cache.clear()
         self._after()
 
+    def fork_sequences(self, parent_ids) -> list:
+        """``[fork_sequence(p) for p in parent_ids]`` in one launch (a parent may occur
+        several times).  An unknown id or a lack of slots raises before any change."""
+        parents = [self._sequences[p] for p in parent_ids]
+        if len(parents) > len(self._free_slots):
+            raise RuntimeError(f"PagedKVCache: out of sequence slots (max_seqs={self.max_seqs})")
+        kids = []
+        for p in parents:
+            cid = self._next_seq_id
+            self._next_seq_id += 1
+            self._sequences[cid] = SequenceState(cid, self.num_layers, self._free_slots.pop(), list(p.num_tokens),
+                                                 list(p.tokens_in_last_block), list(p.num_blocks))
+            kids.append(cid)
+        for a in range(0, len(parents), ops.MAX_SEQS_PER_PAGES_CALL):
+            part = slice(a, a + ops.MAX_SEQS_PER_PAGES_CALL)
+            both = self._upload([p.slot for p in parents[part]] + [self._sequences[c].slot for c in kids[part]])
+            n = both.numel() // 2
+            ops.fork_pages(self, both[:n], both[n:], max(max(p.num_blocks) for p in parents[part]))
+        self._after()
+        return kids
+
+    def free_sequences(self, seq_ids) -> None:
+        """``free_sequence`` of every id, in that order, in one call.  An unknown id, or
+        one that occurs twice, raises before any change."""
+        ids = list(seq_ids)
+        seqs = [self._sequences[s] for s in ids]
+        if len(set(ids)) < len(ids):
+            raise KeyError(next(s for i, s in enumerate(ids) if s in ids[:i]))
+        for a in range(0, len(seqs), ops.MAX_SEQS_PER_PAGES_CALL):
+            part = seqs[a: a + ops.MAX_SEQS_PER_PAGES_CALL]
+            ops.free_pages(self, self._upload([s.slot for s in part]), max(max(s.num_blocks) for s in part))
+        for s in seqs:
+            del self._sequences[s.seq_id]
+            self._free_slots.append(s.slot)
+        self._cache.clear()
+        self._after()
+
+    def compact_sequences(self, seq_ids, keep, *, rotary=None, into_new: bool = False):
+        """Reduces each sequence to the positions ``keep[i]`` (a vector of indices in any
+        order, or one row of them for each layer), which become its positions 0, 1,
+        ...: eviction of cached tokens.  Full pages at the front whose tokens all stay
+        where they are (all pages, if every token stays) are not copied and stay
+        shared with other sequences; the others go to fresh blocks and the old pages are released.  With
+        ``into_new`` the sequences stay as they are and the result is a list of new
+        ones, which share those pages at the front.
+
+        ``rotary``: the :class:`~mentat_b200.Rotary` that the cached keys were turned
+        with.  It turns them on to their new positions, so that the next token's
+        position is again the sequence's length.  The keys are rounded once more.
+
+        An unknown or repeated id, or a position outside its sequence (on the host; a
+        device tensor is checked on the device), raises before any change."""
+        ids = list(seq_ids)
+        seqs = [self._sequences[s] for s in ids]
+        if len(keep) != len(ids):
+            raise ValueError(f"{len(ids)} sequences but {len(keep)} lists of positions")
+        if not into_new and len(set(ids)) < len(ids):
+            raise KeyError(next(s for i, s in enumerate(ids) if s in ids[:i]))
+        if into_new and len(ids) > len(self._free_slots):
+            raise RuntimeError(f"PagedKVCache: out of sequence slots (max_seqs={self.max_seqs})")
+        L, bs = self.num_layers, self.block_size
+        on_device = any(isinstance(k, torch.Tensor) and k.device.type != "cpu" for k in keep)
+        lists, counts, per_layer = [], [], False
+        for seq, k in zip(seqs, keep):
+            if on_device:
+                k = torch.as_tensor(k).to(device=self.device, dtype=torch.int32)
+                ndim, shape = k.dim(), tuple(k.shape)
+            else:
+                k = np.asarray(k)
+                if k.size == 0:
+                    k = k.astype(np.int64)
+                if k.dtype.kind not in "iu":
+                    raise TypeError("kept positions must be whole numbers")
+                ndim, shape = k.ndim, k.shape
+            if ndim not in (1, 2) or (ndim == 2 and shape[0] != L):
+                raise ValueError(f"kept positions {shape} must be (n,) or ({L}, n)")
+            if not on_device and k.size:
+                low = min(seq.num_tokens) if ndim == 1 else np.asarray(seq.num_tokens)[:, None]
+                bad = (k < 0) | (k >= low)
+                if bad.any():
+                    raise IndexError(f"kept position {k[bad].flat[0]} is outside sequence {seq.seq_id}")
+            m = shape[-1]
+            if -(-m // bs) > self.max_blocks_per_seq:
+                raise RuntimeError(f"PagedKVCache: sequence {seq.seq_id} needs {-(-m // bs)} blocks per layer, "
+                                   f"max_blocks_per_seq={self.max_blocks_per_seq}")
+            per_layer |= ndim == 2
+            lists.append(k)
+            counts.append(m)
+        out = []
+        for seq, m in zip(seqs, counts):
+            nb = -(-m // bs)
+            new = ([m] * L, [m - (nb - 1) * bs if m else 0] * L, [nb] * L)
+            if into_new:
+                cid = self._next_seq_id
+                self._next_seq_id += 1
+                self._sequences[cid] = SequenceState(cid, L, self._free_slots.pop(), *new)
+                out.append(cid)
+        step = ops.MAX_SEQS_PER_PAGES_CALL
+        for a in range(0, len(seqs), step):
+            part, ks, cs = seqs[a: a + step], lists[a: a + step], counts[a: a + step]
+            if per_layer:
+                ks = [k.expand(L, -1) if on_device and k.dim() == 1 else
+                      np.broadcast_to(k, (L, k.shape[-1])) if not on_device else k for k in ks]
+            flat = torch.cat(ks, dim=-1) if on_device else \
+                self._upload(np.concatenate(ks, axis=-1)).view((L, -1) if per_layer else (-1,))
+            slots = self._upload([s.slot for s in part])
+            dst = self._upload([self._sequences[c].slot for c in out[a: a + step]]) if into_new else None
+            cu = self._upload(np.concatenate([[0], np.cumsum(cs)]))
+            ops.compact_pages(self, slots, dst, flat, cu, max(cs), rotary=rotary,
+                              max_blocks=max(max(s.num_blocks) for s in part))
+            if self.page_index is not None and max(cs) >= bs:
+                ops.index_sequences(self, slots if dst is None else dst, 0, max(cs) // bs)
+        if not into_new:
+            for seq, m in zip(seqs, counts):
+                nb = -(-m // bs)
+                seq.num_tokens, seq.num_blocks = [m] * L, [nb] * L
+                seq.tokens_in_last_block = [m - (nb - 1) * bs if m else 0] * L
+        self._cache.clear()
+        self._after()
+        return out if into_new else None
+
+    def _upload(self, values) -> torch.Tensor:
+        return self._uploads.upload(np.ascontiguousarray(values, np.int32))
+
+    # ------------------------------------------------------------- page index
+    def enable_page_index(self) -> PageIndex:
+        """The cache's :class:`PageIndex`: made at the first call, from the pages of
+        every live sequence, and from then on kept by every append, trim and
+        compaction of this class (a page is indexed when it is full)."""
+        if self.page_index is None:
+            self.page_index = PageIndex(self)
+            live = list(self._sequences.values())
+            pages = max((max(s.num_tokens) // self.block_size for s in live), default=0)
+            if pages:
+                ops.index_sequences(self, self._upload([s.slot for s in live]), 0, pages)
+        return self.page_index
+
     # ----------------------------------------------------------------- append
     def _rows(self, t: torch.Tensor, n: int):
         if t.dtype != self.dtype:
@@ -406,10 +640,68 @@ class PagedKVCacheManager:
             return
         k, ks = self._rows(k, n)
         v, vs = self._rows(v, n)
+        first = seq.num_tokens[layer_idx]
         self._mirror_append(seq, layer_idx, n)
         _lib.check(self._lib.mentat_kv_append(self._descp, layer_idx, seq.slot, n, k.data_ptr(), ks,
                                               v.data_ptr(), vs, self._s()), "append_tokens")
+        self._index_appended(seq, layer_idx, first)
         self._after()
+
+    def append_rotated(self, seq_id: int, layer_idx: int, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
+                       rotary, positions: torch.Tensor | None = None) -> torch.Tensor | None:
+        """``append_tokens`` of n tokens with ``k`` (n, Hkv, D) and ``q`` (n, Hq, D; may be
+        None) turned (:class:`~mentat_b200.Rotary`) to each token's index in its
+        sequence, or to ``positions`` (n,) int64; returns the turned queries."""
+        seq = self._sequences[seq_id]
+        n, d = k.shape[0], self.head_dim
+        k, v = (ops._check_rows(name, t, n, d, self.dtype, self.device) for name, t in (("k", k), ("v", v)))
+        if k.shape[1] != self.num_key_value_heads or v.shape[1] != self.num_key_value_heads:
+            raise ValueError("k or v shape does not match the cache geometry")
+        ops._check_rotary(rotary, d, self.device)
+        if positions is not None:
+            positions = ops._check_positions(positions, n, self.device)
+        qo = None
+        if q is not None:
+            q = ops._check_rows("q", q, n, d, self.dtype, self.device)
+            qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if n == 0:
+            return qo
+        first = seq.num_tokens[layer_idx]
+        self._mirror_append(seq, layer_idx, n)
+        none = ops._NO_ROWS
+        ops._call(self.device, "append_rotated", self._lib.mentat_kv_append_rotated, self._descp, layer_idx, seq.slot, n,
+                  none if q is None else ops._row_ref(q), none if q is None else ops._row_ref(qo), ops._row_ref(k),
+                  ops._row_ref(v), None if positions is None else positions.data_ptr(), rotary._refs[0])
+        self._index_appended(seq, layer_idx, first)
+        self._after()
+        return qo
+
+    def append_rotated_batched(self, seq_ids, layer_idx: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                               rotary) -> torch.Tensor:
+        """``append_tokens_batched`` with ``k`` and ``q`` (N, Hq, D) turned to each token's
+        index in its sequence; returns the turned queries."""
+        N = len(seq_ids)
+        seqs = [self._sequences[s] for s in seq_ids]  # an unknown id raises before any change
+        q, k, v = (ops._check_rows(name, t, N, self.head_dim, self.dtype, self.device)
+                   for name, t in (("q", q), ("k", k), ("v", v)))
+        if k.shape[1] != self.num_key_value_heads or v.shape[1] != self.num_key_value_heads:
+            raise ValueError("k or v shape does not match the cache geometry")
+        ops._check_rotary(rotary, self.head_dim, self.device)
+        if N == 0:
+            return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        self._mirror_append_batched(seqs, layer_idx)
+        out = ops.append_rotated(self._k_all, self._v_all, self._slots_dev(seq_ids), q, k, v, self._op_id, layer_idx,
+                                 rotary.op_id)
+        self._after()
+        return out
+
+    def _index_appended(self, seq: SequenceState, layer: int, first: int) -> None:
+        """After an append to a sequence that had ``first`` tokens: its newly full pages."""
+        if self.page_index is not None:
+            bs = self.block_size
+            p0, p1 = first // bs, seq.num_tokens[layer] // bs
+            if p1 > p0:
+                ops.index_sequences(self, self._slots_dev([seq.seq_id]), p0, p1 - p0, layer)
 
     def append_tokens_batched(self, seq_ids, layer_idx: int, k: torch.Tensor, v: torch.Tensor) -> None:
         N = len(seq_ids)                                    # :227-284
@@ -418,6 +710,12 @@ class PagedKVCacheManager:
         seqs = [self._sequences[s] for s in seq_ids]  # an unknown id raises before any change
         k, ks = self._rows(k, N)
         v, vs = self._rows(v, N)
+        self._mirror_append_batched(seqs, layer_idx)
+        slots = self._slots_dev(seq_ids)
+        ops.append_batched(self._k_all, self._v_all, slots, k, v, self._op_id, layer_idx)
+        self._after()
+
+    def _mirror_append_batched(self, seqs, layer_idx: int) -> None:
         # host mirror of one token per sequence, inline (this runs for every layer of
         # every decode step); the general walk only where a new block would overflow
         bs, cap, L = self.block_size, self.max_blocks_per_seq, layer_idx
@@ -430,9 +728,6 @@ class PagedKVCacheManager:
             else:
                 s.tokens_in_last_block[L] = tf + 1
             s.num_tokens[L] += 1
-        slots = self._slots_dev(seq_ids)
-        ops.append_batched(self._k_all, self._v_all, slots, k, v, self._op_id, layer_idx)
-        self._after()
 
     def get_kv_length(self, seq_id: int) -> int:            # :285-287
         return self._sequences[seq_id].num_tokens[0]
@@ -543,6 +838,8 @@ class PagedKVCacheManager:
             t = window_size % bs
             seq.tokens_in_last_block[layer] = 0 if window_size == 0 else (t if t else bs)
         _lib.check(self._lib.mentat_kv_trim(self._descp, seq.slot, window_size, self._s()), "trim_to_window")
+        if self.page_index is not None and window_size >= bs:
+            ops.index_sequences(self, self._slots_dev([seq_id]), 0, window_size // bs)
         self._cache.clear()
         self._after()
 

@@ -37,9 +37,10 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib, ops
-from .attention_backend import attn_decode
+from .attention_backend import attn_decode, attn_decode_sparse
 from .gate import Gate, GateConfig
 from .paged_kv_cache import PagedKVCacheManager
+from .rotary import Rotary
 
 
 # ---------------------------------------------------------------------------
@@ -115,8 +116,10 @@ class Tree:
 
     def branch(self, leaf: Node, tokens, log_probs) -> list:                   # :102-138
         kids = []
-        for t, lp in zip(tokens, log_probs):
-            child = Node(node_id=self.new_id(), token_ids=[int(t)], seq_id=self.cache.fork_sequence(leaf.seq_id),
+        tokens, log_probs = list(tokens), list(log_probs)
+        forks = self.cache.fork_sequences([leaf.seq_id] * min(len(tokens), len(log_probs)))
+        for t, lp, sid in zip(tokens, log_probs, forks):
+            child = Node(node_id=self.new_id(), token_ids=[int(t)], seq_id=sid,
                          parent=leaf, cumulative_log_prob=leaf.cumulative_log_prob + float(lp), depth=leaf.depth + 1,
                          entropy_ema=leaf.entropy_ema, seq=leaf.seq + [int(t)], hist=leaf.hist.plus(int(t)))
             if leaf.sem_row is not None and self.sem is not None:
@@ -160,13 +163,14 @@ class Tree:
             self._walk(c, out, active)
 
     def free_all(self) -> None:
-        stack = [self.root]
+        stack, ids = [self.root], []
         while stack:
             n = stack.pop()
             if n.seq_id is not None:
-                self.cache.free_sequence(n.seq_id)
+                ids.append(n.seq_id)
                 n.seq_id = None
             stack.extend(n.children.values())
+        self.cache.free_sequences(ids)
 
 
 # ---------------------------------------------------------------------------
@@ -175,8 +179,13 @@ class Tree:
 class PagedLM:
     """Runs a Hugging Face Qwen3 / Llama causal LM over the paged cache."""
 
-    def __init__(self, model, cache: PagedKVCacheManager, tp_group=None):
+    def __init__(self, model, cache: PagedKVCacheManager, tp_group=None, *, fused_rotary: bool = False,
+                 sparse: Optional[tuple] = None):
         base = model.model
+        # sparse = (budget, sink, recent): decode attends to that many pages (attn_decode_sparse)
+        self.sparse = sparse
+        if sparse is not None:
+            cache.enable_page_index()
         self.model, self.cache = model, cache
         # tensor parallelism by KV head (``tp.shard_model``): the attention and MLP
         # outputs are partial sums over the group, all-reduced before the residual
@@ -187,6 +196,9 @@ class PagedLM:
         self.hq, self.hkv = cfg.num_attention_heads, cfg.num_key_value_heads
         self.hd = getattr(cfg, "head_dim", None) or cfg.hidden_size // self.hq
         self.qk_norm = hasattr(self.layers[0].self_attn, "q_norm")  # Qwen3
+        # queries and keys turned while they are appended (Rotary), in place of the
+        # module's cosines and sines in the model's dtype
+        self.fused = Rotary.from_module(self.rotary, self.hd) if fused_rotary else None
 
     def _sum(self, x: torch.Tensor) -> torch.Tensor:
         if self.tp_group is not None:
@@ -211,15 +223,20 @@ class PagedLM:
         """The prompt (L,) into the cache of ``seq_id``; logits (V,) of its last position."""
         L = input_ids.shape[-1]
         h = self.embed(input_ids.view(1, L))
-        pos = torch.arange(L, device=h.device).view(1, L)
-        cos, sin = self.rotary(h, pos)
-        cos, sin = cos.unsqueeze(2), sin.unsqueeze(2)  # (1, L, 1, hd)
+        if self.fused is None:
+            pos = torch.arange(L, device=h.device).view(1, L)
+            cos, sin = self.rotary(h, pos)
+            cos, sin = cos.unsqueeze(2), sin.unsqueeze(2)  # (1, L, 1, hd)
         for layer_idx, blk in enumerate(self.layers):
             attn = blk.self_attn
             q, k, v = self._qkv(attn, blk.input_layernorm(h), (1, L))
-            q, k = self._rope(q, cos, sin), self._rope(k, cos, sin)
-            self.cache.append_tokens(seq_id, layer_idx, k[0], v[0])
-            o = self.cache.prefill_attention(seq_id, layer_idx, q[0]).view(1, L, self.hq, self.hd)
+            if self.fused is None:
+                q, k = self._rope(q, cos, sin), self._rope(k, cos, sin)
+                self.cache.append_tokens(seq_id, layer_idx, k[0], v[0])
+                q = q[0]
+            else:
+                q = self.cache.append_rotated(seq_id, layer_idx, q[0], k[0], v[0], self.fused)
+            o = self.cache.prefill_attention(seq_id, layer_idx, q).view(1, L, self.hq, self.hd)
             h = h + self._sum(attn.o_proj(o.reshape(1, L, -1)))
             h = h + self._sum(blk.mlp(blk.post_attention_layernorm(h)))
         return self.lm_head(self.norm(h)[0, -1])
@@ -264,17 +281,24 @@ class PagedLM:
         if dec_slots is None:
             dec_slots = slots
         h = self.embed(tokens)
-        pos = c._ntok[0].index_select(0, dec_slots).to(torch.long).view(N, 1)  # lengths before this token
-        cos, sin = self.rotary(h, pos)
+        if self.fused is None:
+            pos = c._ntok[0].index_select(0, dec_slots).to(torch.long).view(N, 1)  # lengths before this token
+            cos, sin = self.rotary(h, pos)
         scale = 1.0 / (self.hd ** 0.5)
         for layer_idx, blk in enumerate(self.layers):
             attn = blk.self_attn
             q, k, v = self._qkv(attn, blk.input_layernorm(h), (N,))
-            q, k = self._rope(q, cos, sin), self._rope(k, cos, sin)
-            ops.append_batched(c._k_all, c._v_all, slots, k, v, c._op_id, layer_idx)
-            # every layer has the tree's sharing structure: plan once per step
-            o = ops.paged_decode(q, dec_slots, self._graph_max_len, c._op_id, layer_idx, scale,
-                                 reuse_plan=layer_idx > 0)
+            if self.fused is None:
+                q, k = self._rope(q, cos, sin), self._rope(k, cos, sin)
+                ops.append_batched(c._k_all, c._v_all, slots, k, v, c._op_id, layer_idx)
+            else:
+                q = ops.append_rotated(c._k_all, c._v_all, slots, q, k, v, c._op_id, layer_idx, self.fused.op_id)
+            if self.sparse is not None:
+                o = ops.paged_sparse_decode(q, dec_slots, self._graph_max_len, c._op_id, layer_idx, scale, *self.sparse)
+            else:
+                # every layer has the tree's sharing structure: plan once per step
+                o = ops.paged_decode(q, dec_slots, self._graph_max_len, c._op_id, layer_idx, scale,
+                                     reuse_plan=layer_idx > 0)
             h = h + self._sum(attn.o_proj(o.reshape(N, -1)))
             h = h + self._sum(blk.mlp(blk.post_attention_layernorm(h)))
         h = self.norm(h)
@@ -344,16 +368,24 @@ class PagedLM:
             self.cache.mirror_decode_step(seq_ids)
             return out
         h = self.embed(tokens.view(N))
-        pos = torch.tensor([self.cache.get_kv_length(s) for s in seq_ids], device=h.device).view(N, 1)
-        cos, sin = self.rotary(h, pos)  # (N, 1, hd): broadcasts over heads
+        if self.fused is None:
+            pos = torch.tensor([self.cache.get_kv_length(s) for s in seq_ids], device=h.device).view(N, 1)
+            cos, sin = self.rotary(h, pos)  # (N, 1, hd): broadcasts over heads
         for layer_idx, blk in enumerate(self.layers):
             attn = blk.self_attn
             q, k, v = self._qkv(attn, blk.input_layernorm(h), (N,))
-            q, k = self._rope(q, cos, sin), self._rope(k, cos, sin)
             # the new token's K/V go in first, so it attends to itself
-            self.cache.append_tokens_batched(seq_ids, layer_idx, k, v)
+            if self.fused is None:
+                q, k = self._rope(q, cos, sin), self._rope(k, cos, sin)
+                self.cache.append_tokens_batched(seq_ids, layer_idx, k, v)
+            else:
+                q = self.cache.append_rotated_batched(seq_ids, layer_idx, q, k, v, self.fused)
             pk, pv, cu, mx = self.cache.build_packed_kv(seq_ids, layer_idx)
-            o = attn_decode(q, pk, pv, None, cu, mx, N)
+            if self.sparse is not None:
+                budget, sink, recent = self.sparse
+                o = attn_decode_sparse(q, pk, pv, budget, sink=sink, recent=recent)
+            else:
+                o = attn_decode(q, pk, pv, None, cu, mx, N)
             h = h + self._sum(attn.o_proj(o.reshape(N, -1)))
             h = h + self._sum(blk.mlp(blk.post_attention_layernorm(h)))
         h = self.norm(h)
@@ -436,7 +468,8 @@ class TreeRollout:
                  soft_explore_initial: float = 0.3, max_seqs: int = 256, cuda_graphs: bool = True,
                  max_prompt_len: int = 4096, entropy_threshold: Optional[float] = None,
                  max_blocks_per_seq: Optional[int] = None, static_decode: bool = False, tp_group=None,
-                 graph_bucket: Optional[int] = None, log_softmax: str = "cpu"):
+                 graph_bucket: Optional[int] = None, log_softmax: str = "cpu", fused_rotary: bool = False,
+                 sparse_budget: Optional[int] = None, sparse_sink: int = 1, sparse_recent: int = 2):
         cfg = model.config
         dev = next(model.parameters()).device
         dtype = next(model.parameters()).dtype
@@ -444,7 +477,10 @@ class TreeRollout:
         hd = getattr(cfg, "head_dim", None) or cfg.hidden_size // hq
         self.cache = PagedKVCacheManager(cfg.num_hidden_layers, cfg.num_key_value_heads, hd, max_blocks, block_size,
                                          dev, dtype, max_seqs=max_seqs, max_blocks_per_seq=max_blocks_per_seq)
-        self.lm = PagedLM(model, self.cache, tp_group)
+        # fused_rotary: q and k turned by the append; sparse_budget: decode attends to at most
+        # that many pages per KV head (the first sparse_sink, the last sparse_recent, the best others)
+        self.lm = PagedLM(model, self.cache, tp_group, fused_rotary=fused_rotary,
+                          sparse=None if sparse_budget is None else (sparse_budget, sparse_sink, sparse_recent))
         self.eos = set(eos_token_id) if isinstance(eos_token_id, (list, tuple)) else {eos_token_id}
         self.M, self.K = max_active_branches, branching_factor
         self.max_new_tokens = max_new_tokens

@@ -1,0 +1,299 @@
+"""Batched fork, batched free, compaction and rotated appends of the paged cache against the
+single calls' oracle (``oracle.allocator``) and the compaction's definition (``oracle.cache_ops``):
+tables, reference counts and the free list's order bit-exact."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle.allocator import OraclePagedKV
+from oracle.cache_ops import compact, turn, turn_tolerance
+from tests.gpu_util import TORCH_DT, round_np
+
+pytestmark = pytest.mark.gpu
+
+
+def pair(L=2, hkv=2, d=64, pool=300, bs=4, dtype="bf16", seed=0, **kw):
+    from mentat_b200 import PagedKVCacheManager
+    order = np.random.default_rng(seed).permutation(pool).tolist()
+    m = PagedKVCacheManager(L, hkv, d, max_blocks=pool, block_size=bs, device="cuda", dtype=TORCH_DT[dtype],
+                            free_order=order, **{"max_seqs": 64, "strict": True, **kw})
+    o = OraclePagedKV(L, hkv, d, pool, bs, order=order, elem_bytes=m.dtype_size)
+    return m, o
+
+
+def fill(m, o, sid, n, rng, dtype="bf16"):
+    for layer in range(m.num_layers):
+        k, v = (round_np(rng.standard_normal((n, m.num_key_value_heads, m.head_dim), dtype=np.float32), dtype)
+                for _ in range(2))
+        m.append_tokens(sid, layer, *(torch.from_numpy(t).cuda().to(m.dtype) for t in (k, v)))
+        o.append_tokens(sid, layer, k, v)
+
+
+def start(m, o, lens, rng, dtype="bf16"):
+    ids = [m.allocate_sequence() for _ in lens]
+    assert ids == [o.allocate_sequence() for _ in lens]
+    for s, n in zip(ids, lens):
+        if n:
+            fill(m, o, s, n, rng, dtype)
+    return ids
+
+
+def same(m, o, tol=None):
+    """Allocator and tables equal, cached rows equal (or within ``tol(want)``)."""
+    snap, want = m.sequence_snapshot(), o.snapshot()
+    assert snap == want["seqs"]
+    assert m.allocator.refcounts == want["refcounts"]
+    assert m.allocator.free_list() == want["free"]
+    assert m.allocator.peak_used == want["peak"]
+    for sid, s in m._sequences.items():  # the host's mirror
+        w = o._sequences[sid]
+        assert s.num_tokens == w.num_tokens and s.tokens_in_last_block == w.tokens_in_last_block
+        assert s.num_blocks == [len(t) for t in w.page_table]
+    ids = sorted(m._sequences)
+    for layer in range(m.num_layers):
+        pk, pv, _, _ = m.packed_kv_tensors(ids, layer)
+        ok, ov, _, _ = o.build_packed_kv(ids, layer)
+        np.testing.assert_array_equal(pv.float().cpu().numpy(), ov)
+        if tol is None:
+            np.testing.assert_array_equal(pk.float().cpu().numpy(), ok)
+        else:
+            assert np.all(np.abs(pk.double().cpu().numpy() - ok) <= tol(ok))
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_batched_fork_and_free_are_the_single_calls(seed):
+    rng = np.random.default_rng(seed)
+    m, o = pair(L=int(rng.integers(1, 4)), pool=2000, seed=seed)
+    live = start(m, o, [0, 1, 3, 4, 5, 40], rng)
+    for step in range(12):
+        parents = rng.choice(live, rng.integers(1, 9)).tolist()  # a parent may have several children
+        if len(m._free_slots) < len(parents):
+            parents = []
+        kids = m.fork_sequences(parents)
+        assert kids == [o.fork_sequence(p) for p in parents]
+        live += kids
+        if step % 3 == 1:
+            for layer in range(m.num_layers):
+                k = round_np(rng.standard_normal((len(live), 2, 64), dtype=np.float32), "bf16")
+                t = torch.from_numpy(k).cuda().bfloat16()
+                m.append_tokens_batched(live, layer, t, t)
+                o.append_tokens_batched(live, layer, k, k)
+        gone = rng.permutation(live)[: rng.integers(0, len(live))].tolist()
+        m.free_sequences(gone)
+        for s in gone:
+            o.free_sequence(s)
+        live = [s for s in live if s not in gone] or start(m, o, [7], rng)
+        same(m, o)
+    m.free_sequences(live)
+    for s in live:
+        o.free_sequence(s)
+    same(m, o)
+    assert m.get_stats() == o.get_stats() and m.get_stats()["blocks_used"] == 0
+
+
+def test_large_batches_of_shared_pages():
+    """Many sequences over one prefix, rows of several chunks, more sequences than one launch takes."""
+    rng = np.random.default_rng(1)
+    m, o = pair(L=3, hkv=1, d=2, pool=8000, bs=2, dtype="f32", max_seqs=1200)
+    (root,) = start(m, o, [1403], rng, "f32")
+    kids = m.fork_sequences([root] * 1100)
+    assert kids == [o.fork_sequence(root) for _ in range(1100)]
+    assert m.allocator.refcounts == o.allocator.refcounts
+    order = rng.permutation(kids + [root]).tolist()
+    last = order.pop()
+    m.free_sequences(order)
+    for s in order:
+        o.free_sequence(s)
+    same(m, o)
+    m.free_sequences([last])
+    o.free_sequence(last)
+    same(m, o)
+
+
+def test_batched_refusals_change_nothing():
+    rng = np.random.default_rng(2)
+    m, o = pair(max_seqs=5)
+    a, b, c = start(m, o, [9, 4, 0], rng)
+    for call in (lambda: m.fork_sequences([a, 99]), lambda: m.free_sequences([a, 99]), lambda: m.free_sequences([a, b, a]),
+                 lambda: m.compact_sequences([a, a], [[0], [1]]), lambda: m.compact_sequences([99], [[0]])):
+        with pytest.raises(KeyError):
+            call()
+    with pytest.raises(RuntimeError, match="out of sequence slots"):
+        m.fork_sequences([a, a, b])
+    with pytest.raises(RuntimeError, match="out of sequence slots"):
+        m.compact_sequences([a, a, b], [[0]] * 3, into_new=True)
+    for keep in ([9], [-1], [[0], [9]], [[0, 1], [3, -2]]):
+        with pytest.raises(IndexError):
+            m.compact_sequences([a], [keep])
+    with pytest.raises(ValueError):
+        m.compact_sequences([a], [[[0], [1], [2]]])
+    with pytest.raises(ValueError):
+        m.compact_sequences([a, b], [[0]])
+    with pytest.raises(TypeError):
+        m.compact_sequences([a], [[0.5]])
+    assert m.fork_sequences([]) == [] and m.free_sequences([]) is None and m.compact_sequences([], []) is None
+    same(m, o)
+
+
+def test_device_refusals_change_nothing():
+    """What only the device can see: slots out of range, twice or in use, positions outside, too few
+    blocks.  Each is recorded, and nothing has changed."""
+    from mentat_b200 import ops
+    rng = np.random.default_rng(3)
+    m, o = pair(L=1, pool=12, strict=False)
+    a, b = start(m, o, [21, 5], rng)  # 6 + 2 of 12 blocks
+    i32 = dict(dtype=torch.int32, device="cuda")
+    sa, sb = m._sequences[a].slot, m._sequences[b].slot
+    free_slot = m._free_slots[-1]
+
+    def ids(*v):
+        return torch.tensor(v, **i32)
+    cu1, cu2 = ids(0, 3), ids(0, 3, 5)
+    bad = [
+        (ValueError, lambda: ops.free_pages(m, ids(sa, sb, sa))),
+        (ValueError, lambda: ops.free_pages(m, ids(sa, 64))),
+        (ValueError, lambda: ops.free_pages(m, ids(-1))),
+        (ValueError, lambda: ops.fork_pages(m, ids(sa, sa), ids(free_slot, free_slot))),
+        (ValueError, lambda: ops.fork_pages(m, ids(sa, sb), ids(free_slot, sa))),
+        (ValueError, lambda: ops.fork_pages(m, ids(64), ids(free_slot))),
+        (ValueError, lambda: ops.fork_pages(m, ids(sa), ids(-5))),
+        (ValueError, lambda: ops.compact_pages(m, ids(sa, sa), None, ids(0, 1, 2, 3, 4), cu2, 3)),
+        (ValueError, lambda: ops.compact_pages(m, ids(sa), ids(sb), ids(0, 1, 2), cu1, 3)),
+        (ValueError, lambda: ops.compact_pages(m, ids(sa), ids(sa), ids(0, 1, 2), cu1, 3)),
+        (IndexError, lambda: ops.compact_pages(m, ids(sa, sb), None, ids(0, 1, 2, 4, 5), cu2, 3)),
+        (IndexError, lambda: ops.compact_pages(m, ids(sa), None, ids(-1, 1, 2), cu1, 3)),
+        (RuntimeError, lambda: ops.compact_pages(m, ids(sa), ids(free_slot), torch.arange(20, 3, -1, **i32), ids(0, 17), 17)),
+    ]
+    for k, (exc, call) in enumerate(bad):
+        call()
+        with pytest.raises(exc):
+            m.check()
+        m.clear_error()
+        try:
+            same(m, o)
+        except AssertionError as e:
+            raise AssertionError(f"refusal {k} changed the cache") from e
+    # a call after an error that nobody has cleared changes nothing either
+    ops.free_pages(m, ids(-1))
+    ops.free_pages(m, ids(sa))
+    ops.fork_pages(m, ids(sa), ids(free_slot))
+    m.clear_error()
+    same(m, o)
+
+
+KEEPS = {
+    "all": lambda n, r: np.arange(n), "none": lambda n, r: np.arange(0), "front": lambda n, r: np.arange(n // 2),
+    "window": lambda n, r: np.concatenate([np.arange(min(3, n)), np.arange(max(min(3, n), n - 7), n)]),
+    "scattered": lambda n, r: np.sort(r.permutation(n)[: (n + 1) // 2]), "reversed": lambda n, r: np.arange(n)[::-1],
+    "repeated": lambda n, r: np.repeat(np.arange(n), 2)[: n + 3], "last": lambda n, r: np.arange(n - 1, n),
+}
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kind", sorted(KEEPS) + ["mixed"])
+@pytest.mark.parametrize("into_new", [False, True], ids=["in place", "new"])
+def test_compaction(kind, into_new, dtype):
+    rng = np.random.default_rng(4)
+    m, o = pair(L=2, pool=400, dtype=dtype)
+    ids = start(m, o, [1, 3, 4, 5, 8, 33, 50], rng, dtype)
+    ids += m.fork_sequences([ids[5], ids[6]])  # shared pages, one tail full and one partly filled
+    for s in (ids[5], ids[6]):
+        o.fork_sequence(s)
+    lens = [m.get_kv_length(s) for s in ids]
+    pick = sorted(KEEPS)
+    keep = [KEEPS[pick[i % len(pick)] if kind == "mixed" else kind](n, rng) for i, n in enumerate(lens)]
+    if kind == "mixed":  # a choice of its own in each layer
+        keep[6] = np.stack([keep[6], np.sort(rng.permutation(lens[6])[: len(keep[6])])])
+    as_given = [k if i % 2 else torch.from_numpy(k.copy()) for i, k in enumerate(keep)]
+    new = m.compact_sequences(ids, as_given, into_new=into_new)
+    assert (new or []) == compact(o, ids, keep, into_new=into_new)
+    same(m, o)
+    # the cache goes on: every sequence appends (copying shared tails), then all are freed
+    every = sorted(m._sequences)
+    for layer in range(2):
+        k = round_np(rng.standard_normal((len(every), 2, 64), dtype=np.float32), dtype)
+        t = torch.from_numpy(k).cuda().to(m.dtype)
+        m.append_tokens_batched(every, layer, t, t)
+        o.append_tokens_batched(every, layer, k, k)
+    same(m, o)
+    m.free_sequences(every)
+    for s in every:
+        o.free_sequence(s)
+    same(m, o)
+
+
+@pytest.mark.parametrize("dtype,d,bs,rd,il", [("bf16", 64, 16, 64, False), ("f32", 128, 4, 64, True), ("f16", 37, 5, 20, False)])
+def test_compaction_turns_keys(dtype, d, bs, rd, il):
+    from mentat_b200 import Rotary
+    rng = np.random.default_rng(6)
+    m, o = pair(L=2, d=d, bs=bs, pool=200, dtype=dtype)
+    ids = start(m, o, [1, 70, 129], rng, dtype)
+    rot = Rotary(d, rotary_dim=rd, interleaved=il, attention_scaling=1.7)  # the factor is not applied again
+    f = rot.inv_freq.cpu().numpy()
+    keep = [[0], np.r_[0:4, 30:70], np.sort(rng.permutation(129)[:61])]
+    m.compact_sequences(ids, keep, rotary=rot)
+    compact(o, ids, keep, turn_keys=lambda k, shift: turn(k, shift, f, interleaved=il))
+    eps = torch.finfo(m.dtype).eps
+    # the tolerance of a turn, from rows of the turned keys (a pair's |x1| + |x2| is at most
+    # sqrt(2) times its turned one's); fp16 steps below 2^-14 are 2^-24 wide
+    same(m, o, lambda want: 1.5 * turn_tolerance(want, f, eps, interleaved=il)(want) + (2.0 ** -25 if dtype == "f16" else 0))
+
+
+def test_compaction_of_device_positions_on_another_stream():
+    rng = np.random.default_rng(8)
+    m, o = pair()
+    ids = start(m, o, [40, 17], rng)
+    keep = [torch.tensor([1, 2, 39], device="cuda"), torch.tensor([[0, 16], [3, 4]], device="cuda", dtype=torch.int32)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        m.compact_sequences(ids, keep)
+    torch.cuda.current_stream().wait_stream(s)
+    compact(o, ids, [k.cpu().numpy() for k in keep])
+    same(m, o)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d,rd,il,bs", [(64, 64, False, 4), (128, 32, True, 16), (38, 10, False, 3)])
+def test_rotated_appends(dtype, d, rd, il, bs):
+    """append_rotated and append_rotated_batched: append_tokens and append_tokens_batched of turned
+    keys, over copied tails, a repeated sequence in a batch, and positions of the caller's."""
+    from mentat_b200 import Rotary
+    rng = np.random.default_rng(9)
+    m, o = pair(L=2, hkv=2, d=d, pool=200, bs=bs, dtype=dtype)
+    rot = Rotary(d, rotary_dim=rd, interleaved=il, base=1e4)
+    f, eps = rot.inv_freq.cpu().numpy(), torch.finfo(m.dtype).eps
+    a = m.allocate_sequence()
+    o.allocate_sequence()
+
+    def rows(n, h):
+        x = round_np(rng.standard_normal((n, h, d), dtype=np.float32), dtype)
+        return x, torch.from_numpy(x).cuda().to(m.dtype)
+
+    def check_q(got, x, pos):
+        want = turn(x, pos, f, interleaved=il)
+        assert np.all(np.abs(got.double().cpu().numpy() - want) <= turn_tolerance(x, f, eps, interleaved=il)(want))
+    for n, first in ((5, 0), (7, 5), (1, 12)):
+        for layer in range(2):
+            (q, tq), (k, tk), (v, tv) = rows(n, 6), rows(n, 2), rows(n, 2)
+            pos = np.arange(first, first + n)
+            if layer:
+                check_q(m.append_rotated(a, layer, tq, tk, tv, rot), q, pos)
+            else:
+                assert m.append_rotated(a, layer, None, tk, tv, rot, positions=torch.from_numpy(pos + 900).cuda()) is None
+                pos = pos + 900
+            o.append_tokens(a, layer, turn(k, pos, f, interleaved=il), v)
+    kids = m.fork_sequences([a, a, a])
+    assert kids == [o.fork_sequence(a) for _ in range(3)]
+    for step in range(bs + 2):
+        batch = [a] + kids if step != 3 else [a, kids[1], a, kids[1]]
+        for layer in range(2):
+            (q, tq), (k, tk), (v, tv) = rows(4, 6), rows(4, 2), rows(4, 2)
+            seen, pos = {}, []
+            for s in batch:
+                seen[s] = seen.get(s, 0) + 1
+                pos.append(o._sequences[s].num_tokens[layer] + seen[s] - 1)
+            check_q(m.append_rotated_batched(batch, layer, tq, tk, tv, rot), q, pos)
+            o.append_tokens_batched(batch, layer, turn(k, pos, f, interleaved=il), v)
+    same(m, o, lambda want: 1.5 * turn_tolerance(want, f, eps, interleaved=il)(want))

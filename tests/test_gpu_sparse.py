@@ -1,0 +1,379 @@
+"""The page index and sparse decode against their definitions (``oracle.cache_ops``): the index and
+the chosen pages exactly, the attention over them in 64 bits."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle.cache_ops import index_page, sparse_decode
+from tests.gpu_util import TORCH_DT
+
+pytestmark = pytest.mark.gpu
+
+
+def tolerance(dtype, v):
+    """Of an output element, from the largest value it averages.  fp32: scores of |s| < 64 carry
+    (d / 4 + 8) 2^-24 of sum |q k| <= 64, so a weight's error is below 41 * 64 * 2^-24 < 2^-12.6, which
+    two-sided normalisation halves for what does not move together; the bound of 2e-5 (2^-15.6) of the
+    other attention tests is kept: |s| here stays near 8.  bf16 / fp16: weights and the result are
+    each rounded at most once to the type (half a step each), and the scores add 2^-16."""
+    eps = torch.finfo(TORCH_DT[dtype]).eps
+    top = float(np.abs(v).max())
+    return 2e-5 * top if dtype == "f32" else (eps + 2.0 ** -14) * top
+
+
+def make(lens, hq, hkv, d, bs, dtype, *, layers=2, shared=0, seed=0, extra=3):
+    """One cache of given lengths; the first `shared` pages of all sequences are the same blocks."""
+    from mentat_b200 import KVCacheView, PageIndex, ops
+    rng = np.random.default_rng(seed)
+    pages = [-(-n // bs) for n in lens]
+    blocks = shared + sum(max(0, p - shared) for p in pages) + extra
+    order = rng.permutation(blocks)
+    cap = max(pages + [1]) + 2
+    tables = np.full((layers, len(lens) + 1, cap), -7, np.int32)
+    nid = shared
+    for i, p in enumerate(pages):
+        a = min(shared, p)
+        tables[:, i, :a] = order[:a]
+        tables[:, i, a:p] = order[nid: nid + p - a]
+        nid += p - a
+    dt = TORCH_DT[dtype]
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    size = torch.exp(0.5 * torch.randn((hkv, d), generator=g, device="cuda"))
+    k = (torch.randn((layers, blocks, 1, hkv, d), generator=g, device="cuda") * 0.7 +
+         torch.randn((layers, blocks, bs, hkv, d), generator=g, device="cuda") * 0.5) * size
+    k, v = k.to(dt), torch.randn((layers, blocks, bs, hkv, d), generator=g, device="cuda").to(dt)
+    ntok = torch.tensor([list(lens) + [0]] * layers, dtype=torch.int32, device="cuda")
+    c = KVCacheView(k, v, torch.from_numpy(tables).cuda(), ntok)
+    x = PageIndex(c)
+    for layer in range(layers):
+        ops.page_index(x, layer, torch.from_numpy(order[:nid].astype(np.int32)).cuda())
+    q = torch.randn((len(lens), hq, d), generator=g, device="cuda").to(dt)
+    return c, x, q, tables
+
+
+def run_and_check(c, x, q, tables, lens, budget, sink, recent, dtype, layer=1, scale=None, slots=None):
+    from mentat_b200 import ops
+    slots = list(range(len(lens))) if slots is None else slots
+    out, pages = ops.sparse_decode(x, layer, torch.tensor(slots, dtype=torch.int32, device="cuda"), q, max(lens + [0]),
+                                   budget, sink=sink, recent=recent, scale=scale, return_pages=True)
+    c.check()
+    kp, vp = (t[layer].double().cpu().numpy() for t in (c._tensors["k_pool"], c._tensors["v_pool"]))
+    want, chosen = sparse_decode(q.double().cpu().numpy(), kp, vp, [tables[layer, s] for s in slots],
+                                 [lens[s] if s < len(lens) else 0 for s in slots], c.block_size,
+                                 x.bounds[layer].cpu().numpy(), x.exps[layer].cpu().numpy(), budget, sink, recent, scale)
+    np.testing.assert_array_equal(pages.cpu().numpy(), chosen)
+    off = np.abs(out.double().cpu().numpy() - want)
+    assert np.all(off <= tolerance(dtype, vp)), float(off.max())
+    only = ops.sparse_decode(x, layer, torch.tensor(slots, dtype=torch.int32, device="cuda"), q, max(lens + [0]), budget,
+                             sink=sink, recent=recent, scale=scale)
+    assert torch.equal(only, out)
+    return out, pages
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hkv,d,bs", [(8, 128, 16), (1, 64, 16), (3, 40, 5), (2, 200, 32)])
+def test_page_index(dtype, hkv, d, bs):
+    from mentat_b200 import KVCacheView, PageIndex, ops
+    g = torch.Generator(device="cuda").manual_seed(0)
+    blocks, layer = 23, 1
+    k = torch.randn((2, blocks, bs, hkv, d), generator=g, device="cuda")
+    k *= torch.exp(4 * torch.randn((2, blocks, 1, 1, 1), generator=g, device="cuda"))
+    k[1, 3] = 0
+    k[1, 4] = -2.0                      # powers of two, and the borders of one unit
+    k[1, 5, 0, 0, 0] = float("nan")
+    k[1, 6, bs - 1, hkv - 1, d - 1] = float("inf")
+    k[1, 7] = 127.0
+    k[1, 8] = 127.5
+    k[1, 9] = 0
+    k[1, 9, 0, 0, 0] = 6e-8             # fp16's smallest
+    k = k.to(TORCH_DT[dtype])
+    if dtype != "f16":
+        k[1, 10] *= 1e30                # saturates
+        k[1, 11] *= 1e-30
+    c = KVCacheView(k, k)
+    x = PageIndex(c)
+    ids = torch.tensor([i for i in range(blocks) if i != 20], dtype=torch.int32, device="cuda")
+    ops.page_index(x, layer, torch.cat([ids, ids[:3]]))  # some twice
+    low, high, exps = ops.page_bounds(x, layer, ids)
+    kk = k[layer].double().cpu().numpy()
+    for i, b in enumerate(ids.tolist()):
+        bounds, e = index_page(kk[b])
+        np.testing.assert_array_equal(x.bounds[layer, b].cpu().numpy(), bounds)
+        np.testing.assert_array_equal(x.exps[layer, b].cpu().numpy(), e)
+        np.testing.assert_array_equal(exps[i].cpu().numpy(), e)
+        fine = e != 127
+        unit = 2.0 ** e[fine].astype(float)[:, None]
+        np.testing.assert_array_equal(low[i].double().cpu().numpy()[fine], bounds[fine, 0] * unit)
+        np.testing.assert_array_equal(high[i].double().cpu().numpy()[fine], bounds[fine, 1] * unit)
+        assert torch.isinf(low[i][torch.from_numpy(~fine)]).all()
+        if b != 10 and fine.all():
+            assert (low[i].double().cpu().numpy() <= kk[b].min(0)).all() and (high[i].double().cpu().numpy() >= kk[b].max(0)).all()
+    assert (x.exps[layer, 20] == 127).all() and (x.exps[0] == 127).all()  # not indexed
+    c.check()
+    ops.page_index(x, layer, torch.tensor([blocks, 0, -1], dtype=torch.int32, device="cuda"))
+    with pytest.raises(AssertionError, match="outside the pool"):
+        c.check()
+
+
+CASES = [  # lens, hq, hkv, d, bs, shared, budget, sink, recent
+    ([0, 1, 15, 16, 17, 33], 8, 8, 128, 16, 0, 2, 0, 1), ([0, 1, 2, 3, 4, 5, 6, 40], 4, 2, 64, 4, 0, 3, 1, 1),
+    ([500, 1, 777, 160], 8, 2, 128, 16, 5, 8, 1, 2), ([1000, 999], 10, 2, 64, 16, 20, 17, 2, 3),
+    ([300], 16, 1, 128, 16, 0, 1, 0, 1), ([640, 641], 32, 4, 128, 32, 3, 6, 0, 1), ([200, 90], 3, 1, 64, 5, 2, 9, 1, 1),
+    ([4097, 70, 2500], 16, 8, 128, 16, 0, 40, 1, 2), ([350, 20], 7, 7, 64, 24, 0, 5, 0, 2),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("case", CASES, ids=lambda c: f"{c[0][0]}x{len(c[0])}-{c[1]}-{c[2]}-{c[3]}-{c[4]}-{c[6]}")
+def test_sparse_decode_matches_definition(case, dtype):
+    lens, hq, hkv, d, bs, shared, budget, sink, recent = case
+    c, x, q, tables = make(lens, hq, hkv, d, bs, dtype, shared=shared)
+    run_and_check(c, x, q, tables, lens, budget, sink, recent, dtype)
+    # strided queries, sequences in another order and twice, another scale, a slot without tokens
+    wide = torch.cat([q, q], dim=1)[:, :hq]
+    slots = [len(lens) - 1, 0, len(lens), 0]
+    run_and_check(c, x, wide[[len(lens) - 1, 0, 0, 0]], tables, lens, budget, sink, recent, dtype, layer=0,
+                  scale=0.3, slots=slots)
+
+
+def test_many_pages():
+    """Long sequences: selection over thousands of pages, a large budget."""
+    lens = [70001, 40000, 64 * 16]
+    c, x, q, tables = make(lens, 8, 2, 64, 16, "bf16", layers=1, shared=1000)
+    for budget in (64, 1500):
+        run_and_check(c, x, q, tables, lens, budget, 1, 2, "bf16", layer=0)
+
+
+def test_ties_go_to_the_lowest_page():
+    from mentat_b200 import ops
+    lens = [2000]
+    c, x, q, tables = make(lens, 4, 1, 64, 16, "bf16", layers=1)
+    x.bounds.zero_()
+    x.exps.zero_()
+    _, pages = ops.sparse_decode(x, 0, torch.zeros(1, dtype=torch.int32, device="cuda"), q, 2000, 9, sink=0, recent=2,
+                                 return_pages=True)
+    assert pages.flatten().tolist() == [0, 1, 2, 3, 4, 5, 6, 123, 124]
+    run_and_check(c, x, q, tables, lens, 9, 0, 2, "bf16", layer=0)
+    run_and_check(c, x, torch.zeros_like(q), tables, lens, 9, 3, 2, "bf16", layer=0)
+
+
+def test_pages_with_infinities_are_chosen_and_show():
+    """A page with a NaN key is attended to, so the output shows it as dense decode does; a query
+    element that is not finite counts as 0 in the score."""
+    from mentat_b200 import ops
+    lens = [800, 800]
+    c, x, q, tables = make(lens, 4, 2, 64, 16, "f32", layers=1)
+    b = int(tables[0, 0, 30])
+    c._tensors["k_pool"][0, b, 3, 1, 5] = float("nan")
+    ops.page_index(x, 0, torch.tensor([b], dtype=torch.int32, device="cuda"))
+    q[1, 0, 7] = float("inf")
+    slots = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    out, pages = ops.sparse_decode(x, 0, slots, q, 800, 4, return_pages=True)
+    assert 30 in pages[0, 1].tolist()
+    assert torch.isfinite(out[0, :2]).all() and torch.isnan(out[0, 2:]).all()
+    assert not torch.isfinite(out[1, 0]).any() and torch.isfinite(out[1, 1:]).all()
+    _, chosen = sparse_decode(np.nan_to_num(q.double().cpu().numpy(), posinf=0.0), c._tensors["k_pool"][0].double().cpu().numpy(),
+                              c._tensors["v_pool"][0].double().cpu().numpy(), [tables[0, 0], tables[0, 1]], lens, 16,
+                              x.bounds[0].cpu().numpy(), x.exps[0].cpu().numpy(), 4, 1, 1)
+    np.testing.assert_array_equal(pages.cpu().numpy(), chosen)
+
+
+def test_sparse_decode_records_bad_state():
+    from mentat_b200 import ops
+    lens = [500, 300]
+    c, x, q, tables = make(lens, 4, 2, 64, 16, "bf16")
+    both = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+
+    def recorded(exc, call):
+        call()
+        with pytest.raises(exc):
+            c.check()
+        c._tensors["ctrl"].zero_()
+    out = ops.sparse_decode(x, 0, both, q, 499, 8)          # longer than max_len: zeros
+    with pytest.raises(RuntimeError, match="overflow"):
+        c.check()
+    c._tensors["ctrl"].zero_()
+    assert not out[0].any() and out[1].any()
+    recorded(ValueError, lambda: ops.sparse_decode(x, 0, both + 2, q, 500, 8))
+    recorded(ValueError, lambda: ops.sparse_decode(x, 0, both - 2, q, 500, 8))
+    c._tensors["tables"][0, 0, 17] = c.max_blocks           # a corrupt table: not read
+    recorded(AssertionError, lambda: ops.sparse_decode(x, 0, both, q, 500, 8))
+    recorded(AssertionError, lambda: ops.sparse_decode(x, 0, both, q, 500, 40))
+    for bad in (dict(budget=2, sink=2, recent=1), dict(budget=2, sink=0, recent=0), dict(budget=2, sink=-1)):
+        with pytest.raises(ValueError):
+            ops.sparse_decode(x, 0, both, q, 500, **bad)
+    with pytest.raises(ValueError):
+        ops.sparse_decode(x, 0, both[:1], q, 500, 8)
+    with pytest.raises(TypeError):
+        ops.sparse_decode(x, 0, both, q.float(), 500, 8)
+    assert ops.sparse_decode(x, 0, both[:0], q[:0], 500, 8).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_sparse_decode_of_every_page_is_dense_decode(dtype):
+    from mentat_b200 import PagedKVCacheManager
+    from mentat_b200.attention_backend import attn_decode, attn_decode_sparse
+    g = torch.Generator(device="cuda").manual_seed(3)
+    m = PagedKVCacheManager(1, 2, 128, max_blocks=200, device="cuda", dtype=TORCH_DT[dtype])
+    with pytest.raises(RuntimeError, match="enable_page_index"):
+        attn_decode_sparse(torch.zeros((0, 8, 128), device="cuda", dtype=m.dtype), *m.build_packed_kv([], 0)[:2], 8)
+    m.enable_page_index()
+    a = m.allocate_sequence()
+    kv = torch.randn((530, 2, 128), generator=g, device="cuda").to(m.dtype)
+    m.append_tokens(a, 0, kv, kv)
+    kids = m.fork_sequences([a] * 3)
+    q = torch.randn((4, 8, 128), generator=g, device="cuda").to(m.dtype)
+    k, v, cu, mx = m.build_packed_kv([a] + kids, 0)
+    dense, sparse = attn_decode(q, k, v, None, cu, mx, 4), attn_decode_sparse(q, k, v, 34)
+    assert np.abs((dense.double() - sparse.double()).cpu().numpy()).max() <= 2 * tolerance(dtype, kv.double().cpu().numpy())
+
+
+def test_index_is_kept_by_the_cache():
+    """Appends of one and many tokens (plain and rotated), forks, copied tails, trims, compaction,
+    recycled blocks: every full page of every sequence is indexed as if anew."""
+    from mentat_b200 import PagedKVCacheManager, Rotary
+    rng = np.random.default_rng(11)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    m = PagedKVCacheManager(2, 2, 64, max_blocks=160, block_size=4, device="cuda", dtype=torch.bfloat16, strict=True)
+    rot = Rotary(64)
+
+    def rows(n):
+        return torch.randn((n, 2, 64), generator=g, device="cuda").bfloat16()
+
+    def check():
+        m.check()
+        for sid, s in m._sequences.items():
+            for layer in range(2):
+                full = s.num_tokens[layer] // 4
+                tab = m.page_table(sid, layer)[:full]
+                for b in tab:
+                    bounds, exps = index_page(m.k_pools[layer][b].double().cpu().numpy())
+                    np.testing.assert_array_equal(m.page_index.bounds[layer, b].cpu().numpy(), bounds)
+                    np.testing.assert_array_equal(m.page_index.exps[layer, b].cpu().numpy(), exps)
+    a = m.allocate_sequence()
+    for layer in range(2):
+        m.append_tokens(a, layer, rows(10), rows(10))
+    m.enable_page_index()  # over what is there
+    assert m.enable_page_index() is m.page_index
+    check()
+    b = m.allocate_sequence()
+    for layer in range(2):
+        m.append_tokens(a, layer, rows(7), rows(7))
+        m.append_rotated(b, layer, rows(9), rows(9), rows(9), rot)
+    check()
+    live = [a, b] + m.fork_sequences([a, a, b])
+    for step in range(30):
+        for layer in range(2):
+            if step % 2:
+                m.append_tokens_batched(live, layer, rows(len(live)), rows(len(live)))
+            else:
+                m.append_rotated_batched(live, layer, rows(len(live)), rows(len(live)), rows(len(live)), rot)
+        if step == 9:
+            m.compact_sequences(live[:2], [np.arange(3, 20), np.arange(5)], rotary=rot)
+            live += m.compact_sequences(live[2:3], [np.r_[0:4, 8:17]], into_new=True)
+        if step == 17:
+            m.trim_to_window(live[3], 9)
+        if step % 8 == 5:
+            gone = rng.permutation(live)[:2].tolist()
+            m.free_sequences(gone)
+            live = [s for s in live if s not in gone]
+            live += m.fork_sequences([live[0], live[0]])
+        if step % 6 == 5 or step in (9, 17):
+            check()
+    check()
+
+
+def test_captured_and_on_another_stream():
+    from mentat_b200 import ops
+    lens = [900, 70]
+    c, x, q, tables = make(lens, 8, 2, 128, 16, "bf16", layers=1)
+    slots = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    want = ops.sparse_decode(x, 0, slots, q, 900, 8)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.sparse_decode(x, 0, slots, q, 900, 8)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(got, want)
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        o1 = ops.sparse_decode(x, 0, slots, q, 900, 8)
+    with torch.cuda.graph(g2):
+        o2 = ops.sparse_decode(x, 0, slots.flip(0), q, 900, 12)
+    c._tensors["ntok"][0, 0] = 850  # replays read the lengths of the time
+    q.mul_(0.5)
+    for _ in range(2):
+        g1.replay()
+        g2.replay()
+    assert torch.equal(o1, ops.sparse_decode(x, 0, slots, q, 900, 8))
+    assert torch.equal(o2, ops.sparse_decode(x, 0, slots.flip(0), q, 900, 12))
+
+
+def test_steps_of_the_set_together():
+    """Decode steps as they are run: rotated appends, forks, sparse attention, a freed branch, compaction,
+    against the definitions over the cache's own rows."""
+    from mentat_b200 import PagedKVCacheManager, Rotary
+    from mentat_b200.attention_backend import attn_decode_sparse
+    g = torch.Generator(device="cuda").manual_seed(6)
+    m = PagedKVCacheManager(2, 2, 64, max_blocks=400, device="cuda", dtype=torch.bfloat16, strict=True)
+    m.enable_page_index()
+    rot = Rotary(64, base=5e5, scaling=dict(rope_type="linear", factor=2.0))
+
+    def rows(n, h):
+        return torch.randn((n, h, 64), generator=g, device="cuda").bfloat16()
+    a = m.allocate_sequence()
+    for layer in range(2):
+        q = m.append_rotated(a, layer, rows(300, 8), rows(300, 2), rows(300, 2), rot)
+        m.prefill_attention(a, layer, q)
+    live = m.fork_sequences([a] * 3)
+    m.free_sequences([a])
+    for step in range(24):
+        for layer in range(2):
+            q = m.append_rotated_batched(live, layer, rows(len(live), 8), rows(len(live), 2), rows(len(live), 2), rot)
+            k, v, _, _ = m.build_packed_kv(live, layer)
+            out, pages = attn_decode_sparse(q, k, v, 7, sink=1, recent=2, return_pages=True)
+            if step % 6 == 0:
+                tabs = [m.page_table(s, layer) for s in live]
+                vp = m.v_pools[layer].double().cpu().numpy()
+                want, chosen = sparse_decode(q.double().cpu().numpy(), m.k_pools[layer].double().cpu().numpy(), vp, tabs,
+                                             k.lens, 16, m.page_index.bounds[layer].cpu().numpy(),
+                                             m.page_index.exps[layer].cpu().numpy(), 7, 1, 2)
+                np.testing.assert_array_equal(pages.cpu().numpy(), chosen)
+                assert np.abs(out.double().cpu().numpy() - want).max() <= tolerance("bf16", vp)
+        if step == 7:
+            live += m.fork_sequences(live[:1] * 2)
+        if step == 11:
+            m.free_sequences(live[1:3])
+            del live[1:3]
+        if step == 15:
+            n = m.get_kv_length(live[0])
+            m.compact_sequences(live[:1], [np.r_[0:16, n - 100:n]], rotary=rot)
+            assert m.get_kv_length(live[0]) == 116
+    m.free_sequences(live)
+    assert m.get_stats()["blocks_used"] == 0
+
+
+@pytest.mark.parametrize("mode", ["graphs", "padded", "static", "eager"])
+def test_rollout_with_fused_rotary_and_all_pages(mode):
+    """The golden fp32 trees again with rotated appends, and with a budget that covers every page."""
+    import json
+    import os
+    from mentat_b200.rollout import TreeRollout
+    from tests.golden.cases import ROLLOUT_CASES, rollout_model, rollout_prompts
+    golden = json.load(open(os.path.join(os.path.dirname(__file__), "golden", "rollout.json")))
+    kw = {"graphs": {}, "padded": dict(graph_bucket=4), "static": dict(cuda_graphs=False, static_decode=True),
+          "eager": dict(cuda_graphs=False)}[mode]
+    for name, c in sorted(ROLLOUT_CASES.items()):
+        model = rollout_model(c, device="cuda")
+        for sparse in (dict(), dict(sparse_budget=64, sparse_sink=2)):
+            r = TreeRollout(model, eos_token_id=c["eos"], max_active_branches=c["max_active_branches"],
+                            branching_factor=c["branching_factor"], max_new_tokens=c["max_new_tokens"], block_size=16,
+                            max_blocks=4096, fused_rotary=True, **sparse, **kw)
+            for got, want in zip(r.generate_many(rollout_prompts(c)), golden[name]):
+                assert [x["token_ids"] for x in got] == [x["token_ids"] for x in want["results"]], name
+                np.testing.assert_allclose([x["log_prob"] for x in got], [x["log_prob"] for x in want["results"]],
+                                           rtol=1e-4, atol=1e-4)
+            assert r.cache.get_stats()["blocks_used"] == 0
