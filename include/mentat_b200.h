@@ -448,11 +448,13 @@ int mentat_page_bounds(const mentat_kv_cache* c, int32_t layer, const int32_t* b
  * the pages before a sequence's last one must be indexed.  max_len: the longest
  * sequence (a longer one gets zeros and MENTAT_DEV_PLAN_OVERFLOW).  pages, if not
  * NULL: device int32 [n][kv_heads][budget], the chosen pages in rising order,
- * then -1.  GQA groups up to 16, head_dim 64 or 128. */
+ * then -1.  workspace: 16-byte aligned, mentat_sparse_workspace_bytes(...) bytes (0
+ * for small batches, which need none).  GQA groups up to 16, head_dim 64 or 128. */
+int64_t mentat_sparse_workspace_bytes(const mentat_kv_cache* c, int32_t n, int32_t max_len, int32_t budget);
 int mentat_sparse_decode(const mentat_kv_cache* c, int32_t layer, const mentat_page_index* x, const int32_t* slots,
                          int32_t n, const void* q, int64_t q_stride, int32_t num_q_heads, void* out,
                          int64_t out_stride, float scale, int32_t max_len, int32_t budget, int32_t sink,
-                         int32_t recent, int32_t* pages, cudaStream_t s);
+                         int32_t recent, int32_t* pages, void* workspace, int64_t workspace_bytes, cudaStream_t s);
 
 #ifdef __cplusplus
 }

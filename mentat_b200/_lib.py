@@ -111,8 +111,9 @@ SIGNATURES = [
     ("mentat_page_index_blocks", C.c_int, [_KV, _I32, _P, _I32, _IDX, _P]),
     ("mentat_page_index_seqs", C.c_int, [_KV, _I32, _P, _I32, _I32, _I32, _IDX, _P]),
     ("mentat_page_bounds", C.c_int, [_KV, _I32, _P, _I32, _IDX, _P, _P, _P, _P]),
+    ("mentat_sparse_workspace_bytes", _I64, [_KV, _I32, _I32, _I32]),
     ("mentat_sparse_decode", C.c_int,
-     [_KV, _I32, _IDX, _P, _I32, _P, _I64, _I32, _P, _I64, _F, _I32, _I32, _I32, _I32, _P, _P]),
+     [_KV, _I32, _IDX, _P, _I32, _P, _I64, _I32, _P, _I64, _F, _I32, _I32, _I32, _I32, _P, _P, _I64, _P]),
 ]
 
 _lib = None
@@ -135,6 +136,22 @@ def load() -> C.CDLL:
         raise RuntimeError("libmentat_b200.so ABI mismatch")
     _lib = lib
     return lib
+
+
+_calls: dict = {}
+
+
+def call(name: str):
+    """Entry point ``name`` as a function of its own whose pointer arguments are plain addresses
+    (or bytes objects, for structures): their conversion costs a tenth of a typed pointer's."""
+    fn = _calls.get(name)
+    if fn is None:
+        args = next(a for n, _, a in SIGNATURES if n == name)
+        fn = load()[name]  # a new function object, whose argtypes are not the typed one's
+        fn.restype = next(r for n, r, _ in SIGNATURES if n == name)
+        fn.argtypes = [C.c_void_p if a in (_KV, _ROT, _ROWS, _IDX) else a for a in args]
+        _calls[name] = fn
+    return fn
 
 
 def check(status: int, what: str) -> None:

@@ -1023,14 +1023,11 @@ static int launch_decode(const mentat_kv_cache* c, int layer, const int32_t* slo
                          int64_t q_stride, int Hq, void* out, int64_t out_stride, float scale, DecodeWs ws,
                          int max_parts, bool reuse_plan, cudaStream_t s) {
     const int G = Hq / c->num_kv_heads;
-    const PoolMaps* maps = nullptr;
+    CUtensorMap mk{}, mv{};
     bool tc_ok = false, narrow_ok = false;
     if constexpr (!std::is_same<T, float>::value) {
         tc_ok = tc_supported(c) && tc_min_rows() <= TC_MAX_ROWS && ((uintptr_t)q % 16 == 0) && (q_stride % 8 == 0);
-        if (tc_ok) {
-            maps = pool_maps(c, layer);
-            tc_ok = maps != nullptr;
-        }
+        if (tc_ok) tc_ok = pool_maps(c, layer, &mk, &mv);
         narrow_ok = tc_ok && D == 128 && narrow_enabled();
         // the shared-memory attribute is per device: one flag per device ordinal
         static bool attr[64] = {};
@@ -1090,7 +1087,7 @@ static int launch_decode(const mentat_kv_cache* c, int layer, const int32_t* slo
     prof_mark(2, s);
     if constexpr (!std::is_same<T, float>::value) {
         if (tc_ok) {
-            if (launch(pdl, k_units_tc<T, D>, dim3(num_sms()), dim3(TC_THREADS), TC_SMEM, s, maps->mk, maps->mv, *c,
+            if (launch(pdl, k_units_tc<T, D>, dim3(num_sms()), dim3(TC_THREADS), TC_SMEM, s, mk, mv, *c,
                        layer, slots, qt, q_stride, Hq, qscale, ws, max_parts, -1, (T*)nullptr, (int64_t)0) !=
                 cudaSuccess)
                 return MENTAT_ERR_CUDA;
@@ -1100,7 +1097,7 @@ static int launch_decode(const mentat_kv_cache* c, int layer, const int32_t* slo
     prof_mark(3, s);
     if constexpr (!std::is_same<T, float>::value && D == 128) {
         if (narrow_ok) {
-            if (launch(pdl, k_units_tcn<T, D>, dim3(num_sms()), dim3(TCN_THREADS), TCN_SMEM, s, maps->mk, maps->mv,
+            if (launch(pdl, k_units_tcn<T, D>, dim3(num_sms()), dim3(TCN_THREADS), TCN_SMEM, s, mk, mv,
                        *c, layer, slots, qt, q_stride, Hq, qscale, ws, max_parts) != cudaSuccess)
                 return MENTAT_ERR_CUDA;
             MENTAT_CHECK_LAUNCH();
@@ -1141,13 +1138,10 @@ static int launch_prefill(const mentat_kv_cache* c, int layer, const int32_t* sl
                           int max_parts, cudaStream_t s) {
     const int G = Hq / c->num_kv_heads;
     bool tc_ok = false;
-    const PoolMaps* maps = nullptr;
+    CUtensorMap mk{}, mv{};
     if constexpr (!std::is_same<T, float>::value) {
         tc_ok = tc_supported(c) && ((uintptr_t)q % 16 == 0) && (q_stride % 8 == 0);
-        if (tc_ok) {
-            maps = pool_maps(c, layer);
-            tc_ok = maps != nullptr;
-        }
+        if (tc_ok) tc_ok = pool_maps(c, layer, &mk, &mv);
         static bool attr[64] = {};
         int dev = 0;
         if (tc_ok && (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)) return MENTAT_ERR_CUDA;
@@ -1180,7 +1174,7 @@ static int launch_prefill(const mentat_kv_cache* c, int layer, const int32_t* sl
     }
     if constexpr (!std::is_same<T, float>::value) {
         if (tc_ok) {
-            if (launch(pdl, k_units_tc<T, D, true>, dim3(num_sms()), dim3(TC_THREADS), TC_SMEM, s, maps->mk, maps->mv, *c,
+            if (launch(pdl, k_units_tc<T, D, true>, dim3(num_sms()), dim3(TC_THREADS), TC_SMEM, s, mk, mv, *c,
                        layer, slot, qt, q_stride, Hq, qscale, ws, max_parts, pos0,
                        direct ? reinterpret_cast<T*>(out) : (T*)nullptr, out_stride) != cudaSuccess)
                 return MENTAT_ERR_CUDA;

@@ -19,6 +19,7 @@ from __future__ import annotations
 import ctypes as C
 import itertools
 import math
+import struct
 import weakref
 from typing import Optional
 
@@ -216,28 +217,45 @@ def prune_similar(sim: torch.Tensor, group_off: torch.Tensor, parent_key: torch.
 # ---------------------------------------------------------------------------
 # rotary positions, pages, sparse decode
 # ---------------------------------------------------------------------------
-def _call(device, what: str, fn, *args) -> None:
-    """``fn(*args, stream)`` on the device's current torch stream, with the device current."""
+try:
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+    from torch._C import _cuda_getDevice as _current_device
+except ImportError:  # the same through the public calls, about a microsecond slower each
+    _current_device = torch.cuda.current_device
+
+    def _raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
+
+
+def _call(device, name: str, *args) -> None:
+    """Entry point ``name`` on the device's current torch stream, with the device current."""
     if device.type != "cuda":
         raise RuntimeError("mentat_b200 runs on CUDA devices only")
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+    fn = _lib.call(name)
+    index = device.index
+    if index == _current_device():
+        status = fn(*args, _raw_stream(index))
     else:
-        _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        _lib.check(status, name)
 
 
-_NO_ROWS = C.byref(_lib.Rows())
+_pack_rows = struct.Struct("@Pqqi4x").pack  # mentat_rows
+_NO_ROWS = _pack_rows(0, 0, 0, 0)
 
 
-def _row_ref(t: torch.Tensor):
-    return C.byref(_lib.Rows(t.data_ptr(), t.stride(0), t.stride(1), t.shape[1]))
+def _row_ref(t: torch.Tensor) -> bytes:
+    s0, s1, _ = t.stride()
+    return _pack_rows(t.data_ptr(), s0, s1, t.shape[1])
 
 
 def _check_rows(name: str, t: torch.Tensor, n: int, d: int, dtype, device) -> torch.Tensor:
-    if t.dim() != 3 or t.shape[0] != n or t.shape[2] != d:
-        raise ValueError(f"{name} {tuple(t.shape)} is not ({n}, heads, {d})")
-    if t.dtype != dtype or dtype not in _DT:
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != n or shape[2] != d:
+        raise ValueError(f"{name} {tuple(shape)} is not ({n}, heads, {d})")
+    if t.dtype is not dtype or dtype not in _DT:
         raise TypeError(f"{name} has dtype {t.dtype}, {dtype if dtype in _DT else 'float32, bfloat16 or float16'} expected")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, {device} expected")
@@ -248,7 +266,7 @@ def _out_rows(name: str, out: Optional[torch.Tensor], x: torch.Tensor) -> torch.
     """``out`` checked as the result of a row operation on ``x``: its own rows distinct, and
     either ``x`` itself or apart from it; a new tensor if None."""
     if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        return x.new_empty(x.shape)
     n, h, d = x.shape
     if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError(f"{name} must have the input's shape, dtype and device")
@@ -276,7 +294,8 @@ def _check_positions(positions: torch.Tensor, n: int, device) -> torch.Tensor:
         raise ValueError(f"positions must be {n} int64 or int32 values")
     if positions.device != device:
         raise ValueError(f"positions are on {positions.device}, {device} expected")
-    return positions.to(torch.int64).contiguous()
+    return positions.to(torch.int64).contiguous() if positions.dtype is torch.int32 or n > 1 and positions.stride(0) != 1 \
+        else positions
 
 
 def _check_rotary(rotary, d: int, device) -> None:
@@ -312,9 +331,9 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         k = _check_rows("k", k, n, d, q.dtype, q.device)
         ko = _out_rows("k_out", k_out, k)
     if n:
-        _call(q.device, "mentat_rotary_apply", _lib.load().mentat_rotary_apply, _DT[q.dtype], d, n, _row_ref(q),
+        _call(q.device, "mentat_rotary_apply", _DT[q.dtype], d, n, _row_ref(q),
               _row_ref(qo), _NO_ROWS if k is None else _row_ref(k), _NO_ROWS if k is None else _row_ref(ko),
-              positions.data_ptr(), rotary._refs[bool(inverse)])
+              positions.data_ptr(), rotary._ptrs[bool(inverse)])
     return qo, ko
 
 
@@ -343,9 +362,9 @@ def rotary_append(cache, layer: int, rows: torch.Tensor, q: Optional[torch.Tenso
         q = _check_rows("q", q, n, d, cache.dtype, dev)
         qo = _out_rows("q_out", q_out, q)
     if n:
-        _call(dev, "mentat_rotary_append", _lib.load().mentat_rotary_append, cache._descp, layer, n, rows.data_ptr(),
+        _call(dev, "mentat_rotary_append", cache._desc_ptr, layer, n, rows.data_ptr(),
               _NO_ROWS if q is None else _row_ref(q), _NO_ROWS if q is None else _row_ref(qo), _row_ref(k), _row_ref(v),
-              positions.data_ptr(), rotary._refs[0])
+              positions.data_ptr(), rotary._ptrs[0])
     return qo
 
 
@@ -355,16 +374,15 @@ def _append_rotated(k_pool: torch.Tensor, v_pool: torch.Tensor, slots: torch.Ten
     token in its sequence; returns the turned queries.  ``rotary`` is the id that
     ``register_cache`` gave a ``Rotary``.  Wraps ``mentat_kv_append_rotated_batched``."""
     mgr, rot = _cache(cache), _cache(rotary)
-    lib = _lib.load()
     n, d = k.shape[0], k.shape[2]
     dev = mgr.device
     q, k, v = (_check_rows(name, t, n, d, mgr.dtype, dev) for name, t in (("q", q), ("k", k), ("v", v)))
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    qo = q.new_empty(q.shape)
     for a in range(0, n, 1024):
         b = min(n, a + 1024)
-        _call(dev, "append_rotated_batched", lib.mentat_kv_append_rotated_batched, mgr._descp, layer,
-              slots.data_ptr() + 4 * a, b - a, _row_ref(q[a:b]), _row_ref(qo[a:b]), _row_ref(k[a:b]), _row_ref(v[a:b]),
-              None, rot._refs[0])
+        _call(dev, "mentat_kv_append_rotated_batched", mgr._desc_ptr, layer,
+              slots.data_ptr() + 4 * a, b - a, *(_row_ref(x if n <= 1024 else x[a:b]) for x in (q, qo, k, v)),
+              None, rot._ptrs[0])
     if mgr.page_index is not None:
         _index_tails(mgr, layer, slots, n)
     return qo
@@ -387,8 +405,8 @@ def append_rotated(k_pool, v_pool, slots, q, k, v, cache, layer, rotary):
 
 def _index_tails(mgr, layer: int, slots: torch.Tensor, n: int) -> None:
     """Indexes each sequence's last page, if it is full (after a batched append)."""
-    _call(mgr.device, "mentat_page_index_seqs", _lib.load().mentat_page_index_seqs, mgr._descp, layer, slots.data_ptr(),
-          n, -1, 1, mgr.page_index._ref)
+    _call(mgr.device, "mentat_page_index_seqs", mgr._desc_ptr, layer, slots.data_ptr(),
+          n, -1, 1, mgr.page_index._ptr)
 
 
 def index_sequences(mgr, slots: torch.Tensor, first_page: int, max_pages: int, layer: int = -1) -> None:
@@ -397,12 +415,12 @@ def index_sequences(mgr, slots: torch.Tensor, first_page: int, max_pages: int, l
     step = max(1, 0x7fffffff // max(1, max_pages))
     for a in range(0, slots.shape[0], step):
         part = slots[a: a + step]
-        _call(mgr.device, "mentat_page_index_seqs", _lib.load().mentat_page_index_seqs, mgr._descp, layer,
-              part.data_ptr(), part.shape[0], first_page, max_pages, mgr.page_index._ref)
+        _call(mgr.device, "mentat_page_index_seqs", mgr._desc_ptr, layer,
+              part.data_ptr(), part.shape[0], first_page, max_pages, mgr.page_index._ptr)
 
 
 def _workspace(cache, n: int) -> tuple:
-    size = int(_lib.load().mentat_pages_workspace_bytes(cache._descp, n))
+    size = _lib.call("mentat_pages_workspace_bytes")(cache._desc_ptr, n)
     return torch.empty(size, dtype=torch.uint8, device=cache.device), size
 
 
@@ -419,7 +437,7 @@ def fork_pages(cache, parents: torch.Tensor, children: torch.Tensor, max_blocks:
     parents = _check_ids("parents", parents, dev, limit=MAX_SEQS_PER_PAGES_CALL)
     children = _check_ids("children", children, dev, parents.shape[0])
     hint = cache.table_capacity if max_blocks is None else max_blocks
-    _call(dev, "fork_pages", _lib.load().mentat_kv_fork_batched, cache._descp, parents.data_ptr(), children.data_ptr(),
+    _call(dev, "mentat_kv_fork_batched", cache._desc_ptr, parents.data_ptr(), children.data_ptr(),
           parents.shape[0], hint)
 
 
@@ -430,7 +448,7 @@ def free_pages(cache, slots: torch.Tensor, max_blocks: Optional[int] = None) -> 
     slots = _check_ids("slots", slots, dev, limit=MAX_SEQS_PER_PAGES_CALL)
     hint = cache.table_capacity if max_blocks is None else max_blocks
     ws, size = _workspace(cache, slots.shape[0])
-    _call(dev, "free_pages", _lib.load().mentat_kv_free_batched, cache._descp, slots.data_ptr(), slots.shape[0], hint,
+    _call(dev, "mentat_kv_free_batched", cache._desc_ptr, slots.data_ptr(), slots.shape[0], hint,
           ws.data_ptr(), size)
 
 
@@ -459,9 +477,9 @@ def compact_pages(cache, src: torch.Tensor, dst: Optional[torch.Tensor], keep: t
         _check_rotary(rotary, cache.head_dim, dev)
     hint = cache.table_capacity if max_blocks is None else max_blocks
     ws, size = _workspace(cache, n)
-    _call(dev, "compact_pages", _lib.load().mentat_kv_compact, cache._descp, src.data_ptr(),
+    _call(dev, "mentat_kv_compact", cache._desc_ptr, src.data_ptr(),
           None if dst is None else dst.data_ptr(), n, keep.data_ptr(), keep.stride(0) if per_layer else 0,
-          cu.data_ptr(), max_keep, hint, None if rotary is None else rotary._refs[0], ws.data_ptr(), size)
+          cu.data_ptr(), max_keep, hint, None if rotary is None else rotary._ptrs[0], ws.data_ptr(), size)
 
 
 def page_index(index, layer: int, blocks: torch.Tensor) -> None:
@@ -470,8 +488,8 @@ def page_index(index, layer: int, blocks: torch.Tensor) -> None:
     ``mentat_page_index_blocks``."""
     c = index.cache
     blocks = _check_ids("blocks", blocks, c.device)
-    _call(c.device, "page_index", _lib.load().mentat_page_index_blocks, c._descp, layer, blocks.data_ptr(),
-          blocks.shape[0], index._ref)
+    _call(c.device, "mentat_page_index_blocks", c._desc_ptr, layer, blocks.data_ptr(),
+          blocks.shape[0], index._ptr)
 
 
 def page_bounds(index, layer: int, blocks: torch.Tensor) -> tuple:
@@ -483,7 +501,7 @@ def page_bounds(index, layer: int, blocks: torch.Tensor) -> tuple:
     n, h, d = blocks.shape[0], c.num_key_value_heads, c.head_dim
     both = torch.empty((2, n, h, d), device=c.device)
     exps = torch.empty((n, h), dtype=torch.int8, device=c.device)
-    _call(c.device, "page_bounds", _lib.load().mentat_page_bounds, c._descp, layer, blocks.data_ptr(), n, index._ref,
+    _call(c.device, "mentat_page_bounds", c._desc_ptr, layer, blocks.data_ptr(), n, index._ptr,
           both[0].data_ptr(), both[1].data_ptr(), exps.data_ptr())
     return both[0], both[1], exps
 
@@ -506,13 +524,15 @@ def sparse_decode(index, layer: int, slots: torch.Tensor, q: torch.Tensor, max_l
     slots = _check_ids("slots", slots, c.device, n)
     if recent < 1 or sink < 0 or sink + recent > budget:
         raise ValueError(f"sink {sink} >= 0 and recent {recent} >= 1 pages must fit in the budget of {budget}")
-    out = torch.empty((n, hq, d), device=q.device, dtype=q.dtype)
-    pages = torch.empty((n, c.num_key_value_heads, budget), dtype=torch.int32, device=q.device) if return_pages else None
+    out = q.new_empty((n, hq, d))
+    pages = slots.new_empty((n, c.num_key_value_heads, budget)) if return_pages else None
     if n:
-        _call(c.device, "mentat_sparse_decode", _lib.load().mentat_sparse_decode, c._descp, layer, index._ref,
+        size = _lib.call("mentat_sparse_workspace_bytes")(c._desc_ptr, n, max_len, budget)
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+        _call(c.device, "mentat_sparse_decode", c._desc_ptr, layer, index._ptr,
               slots.data_ptr(), n, q.data_ptr(), q.stride(0), hq, out.data_ptr(), out.stride(0),
               default_scale(d) if scale is None else scale, max_len, budget, sink, recent,
-              None if pages is None else pages.data_ptr())
+              None if pages is None else pages.data_ptr(), None if ws is None else ws.data_ptr(), size)
     return (out, pages) if return_pages else out
 
 

@@ -251,7 +251,7 @@ class KVCacheView:
         d.max_seqs, d.max_blocks_per_seq = self.max_seqs, self.table_capacity
         for name, t in self._tensors.items():
             setattr(d, name, None if t is None else t.data_ptr())
-        self._desc, self._descp = d, C.byref(d)
+        self._desc, self._descp, self._desc_ptr = d, C.byref(d), C.addressof(d)
         self.page_index = None
 
     def check(self) -> None:
@@ -279,7 +279,7 @@ class PageIndex:
                 raise ValueError(f"{name} must be contiguous int8 {want} on {dev}")
         self.cache, self.bounds, self.exps = cache, bounds, exps
         self._desc = _lib.PageIndex(bounds.data_ptr(), exps.data_ptr())
-        self._ref = C.byref(self._desc)
+        self._ptr = C.addressof(self._desc)
 
 
 class PagedKVCacheManager:
@@ -337,7 +337,7 @@ class PagedKVCacheManager:
         d.nblocks, d.ntok = self._nblocks.data_ptr(), self._ntok.data_ptr()
         d.tail, d.scratch = self._tail.data_ptr(), self._scratch.data_ptr()
         self._desc = d
-        self._descp = C.byref(d)
+        self._descp, self._desc_ptr = C.byref(d), C.addressof(d)
 
         order = None
         if free_order is not None:
@@ -669,9 +669,9 @@ class PagedKVCacheManager:
         first = seq.num_tokens[layer_idx]
         self._mirror_append(seq, layer_idx, n)
         none = ops._NO_ROWS
-        ops._call(self.device, "append_rotated", self._lib.mentat_kv_append_rotated, self._descp, layer_idx, seq.slot, n,
+        ops._call(self.device, "mentat_kv_append_rotated", self._desc_ptr, layer_idx, seq.slot, n,
                   none if q is None else ops._row_ref(q), none if q is None else ops._row_ref(qo), ops._row_ref(k),
-                  ops._row_ref(v), None if positions is None else positions.data_ptr(), rotary._refs[0])
+                  ops._row_ref(v), None if positions is None else positions.data_ptr(), rotary._ptrs[0])
         self._index_appended(seq, layer_idx, first)
         self._after()
         return qo

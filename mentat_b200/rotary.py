@@ -143,7 +143,7 @@ class Rotary:
         self.attention_scaling = 1.0 if attention_scaling is None else float(attention_scaling)
         self._args = tuple(_lib.Rotary(self.inv_freq.data_ptr(), self.rotary_dim // 2, offset, int(self.interleaved),
                                        inverse, self.attention_scaling) for inverse in (0, 1))
-        self._refs = tuple(C.byref(a) for a in self._args)
+        self._ptrs = tuple(C.addressof(a) for a in self._args)
         self.op_id = ops.register_cache(self)  # the id that torch operators take
 
     @classmethod

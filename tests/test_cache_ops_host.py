@@ -173,13 +173,16 @@ def test_c_abi_refuses_sparse_arguments():
 
     def decode(c=_desc(), layer=0, idx=x, slots=4096, n=2, hq=4, scale=0.1, longest=100, budget=8, sink=1, recent=1):
         return lib.mentat_sparse_decode(c, layer, idx, slots, n, 4096, hq * 64, hq, 4096, hq * 64, scale, longest,
-                                        budget, sink, recent, None, None)
+                                        budget, sink, recent, None, None, 0, None)
     assert decode(n=0) == 0
     for bad in (dict(layer=2), dict(idx=_lib.PageIndex(None, 4096)), dict(idx=_lib.PageIndex(4097, 4096)),
                 dict(slots=None), dict(hq=3), dict(scale=0.0), dict(scale=float("nan")), dict(longest=-1),
                 dict(budget=0), dict(sink=-1), dict(recent=0), dict(sink=4, recent=5), dict(c=_desc(k_pool=4100)),
                 dict(c=_desc(tables=None))):
         assert decode(**bad) == ARG, bad
+    assert lib.mentat_sparse_workspace_bytes(_desc(), 2, 100, 8) == 0      # a small batch needs none
+    need = lib.mentat_sparse_workspace_bytes(_desc(), 500, 1000, 8)
+    assert need >= 4 * 500 * 2 * (63 + 8) and decode(n=500, longest=1000) == ARG
     assert decode(hq=34) == UNSUPPORTED and decode(budget=8193) == UNSUPPORTED
     assert decode(c=_desc(head_dim=96)) == UNSUPPORTED and decode(c=_desc(dtype=5)) == UNSUPPORTED
     assert lib.mentat_page_index_blocks(_desc(), 0, None, 1, x, None) == ARG

@@ -147,6 +147,28 @@ def test_many_pages():
         run_and_check(c, x, q, tables, lens, budget, 1, 2, "bf16", layer=0)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_more_pages_than_one_block_holds(dtype):
+    """Pages of one token: 40,000 and 17,000 of them, and a batch beside them without a choice to make."""
+    lens = [40000, 30, 17000]
+    c, x, q, tables = make(lens, 2, 1, 64, 1, dtype, layers=1, shared=7000)
+    run_and_check(c, x, q, tables, lens, 33, 2, 3, dtype, layer=0)
+    x.exps.zero_()
+    x.bounds.zero_()  # all the same: the lowest
+    run_and_check(c, x, q, tables, lens, 33, 2, 3, dtype, layer=0)
+
+
+def test_batches_of_trees():
+    """Batches with a launch of their own for the scores: rows that share all, some or none of their pages,
+    rows without a choice, corrupt and empty ones among them, groups that do not divide the columns."""
+    rng = np.random.default_rng(5)
+    for hq, hkv, d, n in ((24, 8, 64, 41), (10, 2, 128, 90), (16, 1, 64, 160)):
+        lens = [int(v) for v in rng.integers(1, 900, n)]
+        lens[3], lens[5], lens[n - 1] = 0, 17, 897
+        c, x, q, tables = make(lens, hq, hkv, d, 16, "bf16", layers=1, shared=21)
+        run_and_check(c, x, q, tables, lens, 8, 1, 2, "bf16", layer=0)
+
+
 def test_ties_go_to_the_lowest_page():
     from mentat_b200 import ops
     lens = [2000]
