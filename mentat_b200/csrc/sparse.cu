@@ -922,11 +922,12 @@ __global__ void __launch_bounds__(SPARSE_THREADS) k_sparse(const __grid_constant
 // large batches: scores, choice and attention in three launches
 // ---------------------------------------------------------------------------
 // Adjacent sequences of a tree share most of their pages, so a CTA scores its pages for several
-// of them at once: the query heads of up to 64 / GP sequences are the columns of the
-// product (GP columns each, the group rounded up to a power of two; the columns past the group
-// have no part), and where all of them have the same 16 blocks the bounds are read once.  Two warps take 16 pages, half of the columns each; pages that the sequences do not share are
-// scored sequence by sequence, spread over all warps.
-constexpr int SCORE_COLS = 64, SCORE_PAGES = 64, SCORE_THREADS = 256, SCORE_WARPS = SCORE_THREADS / 32;
+// of them at once: the query heads of up to 16 sequences are the columns of the product (GP columns each,
+// the group rounded up to a power of two; the columns past the group have no part; at most 64 columns), and
+// where all of them have the same 16 blocks the bounds are read once.  Two warps take 16 pages, half of the
+// columns each, or, where the pages are not shared, every second sequence each; a warp has the next pages'
+// bounds and the blocks of those after them on the way while it works.
+constexpr int SCORE_THREADS = 256, SCORE_TILES = SCORE_THREADS / 64;  // tiles of 16 pages at a time
 
 // The query heads in 8 bits, [n][Hq][2 D], negative part and positive part, and their units.
 template <typename T, int D>
@@ -954,14 +955,20 @@ __device__ __forceinline__ void score_product(const int4 (&v)[2][2 * D / 64], co
     }
 }
 
+template <int GP>
+struct ScoreShape {  // sequences and columns of a CTA
+    static constexpr int ROWS = GP > 4 ? 64 / GP : 16, COLS = ROWS * GP;
+};
+
 template <int D, int GP>
-__global__ void __launch_bounds__(SCORE_THREADS) k_score(mentat_kv_cache c, mentat_page_index x, SparseArgs a,
+__global__ void __launch_bounds__(SCORE_THREADS, 2) k_score(mentat_kv_cache c, mentat_page_index x, SparseArgs a,
                                                          const uint4* q8, const float* units) {
-    constexpr int ROWS = SCORE_COLS / GP, CH = 2 * D / 64, QS = 2 * D + 16;  // a column's bytes, padded against bank conflicts
-    constexpr int TILES = SCORE_PAGES / 16, HALF = SCORE_COLS / 16;           // tiles of pages, column tiles of a warp
-    extern __shared__ __align__(16) uint8_t smem_q[];  // [SCORE_COLS][QS]
-    __shared__ __align__(8) float s_unit[SCORE_COLS];
-    __shared__ int s_pages[ROWS], s_shared[TILES], s_first[SCORE_PAGES];
+    constexpr int ROWS = ScoreShape<GP>::ROWS, COLS = ScoreShape<GP>::COLS, IDS = ROWS / 2;
+    constexpr int CH = 2 * D / 64, QS = 2 * D + 16;  // a column's bytes, padded against bank conflicts
+    constexpr int HALF = COLS / 16;                  // column tiles of a warp
+    extern __shared__ __align__(16) uint8_t smem_q[];  // [COLS][QS]
+    __shared__ __align__(8) float s_unit[COLS];
+    __shared__ int s_pages[ROWS];
     __shared__ const int32_t* s_row[ROWS];
     griddep_wait();
     griddep_launch();
@@ -985,9 +992,10 @@ __global__ void __launch_bounds__(SCORE_THREADS) k_score(mentat_kv_cache c, ment
         s_row[tid] = P ? table_row(c, a.layer, slot) : nullptr;
     }
     if (tid < ROWS) s_pages[tid] = P;  // 0 for the sequences past the batch
-    const int p0 = blockIdx.x * SCORE_PAGES;
-    if (!__syncthreads_or(P > p0 && P > a.budget)) return;  // past every end, or nothing to choose
-    for (int w = tid; w < SCORE_COLS * (D / 8); w += SCORE_THREADS) {
+    // neighbouring tiles go to different CTAs: the ones that are not shared lie together
+    const int tile0 = (warp >> 1) * gridDim.x + blockIdx.x, step = gridDim.x * SCORE_TILES, half = warp & 1;
+    if (!__syncthreads_or(P > (int)blockIdx.x * 16 && P > a.budget)) return;  // nothing to choose
+    for (int w = tid; w < COLS * (D / 8); w += SCORE_THREADS) {
         const int col = w / (D / 8), ch = w % (D / 8), i = col / GP, e = col % GP;
         const int src = i < rows && e < G ? 16 : 0;
         const uint4* from = q8 + ((int64_t)(n0 + min(i, rows - 1)) * Hq + h * G + min(e, G - 1)) * (D / 8) + ch;
@@ -996,58 +1004,50 @@ __global__ void __launch_bounds__(SCORE_THREADS) k_score(mentat_kv_cache c, ment
                      : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    if (tid < SCORE_COLS) {  // a column without a head: NaN, which no maximum takes
+    if (tid < COLS) {  // a column without a head: NaN, which no maximum takes
         const int i = tid / GP, e = tid % GP;
         s_unit[tid] = i < rows && e < G ? units[(int64_t)(n0 + i) * Hq + h * G + e] : __int_as_float(0x7fffffff);
     }
-    auto block_of = [&](int i, int pp) {  // of sequence i's page, -1 if it has none (or none that can be read)
-        if (pp >= s_pages[i]) return -1;
-        const int id = s_row[i][pp];
-        if ((unsigned)id < (unsigned)c.num_blocks) return id;
-        set_error(c, MENTAT_DEV_BAD_BLOCK, id);
-        return -1;
+    int most = 0;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) most = max(most, s_pages[i]);
+    const int tiles = (most + 15) / 16;
+    const int64_t base = (int64_t)a.layer * c.num_blocks;
+
+    // a lane's blocks of tile tl: page lane % 16 of every second sequence; NONE where a sequence has no such page
+    constexpr int NONE = -2147483647 - 1;
+    auto fetch = [&](int tl, int (&id)[IDS]) {
+        const int pp = tl * 16 + (lane & 15);
+#pragma unroll
+        for (int e = 0; e < IDS; ++e) {
+            const int i = 2 * e + (lane >> 4);
+            id[e] = pp < s_pages[i] ? s_row[i][pp] : NONE;
+        }
     };
-    if (warp < TILES) {  // whether every sequence that has a tile's pages has the same blocks there
-        const int pp = p0 + warp * 16 + (lane & 15);
-        int first = -1;
+    // whether every sequence that has the tile's pages has the same (readable) blocks there; `first`: the blocks
+    auto common = [&](const int (&id)[IDS], int& first) {
+        first = -1;
         bool same = true;
 #pragma unroll
-        for (int i0 = 0; i0 < ROWS; i0 += 16) {
-            int id[8];  // requested together
-            bool has[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int i = i0 + 2 * e + (lane >> 4);
-                has[e] = i < ROWS && pp < s_pages[i < ROWS ? i : 0];
-                id[e] = has[e] ? s_row[i][pp] : -1;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                // with an entry that cannot be read the tile is scored sequence by sequence
-                const bool good = (unsigned)id[e] < (unsigned)c.num_blocks;
-                if (good && first < 0) first = id[e];
-                same = same && (!has[e] || (good && id[e] == first));
-            }
+        for (int e = 0; e < IDS; ++e) {
+            const bool good = (unsigned)id[e] < (unsigned)c.num_blocks;
+            if (good && first < 0) first = id[e];
+            same = same && (id[e] == NONE || (good && id[e] == first));
         }
         const int other = __shfl_xor_sync(0xffffffffu, first, 16);
         same = same && (first < 0 || other < 0 || first == other);
         first = first < 0 ? other : first;
-        const bool all = __all_sync(0xffffffffu, same);
-        if (lane == 0) s_shared[warp] = all;
-        if (lane < 16) s_first[warp * 16 + lane] = first;
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();
-    const int64_t base = (int64_t)a.layer * c.num_blocks;
-    // the bounds of pages p0 + at + g and p0 + at + 8 + g in blocks id[0], id[1] (-1: any)
-    auto load = [&](const int (&id)[2], int4 (&v)[2][CH], int (&ek)[2]) {
+        return (bool)__all_sync(0xffffffffu, same);
+    };
+    // the bounds of pages g and 8 + g of a tile, in blocks b0 and b1 (-1: any)
+    auto load = [&](int b0, int b1, int4 (&v)[2][CH], int (&ek)[2]) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const int64_t at = (base + max(id[r], 0)) * H + h;
-            ek[r] = x.exps[at];
+            const int64_t at = (base + max(r ? b1 : b0, 0)) * H + h;
+            ek[r] = __ldg(x.exps + at);
             const int4* src = reinterpret_cast<const int4*>(x.bounds + at * 2 * D) + t;
 #pragma unroll
-            for (int ch = 0; ch < CH; ++ch) v[r][ch] = src[ch * 4];
+            for (int ch = 0; ch < CH; ++ch) v[r][ch] = __ldg(src + ch * 4);
         }
     };
     // of a sequence's columns in one column tile, the highest score for page g (r 0) or g + 8; u: the lane's units
@@ -1068,80 +1068,104 @@ __global__ void __launch_bounds__(SCORE_THREADS) k_score(mentat_kv_cache c, ment
     };
     auto unit_of = [&](int nt) { return *reinterpret_cast<const float2*>(s_unit + nt * 8 + 2 * t); };
     const uint8_t* cols = smem_q + g * QS + t * 16;
-    static_assert(SCORE_WARPS == 2 * TILES, "two warps for 16 pages");
-    const int tile = warp >> 1, pt = p0 + tile * 16;
-    if (s_shared[tile]) {
-        int4 v[2][CH];
-        int ek[2];
-        const int id[2] = {s_first[tile * 16 + g], s_first[tile * 16 + 8 + g]};
-        load(id, v, ek);
-        int d[HALF][4];
-        const int nt0 = (warp & 1) * HALF;
-        score_product<D, HALF>(v, cols + nt0 * 8 * QS, d);
+
+    int id[IDS], now[IDS], first, ek[2];  // now: the blocks of the tile in hand, if it is not shared
+    int4 v[2][CH];
+    int tl = tile0;
+    bool shared = false;
+    if (tl < tiles) {
+        fetch(tl, id);
+        shared = common(id, first);
+        if (shared) load(__shfl_sync(0xffffffffu, first, g), __shfl_sync(0xffffffffu, first, 8 + g), v, ek);
 #pragma unroll
-        for (int k = 0; k < HALF; ++k) {
-            const int nt = nt0 + k;
-            const float2 u = unit_of(nt);
+        for (int e = 0; e < IDS; ++e) now[e] = id[e];
+        if (tl + step < tiles) fetch(tl + step, id);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    for (; tl < tiles; tl += step) {
+        // the next tile's bounds, and the blocks of the one after it
+        int4 nv[2][CH];
+        int nek[2] = {0, 0}, nid[IDS];
+        bool next_shared = false;
+        if (tl + step < tiles) {
+            next_shared = common(id, first);
+            if (next_shared) load(__shfl_sync(0xffffffffu, first, g), __shfl_sync(0xffffffffu, first, 8 + g), nv, nek);
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int pp = pt + r * 8 + g;
-                if (GP == 1) {  // each column is a sequence
-                    put(nt * 8 + 2 * t, pp, (float)d[k][2 * r] * u.x, ek[r]);
-                    put(nt * 8 + 2 * t + 1, pp, (float)d[k][2 * r + 1] * u.y, ek[r]);
-                } else if (GP <= 8) {
-                    const float best = highest(d[k], u, r);
-                    if (t % (GP > 2 ? GP / 2 : 1) == 0) put((nt * 8 + 2 * t) / GP, pp, best, ek[r]);
-                } else if (k % 2 == 0) {
-                    const float best = fmaxf(highest(d[k], u, r), highest(d[(k + 1) % HALF], unit_of(nt + 1), r));
-                    if (t == 0) put(nt / 2, pp, best, ek[r]);
+            for (int e = 0; e < IDS; ++e) nid[e] = id[e];
+            if (tl + 2 * step < tiles) fetch(tl + 2 * step, id);
+        }
+        const int pt = tl * 16;
+        if (shared) {
+            int d[HALF][4];
+            const int nt0 = half * HALF;
+            score_product<D, HALF>(v, cols + nt0 * 8 * QS, d);
+#pragma unroll
+            for (int k = 0; k < HALF; ++k) {
+                const int nt = nt0 + k;
+                const float2 u = unit_of(nt);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int pp = pt + r * 8 + g;
+                    if (GP == 1) {  // each column is a sequence
+                        put(nt * 8 + 2 * t, pp, (float)d[k][2 * r] * u.x, ek[r]);
+                        put(nt * 8 + 2 * t + 1, pp, (float)d[k][2 * r + 1] * u.y, ek[r]);
+                    } else if (GP <= 8) {
+                        const float best = highest(d[k], u, r);
+                        if (t % (GP > 2 ? GP / 2 : 1) == 0) put((nt * 8 + 2 * t) / GP, pp, best, ek[r]);
+                    } else if (k % 2 == 0) {
+                        const float best = fmaxf(highest(d[k], u, r), highest(d[(k + 1) % HALF], unit_of(nt + 1), r));
+                        if (t == 0) put(nt / 2, pp, best, ek[r]);
+                    }
+                }
+            }
+        } else {
+            // sequence 2 e + half's blocks are in the lanes from 16 half; the next sequence's bounds are on the
+            // way while one is scored
+            constexpr int N1 = GP > 8 ? 2 : 1;
+            auto load_one = [&](int e, int4 (&v)[2][CH], int (&ek)[2]) {
+                int b[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    b[r] = __shfl_sync(0xffffffffu, now[e], 16 * half + 8 * r + g);
+                    if (b[r] != NONE && (unsigned)b[r] >= (unsigned)c.num_blocks) {
+                        if (t == 0) set_error(c, MENTAT_DEV_BAD_BLOCK, b[r]);
+                        b[r] = -1;
+                    }
+                }
+                load(b[0], b[1], v, ek);
+            };
+            load_one(0, v, ek);
+#pragma unroll
+            for (int e = 0; e < IDS; ++e) {
+                const int i = 2 * e + half, nt = i * GP / 8, col = i * GP % 8;  // its first column in its tile
+                const int ex[2] = {ek[0], ek[1]};
+                int d[N1][4];
+                score_product<D, N1>(v, cols + nt * 8 * QS, d);
+                if (e + 1 < IDS) load_one(e + 1 < IDS ? e + 1 : 0, v, ek);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int pp = pt + r * 8 + g;
+                    const float2 u = unit_of(nt);
+                    if (GP == 1) {
+                        if (t == col / 2) put(i, pp, (float)d[0][2 * r + (col & 1)] * (col & 1 ? u.y : u.x), ex[r]);
+                    } else {
+                        float best = highest(d[0], u, r);
+                        if (GP > 8) best = fmaxf(best, highest(d[N1 - 1], unit_of(nt + N1 - 1), r));
+                        if (t == col / 2) put(i, pp, best, ex[r]);
+                    }
                 }
             }
         }
-    }
-    // (tile, sequence) pairs of the tiles that are not shared, each one's bounds on the way while the one
-    // before it is scored
-    constexpr int N1 = GP > 8 ? 2 : 1;
-    struct Pair {
-        int tl, i, ek[2];
-        int4 v[2][CH];
-    };
-    auto fetch = [&](int& y, Pair& w) {  // the next such pair from y, in steps of the warps
-        for (; y < TILES * ROWS; y += SCORE_WARPS) {
-            w.tl = y / ROWS;
-            w.i = y % ROWS;
-            if (s_shared[w.tl] || p0 + w.tl * 16 >= s_pages[w.i]) continue;
-            const int id[2] = {block_of(w.i, p0 + w.tl * 16 + g), block_of(w.i, p0 + w.tl * 16 + 8 + g)};
-            load(id, w.v, w.ek);
-            y += SCORE_WARPS;
-            return true;
-        }
-        return false;
-    };
-    auto score = [&](const Pair& w) {
-        int d[N1][4];
-        const int nt = w.i * GP / 8;
-        score_product<D, N1>(w.v, cols + nt * 8 * QS, d);
+        shared = next_shared;
+#pragma unroll
+        for (int e = 0; e < IDS; ++e) now[e] = nid[e];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const int pp = p0 + w.tl * 16 + r * 8 + g, col = w.i * GP % 8;  // the sequence's first column in its tile
-            const float2 u = unit_of(nt);
-            if (GP == 1) {
-                if (t == col / 2) put(w.i, pp, (float)d[0][2 * r + (col & 1)] * (col & 1 ? u.y : u.x), w.ek[r]);
-            } else {
-                float best = highest(d[0], u, r);
-                if (GP > 8) best = fmaxf(best, highest(d[N1 - 1], unit_of(nt + N1 - 1), r));
-                if (t == col / 2) put(w.i, pp, best, w.ek[r]);
-            }
+            ek[r] = nek[r];
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch) v[r][ch] = nv[r][ch];
         }
-    };
-    int y = warp;
-    Pair w0, w1;
-    bool more = fetch(y, w0);
-    while (more) {
-        const bool two = fetch(y, w1);
-        score(w0);
-        more = two && fetch(y, w0);
-        if (two) score(w1);
     }
 }
 
@@ -1182,23 +1206,24 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) k_choose(mentat_kv_cache c, Sp
 // ---------------------------------------------------------------------------
 // launch
 // ---------------------------------------------------------------------------
-// Whether a batch's scores and choice get launches of their own.
+// How many CTAs share one (sequence, KV head): the largest power of two up to 8 that still runs all CTAs at
+// once (two on an SM with the rings of the tensor-core path, four without).  One sequence of 4,000 tokens,
+// 8 KV heads, budget 64: 24.9 / 17.3 / 13.1 / 11.4 us with 1 / 2 / 4 / 8; 16 sequences: 28.6 / 21.8 / 29.6 / 50.
+static int sparse_cluster(int heads, bool mma) {
+    int cs = 1;
+    while (cs < 8 && (int64_t)heads * cs * 2 <= 148 * (mma ? 2 : 4)) cs *= 2;
+    return cs;
+}
+static bool sparse_mma(const mentat_kv_cache* c) { return c->dtype != MENTAT_F32 && c->block_size % 16 == 0; }
+
+// Whether the scores and the choice get launches of their own: from 600 pages for each CTA to score (and past
+// what k_sparse can hold).  Sequences of up to 1,000 pages, budget 64: 16 of them 33.6 us in one launch and 35.7
+// in several, 24 of them 56 and 50; with a 32,768-token prefix in common 8 of them 28.8 and 29.6, 16 of
+// them 43 and 39, 64 of them 159 and 91.
 static bool sparse_listed(const mentat_kv_cache* c, int n, int max_len, int budget) {
-    static const int forced = [] { const char* e = getenv("MENTAT_SPARSE_LISTED"); return e && *e ? atoi(e) : -1; }();
     const int64_t pages = ((int64_t)max_len + c->block_size - 1) / c->block_size;
     if (pages <= budget) return false;
-    if (pages > HELD_PAGES) return true;
-    if (forced >= 0) return forced;
-    return n * c->num_kv_heads >= 148;
-}
-
-// How many CTAs share one (sequence, KV head): a power of two.
-static int sparse_cluster(int heads) {
-    static const int forced = [] { const char* e = getenv("MENTAT_SPARSE_CLUSTER"); return e && *e ? atoi(e) : 0; }();
-    if (forced) return forced;
-    int cs = 1;
-    while (cs < 8 && (int64_t)heads * cs * 2 <= 148 * 4) cs *= 2;
-    return cs;
+    return pages > HELD_PAGES || pages > 600 * sparse_cluster(n * c->num_kv_heads, sparse_mma(c));
 }
 
 // A kernel over clusters of cs CTAs.
@@ -1231,7 +1256,7 @@ static int launch_cluster(void (*kernel)(KArgs...), int cs, dim3 grid, int threa
 
 template <typename T, int D, int GM, bool MMA, bool LISTED>
 static int launch_sparse(const mentat_kv_cache* c, const mentat_page_index* x, SparseArgs a, cudaStream_t s) {
-    const int pages = (a.max_len + c->block_size - 1) / c->block_size, cs = sparse_cluster(a.n * c->num_kv_heads);
+    const int pages = (a.max_len + c->block_size - 1) / c->block_size, cs = sparse_cluster(a.n * c->num_kv_heads, MMA);
     a.held = pages;
     a.share = (min(pages, a.budget) + cs - 1) / cs;
     const size_t smem = 4 * (size_t)sparse_smem(a.G, GM, D, MMA, LISTED, a.held, a.share).total + 1024;
@@ -1246,7 +1271,7 @@ template <typename T, int D, int GM, bool LISTED>
 static int launch_sparse_kind(const mentat_kv_cache* c, const mentat_page_index* x, const SparseArgs& a,
                               cudaStream_t s) {
     if constexpr (sizeof(T) == 2)
-        if (c->block_size % 16 == 0 && a.qs % 4 == 0 && (uintptr_t)a.q % 8 == 0)
+        if (sparse_mma(c) && a.qs % 4 == 0 && (uintptr_t)a.q % 8 == 0)
             return launch_sparse<T, D, (GM > 8 ? 16 : 8), true, LISTED>(c, x, a, s);
     return launch_sparse<T, D, GM, false, LISTED>(c, x, a, s);
 }
@@ -1262,9 +1287,12 @@ static int launch_sparse_group(const mentat_kv_cache* c, const mentat_page_index
 
 template <int D, int GP>
 static int launch_score(const mentat_kv_cache* c, const mentat_page_index* x, const SparseArgs& a, cudaStream_t s) {
-    const int pages = (a.max_len + c->block_size - 1) / c->block_size, rows = SCORE_COLS / GP;
-    const dim3 grid((pages + SCORE_PAGES - 1) / SCORE_PAGES, c->num_kv_heads, (a.n + rows - 1) / rows);
-    MENTAT_LAUNCH((k_score<D, GP>), grid, dim3(SCORE_THREADS), SCORE_COLS * (2 * D + 16), s, *c, *x, a,
+    constexpr int ROWS = ScoreShape<GP>::ROWS;
+    const int pages = (a.max_len + c->block_size - 1) / c->block_size, per = SCORE_TILES * 16;
+    const int groups = c->num_kv_heads * ((a.n + ROWS - 1) / ROWS), chunks = (pages + per - 1) / per;
+    const int wanted = groups < 2 * 148 ? 2 * 148 / groups : 1;  // all CTAs at once, two on an SM
+    const dim3 grid(wanted < chunks ? wanted : chunks, c->num_kv_heads, (a.n + ROWS - 1) / ROWS);
+    MENTAT_LAUNCH((k_score<D, GP>), grid, dim3(SCORE_THREADS), ScoreShape<GP>::COLS * (2 * D + 16), s, *c, *x, a,
                   reinterpret_cast<const uint4*>(a.q8), a.units);
     return MENTAT_OK;
 }

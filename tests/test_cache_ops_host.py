@@ -181,8 +181,9 @@ def test_c_abi_refuses_sparse_arguments():
                 dict(c=_desc(tables=None))):
         assert decode(**bad) == ARG, bad
     assert lib.mentat_sparse_workspace_bytes(_desc(), 2, 100, 8) == 0      # a small batch needs none
-    need = lib.mentat_sparse_workspace_bytes(_desc(), 500, 1000, 8)
-    assert need >= 4 * 500 * 2 * (63 + 8) and decode(n=500, longest=1000) == ARG
+    long = _desc(max_blocks_per_seq=2000)
+    need = lib.mentat_sparse_workspace_bytes(long, 500, 20000, 8)
+    assert need >= 4 * 500 * 2 * (1250 + 8) and decode(c=long, n=500, longest=20000) == ARG
     assert decode(hq=34) == UNSUPPORTED and decode(budget=8193) == UNSUPPORTED
     assert decode(c=_desc(head_dim=96)) == UNSUPPORTED and decode(c=_desc(dtype=5)) == UNSUPPORTED
     assert lib.mentat_page_index_blocks(_desc(), 0, None, 1, x, None) == ARG
