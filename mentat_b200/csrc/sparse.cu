@@ -79,18 +79,120 @@ __device__ __forceinline__ void index_page(const mentat_kv_cache& c, int layer, 
     __syncthreads();
 }
 
+// min and max that keep a NaN, packed where the type is 16 bits
+template <typename T> struct Extreme;
+template <> struct Extreme<float> {
+    static constexpr int N = 1;
+    using V = float;
+    __device__ __forceinline__ static V lo(V a, V b) {
+        V d;
+        asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+        return d;
+    }
+    __device__ __forceinline__ static V hi(V a, V b) {
+        V d;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+        return d;
+    }
+    __device__ __forceinline__ static float get(V a, int) { return a; }
+};
+template <> struct Extreme<__nv_bfloat16> {
+    static constexpr int N = 2;
+    using V = __nv_bfloat162;
+    __device__ __forceinline__ static V lo(V a, V b) { return __hmin2_nan(a, b); }
+    __device__ __forceinline__ static V hi(V a, V b) { return __hmax2_nan(a, b); }
+    __device__ __forceinline__ static float get(V a, int i) { return __bfloat162float(i ? a.y : a.x); }
+};
+template <> struct Extreme<__half> {
+    static constexpr int N = 2;
+    using V = __half2;
+    __device__ __forceinline__ static V lo(V a, V b) { return __hmin2_nan(a, b); }
+    __device__ __forceinline__ static V hi(V a, V b) { return __hmax2_nan(a, b); }
+    __device__ __forceinline__ static float get(V a, int i) { return __half2float(i ? a.y : a.x); }
+};
+
+// The index of all heads of one block by one CTA, 16 bytes of a row to a thread (head_dim / VEC threads to a
+// head, a power of two within a warp, every thread of which takes part); the page is read once, 8 rows of a
+// thread on the way at a time.  Bound by memory.
 template <typename T>
+__device__ __forceinline__ void index_block(const mentat_kv_cache& c, int layer, int b, const mentat_page_index& x) {
+    using E = Extreme<T>;
+    constexpr int VEC = 16 / sizeof(T), W = VEC / E::N;
+    using Row = Pack<typename E::V, W>;
+    const int D = c.head_dim, H = c.num_kv_heads, per = D / VEC, n = H * per, bs = c.block_size;
+    const Row* k = reinterpret_cast<const Row*>(reinterpret_cast<const T*>(c.k_pool) + pool_row(c, layer, b, 0));
+    for (int u0 = 0; u0 < n; u0 += blockDim.x) {
+        const int u = u0 + threadIdx.x, at = min(u, n - 1);
+        Row lo = k[at], hi = lo;
+        for (int r = 1; r < bs; r += 8) {
+            Row v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = k[(int64_t)min(r + e, bs - 1) * n + at];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    lo.v[w] = E::lo(lo.v[w], v[e].v[w]);
+                    hi.v[w] = E::hi(hi.v[w], v[e].v[w]);
+                }
+        }
+        float top = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+#pragma unroll
+            for (int e = 0; e < E::N; ++e) {
+                const float l = E::get(lo.v[w], e), g = E::get(hi.v[w], e);
+                bad |= !isfinite(l) || !isfinite(g);
+                top = fmaxf(top, fmaxf(fabsf(l), fabsf(g)));
+            }
+        if (bad) top = INFINITY;
+        for (int o = 1; o < per; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        bad = isinf(top);
+        const int e = bad ? 0 : unit_exponent(top);
+        const float inv = pow2(-e);
+        Pack<int8_t, VEC> ol, oh;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+#pragma unroll
+            for (int i = 0; i < E::N; ++i) {
+                const float l = E::get(lo.v[w], i), g = E::get(hi.v[w], i);
+                ol.v[w * E::N + i] = bad ? 0 : (int8_t)fminf(fmaxf(floorf(l * inv), -127.f), 127.f);
+                oh.v[w * E::N + i] = bad ? 0 : (int8_t)fminf(fmaxf(ceilf(g * inv), -127.f), 127.f);
+            }
+        if (u < n) {
+            const int h = u / per, d = (u - h * per) * VEC;
+            const int64_t to = ((int64_t)layer * c.num_blocks + b) * H + h;
+            int8_t* o = x.bounds + to * 2 * D + d;
+            *reinterpret_cast<Pack<int8_t, VEC>*>(o) = ol;
+            *reinterpret_cast<Pack<int8_t, VEC>*>(o + D) = oh;
+            if (d == 0) x.exps[to] = (int8_t)(bad ? EXP_ALL : e);
+        }
+    }
+}
+// threads of a CTA that index_block can use, 0 if the head does not divide into them
+static int index_block_threads(const mentat_kv_cache* c) {
+    const int vec = 16 / dtype_bytes(c->dtype), per = c->head_dim / vec;
+    if (c->head_dim % vec || per > 32 || (per & (per - 1)) || (uintptr_t)c->k_pool % 16) return 0;
+    const int n = (c->num_kv_heads * per + 31) / 32 * 32;
+    return n < 256 ? n : 256;
+}
+
+// One CTA per block (WIDE), or per block and head.
+template <typename T, bool WIDE>
 __global__ void k_index_blocks(mentat_kv_cache c, int layer, const int32_t* blocks, mentat_page_index x) {
     griddep_wait();
+    griddep_launch();
     const int b = blocks[blockIdx.x];
     if ((unsigned)b >= (unsigned)c.num_blocks) {
         if (threadIdx.x == 0) set_error(c, MENTAT_DEV_BAD_BLOCK, b);
         return;
     }
-    index_page<T>(c, layer, b, blockIdx.y, x);
+    if constexpr (WIDE) index_block<T>(c, layer, b, x);
+    else index_page<T>(c, layer, b, blockIdx.y, x);
 }
 
-template <typename T>
+template <typename T, bool WIDE>
 __global__ void k_index_seqs(mentat_kv_cache c, int layer0, const int32_t* slots, int first, mentat_page_index x,
                              int max_pages) {
     griddep_wait();
@@ -113,26 +215,39 @@ __global__ void k_index_seqs(mentat_kv_cache c, int layer0, const int32_t* slots
         if (threadIdx.x == 0) set_error(c, MENTAT_DEV_BAD_BLOCK, b);
         return;
     }
-    index_page<T>(c, layer, b, blockIdx.y, x);
+    if constexpr (WIDE) index_block<T>(c, layer, b, x);
+    else index_page<T>(c, layer, b, blockIdx.y, x);
 }
 
-__global__ void k_page_bounds(mentat_kv_cache c, int layer, const int32_t* blocks, mentat_page_index x, float* low,
-                              float* high, int8_t* exps) {
+__global__ void __launch_bounds__(256) k_page_bounds(mentat_kv_cache c, int layer, const int32_t* blocks, mentat_page_index x,
+                                                     float* low, float* high, int8_t* exps) {
     griddep_wait();
-    const int b = blocks[blockIdx.x], h = blockIdx.y, D = c.head_dim;
+    griddep_launch();
+    const int b = blocks[blockIdx.x], D = c.head_dim, H = c.num_kv_heads;
     if ((unsigned)b >= (unsigned)c.num_blocks) {
         if (threadIdx.x == 0) set_error(c, MENTAT_DEV_BAD_BLOCK, b);
         return;
     }
-    const int64_t at = ((int64_t)layer * c.num_blocks + b) * c.num_kv_heads + h;
-    const int64_t to = (int64_t)blockIdx.x * c.num_kv_heads + h;
-    const int e = x.exps[at];
-    const float unit = e == EXP_ALL ? INFINITY : pow2(e);
-    for (int d = threadIdx.x; d < D; d += blockDim.x) {
-        low[to * D + d] = e == EXP_ALL ? -unit : x.bounds[at * 2 * D + d] * unit;
-        high[to * D + d] = e == EXP_ALL ? unit : x.bounds[at * 2 * D + D + d] * unit;
+    const int64_t at = ((int64_t)layer * c.num_blocks + b) * H, to = (int64_t)blockIdx.x * H;
+    auto value = [&](int v, int e) { return e == EXP_ALL ? 0.f : v * pow2(e); };
+    if (D % 4 == 0 && (((uintptr_t)low | (uintptr_t)high) & 15) == 0 && ((uintptr_t)x.bounds & 3) == 0) {
+        for (int u = threadIdx.x; u < H * D / 2; u += blockDim.x) {  // 4 bytes to 16
+            const int h = u / (D / 2), r = u - h * (D / 2), d = r % (D / 4) * 4, e = x.exps[at + h];
+            const bool top = r >= D / 4;
+            const char4 v = *reinterpret_cast<const char4*>(x.bounds + (at + h) * 2 * D + (top ? D : 0) + d);
+            const float inf = top ? INFINITY : -INFINITY;
+            *reinterpret_cast<float4*>((top ? high : low) + (to + h) * D + d) =
+                e == EXP_ALL ? make_float4(inf, inf, inf, inf)
+                             : make_float4(value(v.x, e), value(v.y, e), value(v.z, e), value(v.w, e));
+        }
+    } else {
+        for (int u = threadIdx.x; u < H * D; u += blockDim.x) {
+            const int h = u / D, d = u - h * D, e = x.exps[at + h];
+            low[(to + h) * D + d] = e == EXP_ALL ? -INFINITY : value(x.bounds[(at + h) * 2 * D + d], e);
+            high[(to + h) * D + d] = e == EXP_ALL ? INFINITY : value(x.bounds[(at + h) * 2 * D + D + d], e);
+        }
     }
-    if (threadIdx.x == 0) exps[to] = (int8_t)e;
+    for (int h = threadIdx.x; h < H; h += blockDim.x) exps[to + h] = x.exps[at + h];
 }
 
 // ---------------------------------------------------------------------------
@@ -1344,8 +1459,12 @@ int mentat_page_index_blocks(const mentat_kv_cache* c, int32_t layer, const int3
                              const mentat_page_index* x, cudaStream_t s) {
     if (bad_index(c, x) || layer < 0 || layer >= c->num_layers || n < 0 || (n > 0 && !blocks)) return MENTAT_ERR_ARG;
     if (n == 0) return MENTAT_OK;
+    if (const int threads = index_block_threads(c)) {
+        MENTAT_BY_DTYPE(MENTAT_LAUNCH((k_index_blocks<T, true>), dim3(n), dim3(threads), 0, s, *c, layer, blocks, *x))
+        return MENTAT_OK;
+    }
     const dim3 grid(n, c->num_kv_heads), block((c->head_dim + 31) / 32 * 32);
-    MENTAT_BY_DTYPE(MENTAT_LAUNCH(k_index_blocks<T>, grid, block, 0, s, *c, layer, blocks, *x))
+    MENTAT_BY_DTYPE(MENTAT_LAUNCH((k_index_blocks<T, false>), grid, block, 0, s, *c, layer, blocks, *x))
     return MENTAT_OK;
 }
 
@@ -1356,9 +1475,14 @@ int mentat_page_index_seqs(const mentat_kv_cache* c, int32_t layer, const int32_
         return MENTAT_ERR_ARG;
     if (first < 0) max_pages = 1;
     if (n == 0 || max_pages == 0) return MENTAT_OK;
-    const dim3 grid(n * max_pages, c->num_kv_heads, layer < 0 ? c->num_layers : 1), block((c->head_dim + 31) / 32 * 32);
-    const int l0 = layer < 0 ? 0 : layer;
-    MENTAT_BY_DTYPE(MENTAT_LAUNCH(k_index_seqs<T>, grid, block, 0, s, *c, l0, slots, first, *x, max_pages))
+    const int l0 = layer < 0 ? 0 : layer, layers = layer < 0 ? c->num_layers : 1;
+    if (const int threads = index_block_threads(c)) {
+        MENTAT_BY_DTYPE(MENTAT_LAUNCH((k_index_seqs<T, true>), dim3(n * max_pages, 1, layers), dim3(threads), 0, s, *c, l0,
+                                      slots, first, *x, max_pages))
+        return MENTAT_OK;
+    }
+    const dim3 grid(n * max_pages, c->num_kv_heads, layers), block((c->head_dim + 31) / 32 * 32);
+    MENTAT_BY_DTYPE(MENTAT_LAUNCH((k_index_seqs<T, false>), grid, block, 0, s, *c, l0, slots, first, *x, max_pages))
     return MENTAT_OK;
 }
 
@@ -1367,7 +1491,7 @@ int mentat_page_bounds(const mentat_kv_cache* c, int32_t layer, const int32_t* b
     if (bad_index(c, x) || layer < 0 || layer >= c->num_layers || n < 0 || (n > 0 && (!blocks || !low || !high || !exps)))
         return MENTAT_ERR_ARG;
     if (n == 0) return MENTAT_OK;
-    MENTAT_LAUNCH(k_page_bounds, dim3(n, c->num_kv_heads), dim3(128), 0, s, *c, layer, blocks, *x, low, high, exps);
+    MENTAT_LAUNCH(k_page_bounds, dim3(n), dim3(256), 0, s, *c, layer, blocks, *x, low, high, exps);
     return MENTAT_OK;
 }
 

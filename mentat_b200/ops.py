@@ -20,6 +20,7 @@ import ctypes as C
 import itertools
 import math
 import struct
+import threading
 import weakref
 from typing import Optional
 
@@ -242,13 +243,33 @@ def _call(device, name: str, *args) -> None:
         _lib.check(status, name)
 
 
-_pack_rows = struct.Struct("@Pqqi4x").pack  # mentat_rows
-_NO_ROWS = _pack_rows(0, 0, 0, 0)
+class _RowArgs(threading.local):
+    """Four ``mentat_rows`` of the calling thread, filled in one step and passed by address (a call
+    has read them when it returns)."""
+
+    def __init__(self):
+        self.buf = bytearray(128)
+        self._keep = (C.c_char * 128).from_buffer(self.buf)
+        a = C.addressof(self._keep)
+        self.at = (a, a + 32, a + 64, a + 96)
 
 
-def _row_ref(t: torch.Tensor) -> bytes:
-    s0, s1, _ = t.stride()
-    return _pack_rows(t.data_ptr(), s0, s1, t.shape[1])
+_row_args = _RowArgs()
+_pack_rows = struct.Struct("@Pqqi4xPqqi4xPqqi4xPqqi4x").pack_into
+
+
+def _rows(a, b, c, d) -> tuple:
+    """Addresses of the four tensors' ``mentat_rows`` (None: no heads)."""
+    args = []
+    for t in (a, b, c, d):
+        if t is None:
+            args += (0, 0, 0, 0)
+        else:
+            s0, s1, _ = t.stride()
+            args += (t.data_ptr(), s0, s1, t.shape[1])
+    r = _row_args
+    _pack_rows(r.buf, 0, *args)
+    return r.at
 
 
 def _check_rows(name: str, t: torch.Tensor, n: int, d: int, dtype, device) -> torch.Tensor:
@@ -266,7 +287,7 @@ def _out_rows(name: str, out: Optional[torch.Tensor], x: torch.Tensor) -> torch.
     """``out`` checked as the result of a row operation on ``x``: its own rows distinct, and
     either ``x`` itself or apart from it; a new tensor if None."""
     if out is None:
-        return x.new_empty(x.shape)
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
     n, h, d = x.shape
     if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError(f"{name} must have the input's shape, dtype and device")
@@ -331,8 +352,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         k = _check_rows("k", k, n, d, q.dtype, q.device)
         ko = _out_rows("k_out", k_out, k)
     if n:
-        _call(q.device, "mentat_rotary_apply", _DT[q.dtype], d, n, _row_ref(q),
-              _row_ref(qo), _NO_ROWS if k is None else _row_ref(k), _NO_ROWS if k is None else _row_ref(ko),
+        _call(q.device, "mentat_rotary_apply", _DT[q.dtype], d, n, *_rows(q, qo, k, ko),
               positions.data_ptr(), rotary._ptrs[bool(inverse)])
     return qo, ko
 
@@ -363,8 +383,7 @@ def rotary_append(cache, layer: int, rows: torch.Tensor, q: Optional[torch.Tenso
         qo = _out_rows("q_out", q_out, q)
     if n:
         _call(dev, "mentat_rotary_append", cache._desc_ptr, layer, n, rows.data_ptr(),
-              _NO_ROWS if q is None else _row_ref(q), _NO_ROWS if q is None else _row_ref(qo), _row_ref(k), _row_ref(v),
-              positions.data_ptr(), rotary._ptrs[0])
+              *_rows(q, qo, k, v), positions.data_ptr(), rotary._ptrs[0])
     return qo
 
 
@@ -377,11 +396,11 @@ def _append_rotated(k_pool: torch.Tensor, v_pool: torch.Tensor, slots: torch.Ten
     n, d = k.shape[0], k.shape[2]
     dev = mgr.device
     q, k, v = (_check_rows(name, t, n, d, mgr.dtype, dev) for name, t in (("q", q), ("k", k), ("v", v)))
-    qo = q.new_empty(q.shape)
+    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
     for a in range(0, n, 1024):
         b = min(n, a + 1024)
         _call(dev, "mentat_kv_append_rotated_batched", mgr._desc_ptr, layer,
-              slots.data_ptr() + 4 * a, b - a, *(_row_ref(x if n <= 1024 else x[a:b]) for x in (q, qo, k, v)),
+              slots.data_ptr() + 4 * a, b - a, *_rows(*((q, qo, k, v) if n <= 1024 else (x[a:b] for x in (q, qo, k, v)))),
               None, rot._ptrs[0])
     if mgr.page_index is not None:
         _index_tails(mgr, layer, slots, n)
@@ -499,11 +518,11 @@ def page_bounds(index, layer: int, blocks: torch.Tensor) -> tuple:
     c = index.cache
     blocks = _check_ids("blocks", blocks, c.device)
     n, h, d = blocks.shape[0], c.num_key_value_heads, c.head_dim
-    both = torch.empty((2, n, h, d), device=c.device)
+    low, high = torch.empty((n, h, d), device=c.device), torch.empty((n, h, d), device=c.device)
     exps = torch.empty((n, h), dtype=torch.int8, device=c.device)
     _call(c.device, "mentat_page_bounds", c._desc_ptr, layer, blocks.data_ptr(), n, index._ptr,
-          both[0].data_ptr(), both[1].data_ptr(), exps.data_ptr())
-    return both[0], both[1], exps
+          low.data_ptr(), high.data_ptr(), exps.data_ptr())
+    return low, high, exps
 
 
 def sparse_decode(index, layer: int, slots: torch.Tensor, q: torch.Tensor, max_len: int, budget: int, *, sink: int = 1,
@@ -524,10 +543,10 @@ def sparse_decode(index, layer: int, slots: torch.Tensor, q: torch.Tensor, max_l
     slots = _check_ids("slots", slots, c.device, n)
     if recent < 1 or sink < 0 or sink + recent > budget:
         raise ValueError(f"sink {sink} >= 0 and recent {recent} >= 1 pages must fit in the budget of {budget}")
-    out = q.new_empty((n, hq, d))
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     pages = slots.new_empty((n, c.num_key_value_heads, budget)) if return_pages else None
     if n:
-        size = _lib.call("mentat_sparse_workspace_bytes")(c._desc_ptr, n, max_len, budget)
+        size = index.workspace_bytes(n, max_len, budget)
         ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
         _call(c.device, "mentat_sparse_decode", c._desc_ptr, layer, index._ptr,
               slots.data_ptr(), n, q.data_ptr(), q.stride(0), hq, out.data_ptr(), out.stride(0),

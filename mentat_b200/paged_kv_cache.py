@@ -280,6 +280,17 @@ class PageIndex:
         self.cache, self.bounds, self.exps = cache, bounds, exps
         self._desc = _lib.PageIndex(bounds.data_ptr(), exps.data_ptr())
         self._ptr = C.addressof(self._desc)
+        self._sizes: dict = {}
+
+    def workspace_bytes(self, n: int, max_len: int, budget: int) -> int:
+        """Bytes of workspace of ``ops.sparse_decode`` for such a batch (they depend on nothing else)."""
+        key = (n, max_len, budget)
+        size = self._sizes.get(key)
+        if size is None:
+            if len(self._sizes) > 4096:
+                self._sizes.clear()
+            size = self._sizes[key] = _lib.call("mentat_sparse_workspace_bytes")(self.cache._desc_ptr, n, max_len, budget)
+        return size
 
 
 class PagedKVCacheManager:
@@ -668,10 +679,8 @@ class PagedKVCacheManager:
             return qo
         first = seq.num_tokens[layer_idx]
         self._mirror_append(seq, layer_idx, n)
-        none = ops._NO_ROWS
         ops._call(self.device, "mentat_kv_append_rotated", self._desc_ptr, layer_idx, seq.slot, n,
-                  none if q is None else ops._row_ref(q), none if q is None else ops._row_ref(qo), ops._row_ref(k),
-                  ops._row_ref(v), None if positions is None else positions.data_ptr(), rotary._ptrs[0])
+                  *ops._rows(q, qo, k, v), None if positions is None else positions.data_ptr(), rotary._ptrs[0])
         self._index_appended(seq, layer_idx, first)
         self._after()
         return qo
