@@ -379,7 +379,7 @@ int mentat_kv_fork_batched(const mentat_kv_cache* c, const int32_t* parents, con
 
 /* free_sequence (paged_kv_cache.py:172-176) of distinct slots, with the state
  * that freeing them one after another leaves, the free list's order included.
- * workspace: mentat_pages_workspace_bytes(c, n) bytes. */
+ * workspace: mentat_pages_workspace_bytes(c, n) bytes, 16-byte aligned. */
 int64_t mentat_pages_workspace_bytes(const mentat_kv_cache* c, int32_t n);
 int mentat_kv_free_batched(const mentat_kv_cache* c, const int32_t* slots, int32_t n, int32_t max_nblocks,
                            void* workspace, int64_t workspace_bytes, cudaStream_t s);

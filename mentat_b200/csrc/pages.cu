@@ -21,6 +21,7 @@
 #include <cooperative_groups.h>
 
 #include "rotary.cuh"
+#include "tma.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -28,7 +29,8 @@ namespace mentat {
 
 constexpr int PAGES_MAX_SEQS = 1024;
 
-// workspace: [0] 1 = stop (an error, now or before), then order, the ids of fresh
+// workspace: [0] 1 = stop (an error, now or before), [1] fresh blocks of a compaction, [2..3] the FIFO's tail before
+// a free, then order, the ids of fresh
 // blocks, and per row the pages at the front that stay, the first of its fresh
 // blocks, the freed (or, before that, the demanded) count, and its exclusive scan
 struct PagesWs {
@@ -133,22 +135,27 @@ __global__ void __launch_bounds__(PAGES_THREADS) k_fork_batched(mentat_kv_cache 
 // ---------------------------------------------------------------------------
 // check and reset: CTA 0 checks the batch, all of them clear `order`
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) k_pages_begin(mentat_kv_cache c, const int32_t* slots, int n, PagesWs w) {
+__global__ void __launch_bounds__(256) k_pages_begin(mentat_kv_cache c, const int32_t* slots, int n, int groups,
+                                                     PagesWs w) {
     extern __shared__ uint32_t bits[];
     __shared__ int s_bad;
     griddep_wait();
     for (int64_t b = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; b < c.num_blocks; b += (int64_t)gridDim.x * blockDim.x)
         w.order[b] = 0;
+    for (int k = blockIdx.x * blockDim.x + threadIdx.x; k < groups; k += gridDim.x * blockDim.x) w.base[k] = 0;
     if (blockIdx.x) return;
     const bool ok = slots_distinct(c, slots, n, bits, &s_bad);
     if (threadIdx.x == 0) {
         if (!ok) set_error(c, MENTAT_DEV_BAD_SLOT, s_bad);
         *w.stop = has_error(c) ? 1 : 0;
+        *reinterpret_cast<long long*>(w.stop + 2) = c.ctrl[MENTAT_CTRL_TAIL];
     }
 }
 
-__global__ void __launch_bounds__(256) k_order_clear(mentat_kv_cache c, PagesWs w) {
+__global__ void __launch_bounds__(256) k_order_clear(mentat_kv_cache c, int groups, PagesWs w) {
     griddep_wait();
+    for (int k = blockIdx.x * blockDim.x + threadIdx.x; k < groups; k += gridDim.x * blockDim.x) w.base[k] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<long long*>(w.stop + 2) = c.ctrl[MENTAT_CTRL_TAIL];
     for (int64_t b = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; b < c.num_blocks; b += (int64_t)gridDim.x * blockDim.x)
         w.order[b] = 0;
 }
@@ -227,30 +234,10 @@ __global__ void __launch_bounds__(PAGES_THREADS) k_free_count(mentat_kv_cache c,
         for (int u = 0; u < 4; ++u) n += frees(c, w, b[u], row, j0 + 32 * u + lane);
     }
     n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) w.count[row] = n;
-}
-
-// exclusive scan of w.count into base by one CTA; returns the total
-__device__ __forceinline__ int scan_rows(const PagesWs& w, int32_t* base, int rows, int* smem32) {
-    int carry = 0;
-    for (int r0 = 0; r0 < rows; r0 += blockDim.x) {
-        const int r = r0 + threadIdx.x;
-        int total;
-        const int at = block_exclusive_scan(r < rows ? w.count[r] : 0, &total, smem32);
-        if (r < rows) base[r] = carry + at;
-        carry += total;
+    if (lane == 0) {
+        w.count[row] = n;
+        if (n) atomicAdd(&w.base[blockIdx.x], n);  // the CTA's rows together
     }
-    return carry;
-}
-
-// the scan, and the FIFO's new tail; base counts from the old tail
-__global__ void __launch_bounds__(1024) k_free_scan(mentat_kv_cache c, int rows, PagesWs w) {
-    __shared__ int smem32[32];
-    griddep_wait();
-    griddep_launch();
-    if (*w.stop) return;
-    const int total = scan_rows(w, w.base, rows, smem32);
-    if (threadIdx.x == 0) c.ctrl[MENTAT_CTRL_TAIL] += total;
 }
 
 // a row's new table and counters after a compaction in place
@@ -266,21 +253,37 @@ __device__ __forceinline__ void install(const mentat_kv_cache& c, const PagesWs&
     }
 }
 
-// push, and the rows' new counters (empty, or what compaction kept: cu); a warp a row
+// push, and the rows' new counters (empty, or what compaction kept: cu); a warp a row.  A CTA adds up the totals of
+// the CTAs before it (8 rows each).
 template <bool LEAD>
 __global__ void __launch_bounds__(PAGES_THREADS) k_free_push(mentat_kv_cache c, const int32_t* slots, const int32_t* cu,
                                                              int rows, PagesWs w) {
+    __shared__ int s_sum[PAGES_WARPS], s_count[PAGES_WARPS];
     griddep_wait();
     griddep_launch();
-    const int lane = threadIdx.x & 31, row = blockIdx.x * PAGES_WARPS + (threadIdx.x >> 5);
-    if (row >= rows || *w.stop) return;
+    if (*w.stop) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.x * PAGES_WARPS + warp;
+    int before = 0;
+    for (int k = threadIdx.x; k < (int)blockIdx.x; k += PAGES_THREADS) before += w.base[k];
+    before = __reduce_add_sync(0xffffffffu, before);
+    if (lane == 0) {
+        s_sum[warp] = before;
+        s_count[warp] = row < rows ? w.count[row] : 0;
+    }
+    __syncthreads();
+    long long at = *reinterpret_cast<const long long*>(w.stop + 2);  // the tail before the batch
+    int all = 0;
+    for (int k = 0; k < PAGES_WARPS; ++k) {
+        at += s_sum[k] + (k < warp ? s_count[k] : 0);
+        all += s_count[k];
+    }
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) c.ctrl[MENTAT_CTRL_TAIL] = at + all;
+    if (row >= rows) return;
     const int i = row / c.num_layers, l = row - i * c.num_layers;
     const int64_t si = seq_index(c, l, slots[i]);
     int32_t* t = table_row(c, l, slots[i]);
-    if (w.count[row]) {
+    if (s_count[warp]) {
         const int nb = c.nblocks[si];
-        // base counts from the tail before the batch, which the scan has moved past all rows
-        long long at = c.ctrl[MENTAT_CTRL_TAIL] - (w.base[rows - 1] + w.count[rows - 1]) + w.base[row];
         for (int j0 = LEAD ? w.lead[row] : 0; j0 < nb; j0 += 32) {
             const int j = j0 + lane, b = j < nb ? t[j] : -1;
             const bool go = frees(c, w, b, row, j);
@@ -297,16 +300,17 @@ __global__ void __launch_bounds__(PAGES_THREADS) k_free_push(mentat_kv_cache c, 
 }
 
 // ---------------------------------------------------------------------------
-// the same in one cluster: warps take ranges of rows, so a scan over the warps' totals orders the pushes
+// the same in one cluster
 // ---------------------------------------------------------------------------
-constexpr int CLUSTER_CTAS = 8, CLUSTER_THREADS = 512, CLUSTER_WARPS = CLUSTER_THREADS / 32;
+constexpr int CLUSTER_CTAS = 8, CLUSTER_THREADS = 1024, CLUSTER_WARPS = CLUSTER_THREADS / 32;
+constexpr int CLUSTER_ALL_WARPS = CLUSTER_CTAS * CLUSTER_WARPS;
 
 // the sum of s_total over the warps of the cluster before this one, and over all of them (a cluster barrier
 // between the writes and this call)
 __device__ __forceinline__ int before_warp(cg::cluster_group& cluster, int* s_total, int* all) {
     const int lane = threadIdx.x & 31, me = cluster.block_rank() * CLUSTER_WARPS + (threadIdx.x >> 5);
     int before = 0, total = 0;
-    for (int w = lane; w < CLUSTER_CTAS * CLUSTER_WARPS; w += 32) {
+    for (int w = lane; w < CLUSTER_ALL_WARPS; w += 32) {
         const int v = cluster.map_shared_rank(s_total, w / CLUSTER_WARPS)[w % CLUSTER_WARPS];
         total += v;
         before += w < me ? v : 0;
@@ -315,68 +319,100 @@ __device__ __forceinline__ int before_warp(cg::cluster_group& cluster, int* s_to
     return __reduce_add_sync(0xffffffffu, before);
 }
 
+// Items are 32 entries of a row (the last chunk of a row goes on to its end); a warp takes `per` items that
+// follow one another, so a scan over the warps' totals orders the pushes.  Entries stay in shared memory
+// between the steps: [CLUSTER_WARPS][per][32], negative once they are settled.
 template <bool LEAD>
 __global__ void __launch_bounds__(CLUSTER_THREADS) k_free_cluster(mentat_kv_cache c, const int32_t* slots, const int32_t* cu,
-                                                                  int n, PagesWs w) {
-    extern __shared__ uint32_t bits[];
+                                                                  int n, int chunks, int per, PagesWs w) {
+    extern __shared__ uint32_t dyn[];
     __shared__ int s_bad, s_total[CLUSTER_WARPS];
     cg::cluster_group cluster = cg::this_cluster();
     griddep_wait();
     griddep_launch();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = cluster.block_rank();
+    int* held = reinterpret_cast<int*>(dyn) + warp * per * 32 + lane;
+    uint32_t* bits = dyn + CLUSTER_WARPS * per * 32;
     bool stop = LEAD ? *w.stop != 0 : !slots_distinct(c, slots, n, bits, &s_bad);
     if (!LEAD && stop && threadIdx.x == 0) set_error(c, MENTAT_DEV_BAD_SLOT, s_bad);
     if (!LEAD) stop = __syncthreads_or(stop || has_error(c));
     // an earlier error, or this one, stops every CTA: nothing of this call is recorded before all have looked
     if (stop) return;
-    const int rows = n * c.num_layers, per = (rows + CLUSTER_CTAS * CLUSTER_WARPS - 1) / (CLUSTER_CTAS * CLUSTER_WARPS);
-    const int r0 = min(rows, (rank * CLUSTER_WARPS + warp) * per), r1 = min(rows, r0 + per);
+    const int rows = n * c.num_layers, items = rows * chunks, me = rank * CLUSTER_WARPS + warp;
+    const int y0 = min(items, me * per), y1 = min(items, y0 + per);
     const long long tail0 = c.ctrl[MENTAT_CTRL_TAIL];
-    auto each = [&](auto&& f) {  // f(row, entry, block) over the warp's rows, a lane an entry
-        for (int row = r0; row < r1; ++row) {
-            const int i = row / c.num_layers, l = row - i * c.num_layers;
-            const int nb = c.nblocks[seq_index(c, l, slots[i])];
-            const int32_t* t = table_row(c, l, slots[i]);
-            for (int j0 = LEAD ? w.lead[row] : 0; j0 < nb; j0 += 32) {
-                const int j = j0 + lane, b = j < nb ? t[j] : -1;
-                f(row, j, (unsigned)b < (unsigned)c.num_blocks ? b : -1, j < nb);
-            }
+    // entries past an item's first 32 (a table longer than the launch was sized for) are read again each time
+    auto rest = [&](int y, auto&& f) {
+        if (y % chunks != chunks - 1) return;
+        const int row = y / chunks, i = row / c.num_layers, l = row - i * c.num_layers;
+        const int nb = c.nblocks[seq_index(c, l, slots[i])], lead = LEAD ? w.lead[row] : 0;
+        const int32_t* t = table_row(c, l, slots[i]);
+        for (int j0 = chunks * 32; j0 < nb; j0 += 32) {
+            const int j = j0 + lane, b = j < nb && j >= lead ? t[j] : -1;
+            f(row, j, (unsigned)b < (unsigned)c.num_blocks ? b : -1);
         }
     };
-    each([&](int, int, int b, bool) {
-        if (b >= 0) w.order[b] = 0;
-    });
-    cluster.sync();
-    each([&](int row, int j, int b, bool have) {
-        if (b < 0) {
-            if (have) set_error(c, MENTAT_DEV_BAD_BLOCK, table_row(c, row % c.num_layers, slots[row / c.num_layers])[j]);
-            return;
+    for (int y = y0; y < y1; ++y) {
+        const int row = y / chunks, j = y % chunks * 32 + lane, i = row / c.num_layers, l = row - i * c.num_layers;
+        const int slot = slots[i], nb = c.nblocks[seq_index(c, l, slot)];
+        int b = -1;
+        if (j < nb && (!LEAD || j >= w.lead[row])) {
+            b = table_row(c, l, slot)[j];
+            if ((unsigned)b >= (unsigned)c.num_blocks) {
+                b = -2;  // recorded once all CTAs have looked at the error word
+            } else {
+                w.order[b] = 0;
+            }
         }
+        held[(y - y0) * 32] = b;
+        rest(y, [&](int, int, int b) {
+            if (b >= 0) w.order[b] = 0;
+        });
+    }
+    cluster.sync();
+    auto mark = [&](int row, int j, int b) {
+        if (b < 0) return;
         if (atomicSub(&c.refcounts[b], 1) <= 0) {
             atomicAdd(&c.refcounts[b], 1);
             set_error(c, MENTAT_DEV_RELEASE_FREE, b);
             return;
         }
         atomicMax(&w.order[b], release_index(c, row, j));
-    });
+    };
+    for (int y = y0; y < y1; ++y) {
+        const int row = y / chunks, j = y % chunks * 32 + lane, b = held[(y - y0) * 32];
+        if (b == -2) set_error(c, MENTAT_DEV_BAD_BLOCK, table_row(c, row % c.num_layers, slots[row / c.num_layers])[j]);
+        mark(row, j, b);
+        rest(y, mark);
+    }
     cluster.sync();
     auto freed = [&](int row, int j, int b) {
         return b >= 0 && __ldcg(&w.order[b]) == release_index(c, row, j) && __ldcg(&c.refcounts[b]) == 0;
     };
     int mine = 0;
-    each([&](int row, int j, int b, bool) { mine += __popc(__ballot_sync(0xffffffffu, freed(row, j, b))); });
+    for (int y = y0; y < y1; ++y) {
+        const int b = held[(y - y0) * 32];
+        const bool go = freed(y / chunks, y % chunks * 32 + lane, b);
+        if (!go) held[(y - y0) * 32] = -1;
+        mine += __popc(__ballot_sync(0xffffffffu, go));
+        rest(y, [&](int row, int j, int b) { mine += __popc(__ballot_sync(0xffffffffu, freed(row, j, b))); });
+    }
     if (lane == 0) s_total[warp] = mine;
     cluster.sync();
     int all;
     long long at = tail0 + before_warp(cluster, s_total, &all);
-    each([&](int row, int j, int b, bool) {
-        const bool go = freed(row, j, b);
-        const uint32_t who = __ballot_sync(0xffffffffu, go);
-        if (go) c.free_ring[(at + __popc(who & ((1u << lane) - 1))) % c.num_blocks] = b;
+    auto push = [&](int b) {
+        const uint32_t who = __ballot_sync(0xffffffffu, b >= 0);
+        if (b >= 0) c.free_ring[(at + __popc(who & ((1u << lane) - 1))) % c.num_blocks] = b;
         at += __popc(who);
-    });
-    __syncwarp();
-    for (int row = r0; row < r1; ++row) {
+    };
+    for (int y = y0; y < y1; ++y) {
+        push(held[(y - y0) * 32]);
+        rest(y, [&](int row, int j, int b) { push(freed(row, j, b) ? b : -1); });
+    }
+    cluster.sync();  // every CTA has read the old tail, the others' totals and the tables
+    if (rank == 0 && threadIdx.x == 0) c.ctrl[MENTAT_CTRL_TAIL] = tail0 + all;
+    for (int row = me; row < rows; row += CLUSTER_ALL_WARPS) {
         const int i = row / c.num_layers, l = row - i * c.num_layers;
         const int64_t si = seq_index(c, l, slots[i]);
         if (LEAD)
@@ -384,8 +420,6 @@ __global__ void __launch_bounds__(CLUSTER_THREADS) k_free_cluster(mentat_kv_cach
         else if (lane == 0)
             c.nblocks[si] = c.ntok[si] = c.tail[si] = 0;
     }
-    cluster.sync();  // every CTA has read the old tail and the others' totals
-    if (rank == 0 && threadIdx.x == 0) c.ctrl[MENTAT_CTRL_TAIL] = tail0 + all;
 }
 
 // ---------------------------------------------------------------------------
@@ -400,7 +434,7 @@ struct CompactArgs {
     int n;
 };
 
-constexpr int PLAN_CHUNK = 1024;  // kept positions of a warp's step; the last chunk goes on to the end of a list
+constexpr int PLAN_CHUNK = 512;  // kept positions of a warp's step; the last chunk goes on to the end of a list
 // The plan, in one cluster, a warp a range of rows: the batch is checked, the kept positions are inside their
 // sequences; how many pages at the front stay, and the fresh blocks of the others.  (The lists are a
 // thousandth of the bytes that are moved.)
@@ -429,14 +463,14 @@ __global__ void __launch_bounds__(CLUSTER_THREADS) k_compact_plan(mentat_kv_cach
     ok = !__syncthreads_or(no) && ok;
     if (!ok && threadIdx.x == 0) set_error(c, MENTAT_DEV_BAD_SLOT, s_bad);
     bool stop = __syncthreads_or(!ok || has_error(c));
-    const int rows = a.n * L, per = (rows + CLUSTER_CTAS * CLUSTER_WARPS - 1) / (CLUSTER_CTAS * CLUSTER_WARPS);
+    const int rows = a.n * L, per = (rows + CLUSTER_ALL_WARPS - 1) / CLUSTER_ALL_WARPS;
     const int r0 = min(rows, (rank * CLUSTER_WARPS + warp) * per), r1 = min(rows, r0 + per);
     if (!stop)
         for (int row = r0 + lane; row < r1; row += 32) w.count[row] = a.cu[row / L + 1] - a.cu[row / L];
     cluster.sync();  // all have looked at the error word before this call writes it
     // the first position that moves: chunks of the lists over all warps
     if (!stop)
-        for (int64_t y = rank * CLUSTER_WARPS + warp; y < (int64_t)rows * chunks; y += CLUSTER_CTAS * CLUSTER_WARPS) {
+        for (int64_t y = rank * CLUSTER_WARPS + warp; y < (int64_t)rows * chunks; y += CLUSTER_ALL_WARPS) {
             const int row = (int)(y / chunks), i = row / L, l = row - i * L;
             const int m = a.cu[i + 1] - a.cu[i], j0 = (int)(y % chunks) * PLAN_CHUNK, j1 = chunks - 1 == y % chunks ? m : min(m, j0 + PLAN_CHUNK);
             if (j0 >= j1) continue;
@@ -485,7 +519,8 @@ __global__ void __launch_bounds__(CLUSTER_THREADS) k_compact_plan(mentat_kv_cach
     cluster.sync();  // everyone has read the error word, the totals and the control words
     if (rank == 0 && threadIdx.x == 0) {
         if (short_of) set_error(c, MENTAT_DEV_OUT_OF_BLOCKS, c.num_blocks);
-        *w.stop = stop || short_of;
+        w.stop[0] = stop || short_of;
+        w.stop[1] = all;
         if (!stop && !short_of) {
             c.ctrl[MENTAT_CTRL_HEAD] = head + all;
             const long long used = c.num_blocks - (tail - head - all);
@@ -506,176 +541,274 @@ __global__ void __launch_bounds__(CLUSTER_THREADS) k_compact_plan(mentat_kv_cach
     }
 }
 
-// One CTA per (row, page): the kept tokens of one fresh page, a warp a token.  The cosines and sines of a
-// token's shift are computed once for all of its heads, and once for neighbours that moved together; K is
-// turned and V copied 16 bytes at a time.  Into new sequences it also writes their tables.  Bound by memory.
-constexpr int MOVE_THREADS = 256, MOVE_TOKENS = 16;
-
-// n elements of a row by a warp, four vectors of a lane on the way
-template <typename T, int VEC>
-__device__ __forceinline__ void copy_row(const T* src, T* dst, int n) {
-    using P = Pack<T, VEC>;
-    const P* s = reinterpret_cast<const P*>(src);
-    P* d = reinterpret_cast<P*>(dst);
-    for (int x = threadIdx.x & 31; x < n / VEC; x += 128) {
-        P v[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (x + 32 * u < n / VEC) v[u] = s[x + 32 * u];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (x + 32 * u < n / VEC) d[x + 32 * u] = v[u];
-    }
-}
-// the tokens' V rows, a warp a token
-template <typename T, int VEC>
-__device__ __forceinline__ void move_v(T* vp, int64_t dst, const int64_t* from, int count, int n) {
-    for (int k = threadIdx.x >> 5; k < count; k += MOVE_THREADS / 32)
-        if (from[k] >= 0) copy_row<T, VEC>(vp + from[k], vp + dst + (int64_t)k * n, n);
-}
-// a token's heads turned by a table (cosines, then sines) by a warp.  Where the 32 lanes cover whole heads, a
-// lane has the same pairs in every head and keeps their cosines and sines.
-template <typename T, int VEC, bool IL>
-__device__ __forceinline__ void turn_row(const T* src, T* dst, int H, int D, const mentat_rotary& r, const float* tab) {
-    using P = Pack<T, VEC>;
-    const int lane = threadIdx.x & 31, pairs = r.pairs, off = r.offset;
-    const int turned = IL ? D / VEC : pairs / VEC, tasks = IL ? turned : turned + (D - 2 * pairs) / VEC;
-    const bool whole = 32 % tasks == 0;
-    constexpr int N = IL ? VEC / 2 : VEC;
-    float co[N], sn[N];
-    auto fetch = [&](int t) {
-        const int e0 = IL ? (t * VEC - off) / 2 : t * VEC;
-        const bool in = IL ? t * VEC >= off && t * VEC < off + 2 * pairs : t < turned;
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            co[e] = in ? tab[e0 + e] : 1.f;
-            sn[e] = in ? tab[pairs + e0 + e] : 0.f;
-        }
-    };
-    if (whole) fetch(lane % tasks);
-    const int total = H * tasks;
-    for (int x0 = lane; x0 < total; x0 += 64) {
-        P a[2], b[2];
-        int d1[2], d2[2];
-        bool pair[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int x = x0 + 32 * u;
-            if (x >= total) continue;
-            const int h = x / tasks, t = x - h * tasks;
-            pair[u] = IL || t < turned;
-            if (IL) {
-                d1[u] = d2[u] = h * D + t * VEC;
-            } else if (t < turned) {
-                d1[u] = h * D + off + t * VEC;
-                d2[u] = d1[u] + pairs;
-            } else {  // passed through
-                const int d = (t - turned) * VEC;
-                d1[u] = d2[u] = h * D + (d >= off ? d + 2 * pairs : d);
-            }
-            a[u] = *reinterpret_cast<const P*>(src + d1[u]);
-            if (!IL && pair[u]) b[u] = *reinterpret_cast<const P*>(src + d2[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int x = x0 + 32 * u;
-            if (x >= total) continue;
-            if (!whole) fetch(x % tasks);
-            if (IL) {
-#pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const float p = Elem<T>::to_f(a[u].v[2 * e]), q = Elem<T>::to_f(a[u].v[2 * e + 1]);
-                    a[u].v[2 * e] = Elem<T>::from_f(p * co[e] - q * sn[e]);
-                    a[u].v[2 * e + 1] = Elem<T>::from_f(p * sn[e] + q * co[e]);
-                }
-            } else if (pair[u]) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float p = Elem<T>::to_f(a[u].v[e]), q = Elem<T>::to_f(b[u].v[e]);
-                    a[u].v[e] = Elem<T>::from_f(p * co[e] - q * sn[e]);
-                    b[u].v[e] = Elem<T>::from_f(p * sn[e] + q * co[e]);
-                }
-                *reinterpret_cast<P*>(dst + d2[u]) = b[u];
-            }
-            *reinterpret_cast<P*>(dst + d1[u]) = a[u];
-        }
-    }
-}
-template <typename T, int VEC, bool IL>
-__global__ void __launch_bounds__(MOVE_THREADS, 3) k_compact_move(mentat_kv_cache c, CompactArgs a, mentat_rotary r, PagesWs w) {
-    extern __shared__ float cs[];  // [MOVE_TOKENS][2 pairs]
-    __shared__ int64_t s_from[MOVE_TOKENS];
-    __shared__ int s_shift[MOVE_TOKENS], s_table[MOVE_TOKENS];
-    griddep_wait();
-    griddep_launch();
-    if (*w.stop) return;
-    const int tid = threadIdx.x, row = blockIdx.x, i = row / c.num_layers, l = row - i * c.num_layers;
-    const int D = c.head_dim, H = c.num_kv_heads, bs = c.block_size, lead = w.lead[row];
-    const int m = a.cu[i + 1] - a.cu[i], pages = (m + bs - 1) / bs;
-    const int32_t* keep = a.keep + l * a.keep_ls + a.cu[i];
-    const int32_t* t = table_row(c, l, a.src[i]);
-    const int32_t* fresh = w.fresh + w.first[row];
-    T* kp = reinterpret_cast<T*>(c.k_pool);
-    T* vp = reinterpret_cast<T*>(c.v_pool);
-    if (a.dst && blockIdx.y == 0) {  // the new sequence: shared pages, fresh ones, counters
+// What a compaction into new sequences leaves in their tables: shared pages with a reference more, fresh ones,
+// counters; rows spread over the grid.
+__device__ __forceinline__ void install_new(const mentat_kv_cache& c, const CompactArgs& a, const PagesWs& w, int step) {
+    const int rows = a.n * c.num_layers;
+    for (int row = blockIdx.x; row < rows; row += step) {
+        const int i = row / c.num_layers, l = row - i * c.num_layers, lead = w.lead[row];
+        const int32_t* s = table_row(c, l, a.src[i]);
         int32_t* to = table_row(c, l, a.dst[i]);
-        for (int j = tid; j < lead; j += MOVE_THREADS) {
-            const int b = t[j];
+        for (int j = threadIdx.x; j < lead; j += blockDim.x) {
+            const int b = s[j];
             to[j] = b;
             if ((unsigned)b >= (unsigned)c.num_blocks) set_error(c, MENTAT_DEV_BAD_BLOCK, b);
             else if (atomicAdd(&c.refcounts[b], 1) <= 0) set_error(c, MENTAT_DEV_REF_FREE, b);
         }
-        install(c, w, row, m, seq_index(c, l, a.dst[i]), to, tid, MOVE_THREADS);
+        install(c, w, row, a.cu[i + 1] - a.cu[i], seq_index(c, l, a.dst[i]), to, threadIdx.x, blockDim.x);
     }
-    for (int p = lead + blockIdx.y; p < pages; p += gridDim.y) {
-        const int64_t to = pool_row(c, l, fresh[p - lead], 0);
-        for (int j0 = p * bs; j0 < min(m, (p + 1) * bs); j0 += MOVE_TOKENS) {
-            const int count = min(min(m, (p + 1) * bs) - j0, MOVE_TOKENS);
-            const int64_t dst = to + (int64_t)(j0 - p * bs) * H * D;
-            __syncthreads();
-            if (tid < count) {
-                const int from = keep[j0 + tid], b = t[from / bs], shift = r.pairs ? j0 + tid - from : 0;
-                const bool ok = (unsigned)b < (unsigned)c.num_blocks;
-                if (!ok) set_error(c, MENTAT_DEV_BAD_BLOCK, b);
-                s_shift[tid] = shift;
-                s_from[tid] = ok ? pool_row(c, l, b, from % bs) : -1;
-                // tokens that moved together share a table
-                s_table[tid] = shift == 0 || (tid && j0 + tid - 1 - keep[j0 + tid - 1] == shift) ? 0 : 1;
-            }
+}
+
+// Where fresh page f goes: its row, found from the rows' first fresh pages, and its place in the row
+struct FreshPage {
+    int row, page;
+};
+__device__ __forceinline__ FreshPage fresh_page(const PagesWs& w, int rows, int f) {
+    int lo = 0, hi = rows - 1;  // the last row that begins at or before f (rows without fresh pages begin where the next does)
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (w.first[mid] <= f) lo = mid; else hi = mid - 1;
+    }
+    return FreshPage{lo, w.lead[lo] + f - w.first[lo]};
+}
+
+// The kept tokens of the fresh pages, element by element (heads that 16-byte accesses do not divide, or rows too
+// long for the ring of k_compact_stream): a CTA a page, a warp a token.
+constexpr int MOVE_THREADS = 256, MOVE_TOKENS = 16;
+template <typename T, bool IL>
+__global__ void __launch_bounds__(MOVE_THREADS) k_compact_move(mentat_kv_cache c, CompactArgs a, mentat_rotary r, PagesWs w) {
+    extern __shared__ float cs[];  // [MOVE_TOKENS][2 pairs]
+    griddep_wait();
+    griddep_launch();
+    if (*w.stop) return;
+    if (a.dst) install_new(c, a, w, gridDim.x);
+    const int tid = threadIdx.x, lane = tid & 31, D = c.head_dim, H = c.num_kv_heads, bs = c.block_size, n = H * D;
+    T* kp = reinterpret_cast<T*>(c.k_pool);
+    T* vp = reinterpret_cast<T*>(c.v_pool);
+    for (int f = blockIdx.x; f < w.stop[1]; f += gridDim.x) {
+        const FreshPage fp = fresh_page(w, a.n * c.num_layers, f);
+        const int i = fp.row / c.num_layers, l = fp.row - i * c.num_layers, m = a.cu[i + 1] - a.cu[i];
+        const int32_t* keep = a.keep + l * a.keep_ls + a.cu[i];
+        const int32_t* t = table_row(c, l, a.src[i]);
+        const int64_t to = pool_row(c, l, w.fresh[f], 0);
+        for (int j0 = fp.page * bs; j0 < min(m, (fp.page + 1) * bs); j0 += MOVE_TOKENS) {
+            const int count = min(min(m, (fp.page + 1) * bs) - j0, MOVE_TOKENS);
             __syncthreads();
             for (int x = tid; x < count * r.pairs; x += MOVE_THREADS) {
                 const int k = x / r.pairs, e = x - k * r.pairs;
-                if (s_table[k]) rotary_angle(r, e, s_shift[k], cs + k * 2 * r.pairs + e, cs + k * 2 * r.pairs + r.pairs + e);
+                rotary_angle(r, e, j0 + k - keep[j0 + k], cs + k * 2 * r.pairs + e, cs + k * 2 * r.pairs + r.pairs + e);
             }
-            if constexpr (VEC > 1) move_v<T, VEC>(vp, dst, s_from, count, H * D);
-            __syncthreads();  // the tables
+            __syncthreads();
             for (int k = tid >> 5; k < count; k += MOVE_THREADS / 32) {
-                if (s_from[k] < 0) continue;
-                const T* src = kp + s_from[k];
-                T* out = kp + dst + (int64_t)k * H * D;
-                int own = k;
-                while (s_shift[k] && !s_table[own]) --own;
-                const float* tab = cs + own * 2 * r.pairs;
-                if constexpr (VEC > 1) {
-                    if (s_shift[k]) turn_row<T, VEC, IL>(src, out, H, D, r, tab);
-                    else copy_row<T, VEC>(src, out, H * D);
-                } else {
-                    for (int x = tid & 31; x < H * D; x += 32) {
-                        const int d = x % D - r.offset;
-                        float v = Elem<T>::to_f(src[x]);
-                        if (s_shift[k] && d >= 0 && d < 2 * r.pairs) {
-                            const bool low = IL ? !(d & 1) : d < r.pairs;  // first or second of its pair
-                            const int e = IL ? d / 2 : low ? d : d - r.pairs, step = IL ? 1 : r.pairs;
-                            const float o = Elem<T>::to_f(src[low ? x + step : x - step]);
-                            v = low ? v * tab[e] - o * tab[r.pairs + e] : o * tab[r.pairs + e] + v * tab[e];
-                        }
-                        out[x] = Elem<T>::from_f(v);
+                const int from = keep[j0 + k], b = t[from / bs];
+                if ((unsigned)b >= (unsigned)c.num_blocks) {
+                    if (lane == 0) set_error(c, MENTAT_DEV_BAD_BLOCK, b);
+                    continue;
+                }
+                const int64_t src = pool_row(c, l, b, from % bs), dst = to + (int64_t)(j0 + k - fp.page * bs) * n;
+                const float* tab = cs + k * 2 * r.pairs;
+                for (int x = lane; x < n; x += 32) {
+                    const int d = x % D - r.offset;
+                    float v = Elem<T>::to_f(kp[src + x]);
+                    if (from != j0 + k && d >= 0 && d < 2 * r.pairs) {
+                        const bool low = IL ? !(d & 1) : d < r.pairs;  // first or second of its pair
+                        const int e = IL ? d / 2 : low ? d : d - r.pairs, step = IL ? 1 : r.pairs;
+                        const float o = Elem<T>::to_f(kp[src + (low ? x + step : x - step)]);
+                        v = low ? v * tab[e] - o * tab[r.pairs + e] : o * tab[r.pairs + e] + v * tab[e];
                     }
-                    for (int x = tid & 31; x < H * D; x += 32) vp[dst + (int64_t)k * H * D + x] = vp[s_from[k] + x];
+                    kp[dst + x] = Elem<T>::from_f(v);
+                    vp[dst + x] = vp[src + x];
                 }
             }
         }
     }
+}
+
+// A token's heads turned in place in shared memory by a table (cosines, then sines), a warp.  Where the 32 lanes
+// cover whole heads, a lane has the same pairs in every head and keeps their cosines and sines.
+template <typename T, int VEC, bool IL>
+__device__ __forceinline__ void turn_row(T* row, int H, int D, const mentat_rotary& r, const float* tab) {
+    using P = Pack<T, VEC>;
+    const int lane = threadIdx.x & 31, pairs = r.pairs, off = r.offset;
+    const int tasks = IL ? 2 * pairs / VEC : pairs / VEC, total = H * tasks;
+    constexpr int N = IL ? VEC / 2 : VEC;
+    float co[N], sn[N];
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            co[e] = tab[t * N + e];
+            sn[e] = tab[pairs + t * N + e];
+        }
+    };
+    const bool whole = 32 % tasks == 0;
+    if (whole) fetch(lane % tasks);
+    for (int x = lane; x < total; x += 32) {
+        const int h = x / tasks, t = x - h * tasks;
+        if (!whole) fetch(t);
+        T* p = row + h * D + off + t * VEC;
+        P a = *reinterpret_cast<const P*>(p);
+        if (IL) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float u = Elem<T>::to_f(a.v[2 * e]), v = Elem<T>::to_f(a.v[2 * e + 1]);
+                a.v[2 * e] = Elem<T>::from_f(u * co[e] - v * sn[e]);
+                a.v[2 * e + 1] = Elem<T>::from_f(u * sn[e] + v * co[e]);
+            }
+        } else {
+            P b = *reinterpret_cast<const P*>(p + pairs);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float u = Elem<T>::to_f(a.v[e]), v = Elem<T>::to_f(b.v[e]);
+                a.v[e] = Elem<T>::from_f(u * co[e] - v * sn[e]);
+                b.v[e] = Elem<T>::from_f(u * sn[e] + v * co[e]);
+            }
+            *reinterpret_cast<P*>(p + pairs) = b;
+        }
+        *reinterpret_cast<P*>(p) = a;
+    }
+}
+
+// The same with the rows in shared memory: persistent CTAs take ranges of the fresh pages, `tokens` rows at a time
+// through a ring of stages.  A producer warp looks up where the rows come from and copies them in with bulk
+// copies, K and V, a stage ahead or more; eight warps turn K in place; the stage, which is contiguous in the
+// fresh page, leaves as two bulk copies.  So the bytes pass through registers only where they change, and the
+// next rows are always on the way.  Bound by memory.
+constexpr int STREAM_WORKERS = 256, STREAM_THREADS = STREAM_WORKERS + 32, STREAM_MAX_STAGES = 4;
+template <typename T, int VEC, bool IL>
+__global__ void __launch_bounds__(STREAM_THREADS) k_compact_stream(mentat_kv_cache c, CompactArgs a, mentat_rotary r,
+                                                                   int tokens, int stages, PagesWs w) {
+    extern __shared__ __align__(128) uint8_t ring[];  // [stages][K, V][tokens][row], then cosines and sines [tokens][2 pairs]
+    __shared__ uint64_t s_full[STREAM_MAX_STAGES], s_empty[STREAM_MAX_STAGES];
+    __shared__ int s_shift[STREAM_MAX_STAGES][MOVE_TOKENS], s_count[STREAM_MAX_STAGES], s_abort;
+    __shared__ int64_t s_to[STREAM_MAX_STAGES];
+    const int tid = threadIdx.x, lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(smem_u32(s_full + s), 1);
+            mbar_init(smem_u32(s_empty + s), 1);
+        }
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    griddep_wait();
+    griddep_launch();
+    if (*w.stop) return;
+    __syncthreads();
+    if (a.dst) install_new(c, a, w, gridDim.x);
+    const int D = c.head_dim, H = c.num_kv_heads, bs = c.block_size, rows = a.n * c.num_layers;
+    const uint32_t row_bytes = H * D * sizeof(T), tile = tokens * row_bytes;
+    const int64_t total = w.stop[1];
+    const int f0 = (int)(total * blockIdx.x / gridDim.x), f1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
+    const int groups = (bs + tokens - 1) / tokens, items = (f1 - f0) * groups;
+    T* kp = reinterpret_cast<T*>(c.k_pool);
+    T* vp = reinterpret_cast<T*>(c.v_pool);
+    if (tid >= STREAM_WORKERS) {  // producer
+        FreshPage fp = fresh_page(w, rows, min(f0, (int)total - 1 < 0 ? 0 : (int)total - 1));
+        int row_end = 0, i = 0, l = 0, m = 0, it = 0;
+        const int32_t *keep = nullptr, *t = nullptr;
+        auto enter = [&]() {  // fp.row's data
+            i = fp.row / c.num_layers;
+            l = fp.row - i * c.num_layers;
+            m = a.cu[i + 1] - a.cu[i];
+            keep = a.keep + l * a.keep_ls + a.cu[i];
+            t = table_row(c, l, a.src[i]);
+            row_end = w.first[fp.row] + w.count[fp.row];
+        };
+        if (items) enter();
+        for (; it < items; ++it) {
+            const int f = f0 + it / groups, s = it % stages;
+            if (it % groups == 0 && it) {
+                ++fp.page;
+                while (f >= row_end) {  // the next row with fresh pages
+                    ++fp.row;
+                    fp.page = w.lead[fp.row];
+                    enter();
+                }
+            }
+            const int j0 = fp.page * bs + it % groups * tokens;
+            const int count = max(0, min(min(m, (fp.page + 1) * bs) - j0, tokens));
+            int from = -1;
+            int64_t src = -1;
+            if (lane < count) {
+                from = keep[j0 + lane];
+                const int b = t[from / bs];
+                if ((unsigned)b < (unsigned)c.num_blocks) src = pool_row(c, l, b, from % bs);
+                else set_error(c, MENTAT_DEV_BAD_BLOCK, b);
+            }
+            const int to = w.fresh[f];
+            if (it >= stages && !__all_sync(0xffffffffu, mbar_wait(smem_u32(s_empty + s), (it / stages - 1) & 1))) {
+                if (lane == 0) {
+                    set_error(c, MENTAT_DEV_DECODE_TIMEOUT, 9);
+                    *(volatile int*)&s_abort = 1;
+                }
+                break;
+            }
+            if (lane < tokens) s_shift[s][lane] = src >= 0 && r.pairs ? j0 + lane - from : 0;
+            if (lane == 0) {
+                s_count[s] = count;
+                s_to[s] = pool_row(c, l, to, 0) + (int64_t)(j0 - fp.page * bs) * H * D;
+            }
+            const uint32_t good = __ballot_sync(0xffffffffu, src >= 0);
+            __syncwarp();
+            const uint32_t bar = smem_u32(s_full + s), dst = smem_u32(ring) + s * 2 * tile + lane * row_bytes;
+            if (lane == 0) mbar_expect_tx(bar, 2 * row_bytes * __popc(good));
+            __syncwarp();
+            if (src >= 0) {
+                bulk_load(dst, kp + src, row_bytes, bar);
+                bulk_load(dst + tile, vp + src, row_bytes, bar);
+            }
+        }
+        // every stage that was asked for has arrived before the CTA may end
+        for (int k = max(0, it - stages); k < it; ++k) (void)mbar_wait(smem_u32(s_full + k % stages), (k / stages) & 1);
+        return;
+    }
+    float* tab = reinterpret_cast<float*>(ring + (size_t)stages * 2 * tile);
+    for (int it = 0; it < items; ++it) {
+        const int s = it % stages;
+        if (!mbar_wait(smem_u32(s_full + s), (it / stages) & 1)) {
+            set_error(c, MENTAT_DEV_DECODE_TIMEOUT, 10);
+            *(volatile int*)&s_abort = 1;
+        }
+        const int count = s_count[s];
+        if (r.pairs) {
+            for (int x = tid; x < count * r.pairs; x += STREAM_WORKERS) {
+                const int k = x / r.pairs, e = x - k * r.pairs, shift = s_shift[s][k];
+                // neighbours that moved together share the table of the first of them
+                if (shift && (k == 0 || s_shift[s][k - 1] != shift))
+                    rotary_angle(r, e, shift, tab + k * 2 * r.pairs + e, tab + k * 2 * r.pairs + r.pairs + e);
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            for (int k = tid >> 5; k < count; k += STREAM_WORKERS / 32) {
+                const int shift = s_shift[s][k];
+                if (!shift) continue;
+                int own = k;
+                while (own && s_shift[s][own - 1] == shift) --own;
+                turn_row<T, VEC, IL>(reinterpret_cast<T*>(ring + (size_t)s * 2 * tile + k * row_bytes), H, D, r,
+                                     tab + own * 2 * r.pairs);
+            }
+            fence_proxy_async();
+        }
+        // the workers leave together, whatever each has seen of the flag
+        int gone;
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\t"
+                     "selp.s32 %0, 1, 0, q;\n\t}"
+                     : "=r"(gone)
+                     : "r"(*(volatile int*)&s_abort)
+                     : "memory");
+        if (gone) break;
+        if (tid == 0) {
+            if (count) {
+                bulk_store(kp + s_to[s], smem_u32(ring) + s * 2 * tile, count * row_bytes);
+                bulk_store(vp + s_to[s], smem_u32(ring) + s * 2 * tile + tile, count * row_bytes);
+            } else {
+                asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.commit_group;" ::: "memory");
+            }
+            // the stage before has been read by its copies: two groups a stage
+            asm volatile("cp.async.bulk.wait_group.read 2;" ::: "memory");
+            if (it) mbar_arrive(smem_u32(s_empty + (it - 1) % stages));
+        }
+    }
+    if (tid == 0) bulk_wait_all();
 }
 
 }  // namespace mentat
@@ -713,7 +846,9 @@ static int launch_one_cluster(void (*kernel)(KArgs...), size_t smem, cudaStream_
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    if (cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...) != cudaSuccess) {
+    if ((smem > 40 * 1024 &&
+         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) ||
+        cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...) != cudaSuccess) {
         (void)cudaGetLastError();
         return MENTAT_ERR_CUDA;
     }
@@ -721,24 +856,25 @@ static int launch_one_cluster(void (*kernel)(KArgs...), size_t smem, cudaStream_
     return MENTAT_OK;
 }
 
-// Releases of up to this many table entries (rows times the longest table) are one cluster's work.
-constexpr int64_t FREE_CLUSTER_ENTRIES = 32768;
+// Releases are one cluster's work while a warp has at most this many groups of 32 table entries.
+constexpr int FREE_CLUSTER_PER = 4;
 
 template <bool LEAD>
 static int launch_free(const mentat_kv_cache* c, const int32_t* slots, const int32_t* cu, int32_t n, int32_t max_nb,
                        const PagesWs& w, cudaStream_t s) {
-    const int rows = n * c->num_layers;
-    if ((int64_t)rows * max_nb <= FREE_CLUSTER_ENTRIES)
-        return launch_one_cluster(k_free_cluster<LEAD>, bitmap_bytes(c), s, *c, slots, cu, n, w);
+    const int rows = n * c->num_layers, chunks = max_nb < 1 ? 1 : (max_nb + 31) / 32;
+    const int64_t per = ((int64_t)rows * chunks + CLUSTER_ALL_WARPS - 1) / CLUSTER_ALL_WARPS;
+    const size_t held = (size_t)CLUSTER_WARPS * per * 32 * 4;
+    if (per <= FREE_CLUSTER_PER && held + bitmap_bytes(c) <= 100 * 1024)
+        return launch_one_cluster(k_free_cluster<LEAD>, held + bitmap_bytes(c), s, *c, slots, cu, n, chunks, (int)per, w);
+    const dim3 clear(chunks_of(c->num_blocks, 1024, 148)), by_row((rows + PAGES_WARPS - 1) / PAGES_WARPS);
     if (!LEAD)
-        MENTAT_LAUNCH(k_pages_begin, dim3(chunks_of(c->num_blocks, 1024, 148)), dim3(256), bitmap_bytes(c), s, *c, slots, n, w);
+        MENTAT_LAUNCH(k_pages_begin, clear, dim3(256), bitmap_bytes(c), s, *c, slots, n, (int)by_row.x, w);
     else
-        MENTAT_LAUNCH(k_order_clear, dim3(chunks_of(c->num_blocks, 1024, 148)), dim3(256), 0, s, *c, w);
+        MENTAT_LAUNCH(k_order_clear, clear, dim3(256), 0, s, *c, (int)by_row.x, w);
     const dim3 marks((n + MARK_SEQS - 1) / MARK_SEQS * c->num_layers, chunks_of(max_nb, 256, 64));
-    const dim3 by_row((rows + PAGES_WARPS - 1) / PAGES_WARPS);
     MENTAT_LAUNCH(k_free_mark<LEAD>, marks, dim3(256), 0, s, *c, slots, n, w);
     MENTAT_LAUNCH(k_free_count<LEAD>, by_row, dim3(PAGES_THREADS), 0, s, *c, slots, rows, w);
-    MENTAT_LAUNCH(k_free_scan, dim3(1), dim3(1024), 0, s, *c, rows, w);
     MENTAT_LAUNCH(k_free_push<LEAD>, by_row, dim3(PAGES_THREADS), 0, s, *c, slots, cu, rows, w);
     return MENTAT_OK;
 }
@@ -753,14 +889,35 @@ struct LaunchCompactMove {
     cudaStream_t s;
     template <typename T, int VEC, bool IL>
     int operator()() {
-        const dim3 grid(a.n * c.num_layers, chunks_of(max_keep, c.block_size, 65535));
-        const size_t smem = (size_t)MOVE_TOKENS * 2 * r.pairs * sizeof(float);
-        if (smem > 40 * 1024 && cudaFuncSetAttribute(k_compact_move<T, VEC, IL>,
-                                                     cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+        const int64_t rows = (int64_t)a.n * c.num_layers, most = rows * ((max_keep + c.block_size - 1) / c.block_size);
+        const size_t table = (size_t)MOVE_TOKENS * 2 * r.pairs * sizeof(float);
+        if constexpr (VEC > 1) {
+            // stages of up to 16 tokens and 64 KB, three of them or four; several CTAs on an SM where they are small
+            const int64_t row = (int64_t)c.num_kv_heads * c.head_dim * sizeof(T);
+            int tokens = c.block_size < MOVE_TOKENS ? c.block_size : MOVE_TOKENS;
+            while (tokens > 1 && 2 * tokens * row > 64 * 1024) tokens /= 2;
+            const int64_t room = 220 * 1024 - (int64_t)table - 1024, stage = 2 * tokens * row;
+            int stages = (int)(room / stage < STREAM_MAX_STAGES ? room / stage : STREAM_MAX_STAGES);
+            if (stages >= 2) {
+                const size_t smem = stages * stage + table;
+                int per_sm = (int)(220 * 1024 / (smem + 2048));
+                per_sm = per_sm < 1 ? 1 : per_sm > 6 ? 6 : per_sm;
+                const auto kernel = k_compact_stream<T, VEC, IL>;
+                if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+                    (void)cudaGetLastError();
+                    return MENTAT_ERR_CUDA;
+                }
+                MENTAT_LAUNCH(kernel, dim3(chunks_of(most, 1, 148 * per_sm)), dim3(STREAM_THREADS), smem, s, c, a, r, tokens,
+                              stages, w);
+                return MENTAT_OK;
+            }
+        }
+        if (table > 40 * 1024 && cudaFuncSetAttribute(k_compact_move<T, IL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                      (int)table) != cudaSuccess) {
             (void)cudaGetLastError();
             return MENTAT_ERR_CUDA;
         }
-        MENTAT_LAUNCH(k_compact_move<T, VEC, IL>, grid, dim3(MOVE_THREADS), smem, s, c, a, r, w);
+        MENTAT_LAUNCH((k_compact_move<T, IL>), dim3(chunks_of(most, 1, 148 * 8)), dim3(MOVE_THREADS), table, s, c, a, r, w);
         return MENTAT_OK;
     }
 };
@@ -785,7 +942,7 @@ int mentat_kv_fork_batched(const mentat_kv_cache* c, const int32_t* parents, con
 
 int mentat_kv_free_batched(const mentat_kv_cache* c, const int32_t* slots, int32_t n, int32_t max_nb, void* workspace,
                            int64_t workspace_bytes, cudaStream_t s) {
-    if (bad_pages(c, n) || max_nb < 0 || (n > 0 && (!slots || !workspace))) return MENTAT_ERR_ARG;
+    if (bad_pages(c, n) || max_nb < 0 || (n > 0 && (!slots || !workspace || ((uintptr_t)workspace & 15)))) return MENTAT_ERR_ARG;
     if (n == 0) return MENTAT_OK;
     if (!pages_fit(c, n)) return MENTAT_ERR_UNSUPPORTED;
     PagesWs w;
@@ -797,7 +954,7 @@ int mentat_kv_compact(const mentat_kv_cache* c, const int32_t* src, const int32_
                       int64_t keep_ls, const int32_t* cu, int32_t max_keep, int32_t max_nb, const mentat_rotary* r,
                       void* workspace, int64_t workspace_bytes, cudaStream_t s) {
     if (bad_pages(c, n) || max_keep < 0 || max_nb < 0 || keep_ls < 0 || c->head_dim <= 0 || c->num_kv_heads <= 0 ||
-        (n > 0 && (!src || !cu || !workspace || !c->k_pool || !c->v_pool || (max_keep > 0 && !keep))) ||
+        (n > 0 && (!src || !cu || !workspace || ((uintptr_t)workspace & 15) || !c->k_pool || !c->v_pool || (max_keep > 0 && !keep))) ||
         (r && !rotary_ok(r, c->head_dim)))
         return MENTAT_ERR_ARG;
     if (n == 0) return MENTAT_OK;
