@@ -355,7 +355,7 @@ struct AppendRotaryArgs {
 };
 
 template <typename T, int VEC, bool IL>
-__global__ void __launch_bounds__(256) k_append_rotary_data(mentat_kv_cache c, int layer, int n, AppendRotaryArgs a) {
+__global__ void __launch_bounds__(ROTARY_THREADS) k_append_rotary_data(mentat_kv_cache c, int layer, int n, AppendRotaryArgs a) {
     extern __shared__ float cs[];
     griddep_wait();
     griddep_launch();
@@ -505,7 +505,7 @@ __global__ void k_append_multi_data(mentat_kv_cache c, int layer, int slot, int 
 
 // the same with q and k turned on the way
 template <typename T, int VEC, bool IL>
-__global__ void __launch_bounds__(256) k_append_multi_rotary_data(mentat_kv_cache c, int layer, int slot, int n,
+__global__ void __launch_bounds__(ROTARY_THREADS) k_append_multi_rotary_data(mentat_kv_cache c, int layer, int slot, int n,
                                                                   AppendRotaryArgs a) {
     extern __shared__ float cs[];
     const int32_t* sc = c.scratch;
@@ -661,10 +661,10 @@ struct LaunchAppendRotary {
     int operator()() {
         const size_t smem = 2 * a.r.pairs * sizeof(float);
         if (slot >= 0) {
-            k_append_multi_rotary_data<T, VEC, IL><<<n < 1184 ? n + 1 : 1185, 256, smem, s>>>(c, layer, slot, n, a);
+            k_append_multi_rotary_data<T, VEC, IL><<<n < 148 * 16 ? n + 1 : 148 * 16 + 1, ROTARY_THREADS, smem, s>>>(c, layer, slot, n, a);
             MENTAT_CHECK_LAUNCH();
         } else {
-            MENTAT_LAUNCH(k_append_rotary_data<T, VEC, IL>, dim3(n), dim3(256), smem, s, c, layer, n, a);
+            MENTAT_LAUNCH(k_append_rotary_data<T, VEC, IL>, dim3(n), dim3(ROTARY_THREADS), smem, s, c, layer, n, a);
         }
         return MENTAT_OK;
     }

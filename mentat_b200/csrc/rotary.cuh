@@ -14,6 +14,7 @@
 
 namespace mentat {
 
+constexpr int ROTARY_THREADS = 128;   // most threads that share a token
 constexpr int ROTARY_MAX_DIM = 1024;  // largest head_dim of the rotary entry points
 
 __device__ __forceinline__ void rotary_angle(const mentat_rotary& r, int i, int64_t pos, float* c, float* s) {

@@ -219,35 +219,56 @@ __global__ void k_index_seqs(mentat_kv_cache c, int layer0, const int32_t* slots
     else index_page<T>(c, layer, b, blockIdx.y, x);
 }
 
-__global__ void __launch_bounds__(256) k_page_bounds(mentat_kv_cache c, int layer, const int32_t* blocks, mentat_page_index x,
-                                                     float* low, float* high, int8_t* exps) {
+// Four pages to a CTA, each thread one piece of each of them on the way.
+constexpr int BOUNDS_PAGES = 4;
+__global__ void __launch_bounds__(256) k_page_bounds(mentat_kv_cache c, int layer, const int32_t* blocks, int n,
+                                                     mentat_page_index x, float* low, float* high, int8_t* exps) {
     griddep_wait();
     griddep_launch();
-    const int b = blocks[blockIdx.x], D = c.head_dim, H = c.num_kv_heads;
-    if ((unsigned)b >= (unsigned)c.num_blocks) {
-        if (threadIdx.x == 0) set_error(c, MENTAT_DEV_BAD_BLOCK, b);
-        return;
+    const int D = c.head_dim, H = c.num_kv_heads, i0 = blockIdx.x * BOUNDS_PAGES;
+    int64_t at[BOUNDS_PAGES];  // of the page's first head; -1: none
+#pragma unroll
+    for (int k = 0; k < BOUNDS_PAGES; ++k) {
+        const int b = i0 + k < n ? blocks[i0 + k] : -1;
+        at[k] = (unsigned)b < (unsigned)c.num_blocks ? ((int64_t)layer * c.num_blocks + b) * H : -1;
+        if (i0 + k < n && at[k] < 0 && threadIdx.x == 0) set_error(c, MENTAT_DEV_BAD_BLOCK, b);
     }
-    const int64_t at = ((int64_t)layer * c.num_blocks + b) * H, to = (int64_t)blockIdx.x * H;
-    auto value = [&](int v, int e) { return e == EXP_ALL ? 0.f : v * pow2(e); };
+    auto value = [&](int v, int e) { return v * pow2(e); };
+    const int64_t to = (int64_t)i0 * H;
     if (D % 4 == 0 && (((uintptr_t)low | (uintptr_t)high) & 15) == 0 && ((uintptr_t)x.bounds & 3) == 0) {
         for (int u = threadIdx.x; u < H * D / 2; u += blockDim.x) {  // 4 bytes to 16
-            const int h = u / (D / 2), r = u - h * (D / 2), d = r % (D / 4) * 4, e = x.exps[at + h];
+            const int h = u / (D / 2), r = u - h * (D / 2);
             const bool top = r >= D / 4;
-            const char4 v = *reinterpret_cast<const char4*>(x.bounds + (at + h) * 2 * D + (top ? D : 0) + d);
+            const int d = (top ? r - D / 4 : r) * 4;
+            char4 v[BOUNDS_PAGES];
+            int e[BOUNDS_PAGES];
+#pragma unroll
+            for (int k = 0; k < BOUNDS_PAGES; ++k)
+                if (at[k] >= 0) {
+                    v[k] = *reinterpret_cast<const char4*>(x.bounds + (at[k] + h) * 2 * D + (top ? D : 0) + d);
+                    e[k] = x.exps[at[k] + h];
+                }
             const float inf = top ? INFINITY : -INFINITY;
-            *reinterpret_cast<float4*>((top ? high : low) + (to + h) * D + d) =
-                e == EXP_ALL ? make_float4(inf, inf, inf, inf)
-                             : make_float4(value(v.x, e), value(v.y, e), value(v.z, e), value(v.w, e));
+#pragma unroll
+            for (int k = 0; k < BOUNDS_PAGES; ++k)
+                if (at[k] >= 0)
+                    *reinterpret_cast<float4*>((top ? high : low) + (to + (int64_t)k * H + h) * D + d) =
+                        e[k] == EXP_ALL ? make_float4(inf, inf, inf, inf)
+                                        : make_float4(value(v[k].x, e[k]), value(v[k].y, e[k]), value(v[k].z, e[k]),
+                                                      value(v[k].w, e[k]));
         }
     } else {
-        for (int u = threadIdx.x; u < H * D; u += blockDim.x) {
-            const int h = u / D, d = u - h * D, e = x.exps[at + h];
-            low[(to + h) * D + d] = e == EXP_ALL ? -INFINITY : value(x.bounds[(at + h) * 2 * D + d], e);
-            high[(to + h) * D + d] = e == EXP_ALL ? INFINITY : value(x.bounds[(at + h) * 2 * D + D + d], e);
+        for (int u = threadIdx.x; u < BOUNDS_PAGES * H * D; u += blockDim.x) {
+            const int k = u / (H * D), h = u / D % H, d = u % D;
+            if (at[k] < 0) continue;
+            const int e = x.exps[at[k] + h];
+            const int8_t* b = x.bounds + (at[k] + h) * 2 * D + d;
+            low[(to + (int64_t)k * H + h) * D + d] = e == EXP_ALL ? -INFINITY : value(b[0], e);
+            high[(to + (int64_t)k * H + h) * D + d] = e == EXP_ALL ? INFINITY : value(b[D], e);
         }
     }
-    for (int h = threadIdx.x; h < H; h += blockDim.x) exps[to + h] = x.exps[at + h];
+    for (int u = threadIdx.x; u < BOUNDS_PAGES * H; u += blockDim.x)
+        if (at[u / H] >= 0) exps[to + u] = x.exps[at[u / H] + u % H];
 }
 
 // ---------------------------------------------------------------------------
@@ -705,7 +726,13 @@ __device__ __forceinline__ void attend_simple(const mentat_kv_cache& c, const Sp
             for (int g = 0; g < GM; ++g) {
                 if (g >= G) break;
 #pragma unroll
-                for (int j = 0; j < V; ++j) s[g] = fmaf(Elem<T>::to_f(kv.v[j]), qh[g * D + d + j], s[g]);
+                for (int j = 0; j < V; j += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(qh + g * D + d + j);
+                    s[g] = fmaf(Elem<T>::to_f(kv.v[j]), x.x, s[g]);
+                    s[g] = fmaf(Elem<T>::to_f(kv.v[j + 1]), x.y, s[g]);
+                    s[g] = fmaf(Elem<T>::to_f(kv.v[j + 2]), x.z, s[g]);
+                    s[g] = fmaf(Elem<T>::to_f(kv.v[j + 3]), x.w, s[g]);
+                }
             }
         }
 #pragma unroll
@@ -1491,7 +1518,8 @@ int mentat_page_bounds(const mentat_kv_cache* c, int32_t layer, const int32_t* b
     if (bad_index(c, x) || layer < 0 || layer >= c->num_layers || n < 0 || (n > 0 && (!blocks || !low || !high || !exps)))
         return MENTAT_ERR_ARG;
     if (n == 0) return MENTAT_OK;
-    MENTAT_LAUNCH(k_page_bounds, dim3(n), dim3(256), 0, s, *c, layer, blocks, *x, low, high, exps);
+    MENTAT_LAUNCH(k_page_bounds, dim3((n + BOUNDS_PAGES - 1) / BOUNDS_PAGES), dim3(256), 0, s, *c, layer, blocks, n, *x, low,
+                  high, exps);
     return MENTAT_OK;
 }
 

@@ -258,48 +258,64 @@ _row_args = _RowArgs()
 _pack_rows = struct.Struct("@Pqqi4xPqqi4xPqqi4xPqqi4x").pack_into
 
 
+_NO_ROWS = (0, 0, 0, 0)
+
+
 def _rows(a, b, c, d) -> tuple:
-    """Addresses of the four tensors' ``mentat_rows`` (None: no heads)."""
-    args = []
-    for t in (a, b, c, d):
-        if t is None:
-            args += (0, 0, 0, 0)
-        else:
-            s0, s1, _ = t.stride()
-            args += (t.data_ptr(), s0, s1, t.shape[1])
+    """Addresses of four ``mentat_rows``, given as (address, token stride, head stride, heads)."""
     r = _row_args
-    _pack_rows(r.buf, 0, *args)
+    _pack_rows(r.buf, 0, *a, *b, *c, *d)
     return r.at
 
 
-def _check_rows(name: str, t: torch.Tensor, n: int, d: int, dtype, device) -> torch.Tensor:
-    shape = t.shape
+def _operand(name: str, t: torch.Tensor, n: int, d: int, dtype, device) -> tuple:
+    """``t`` checked as rows (n, heads, d), its last dimension made contiguous, and its ``mentat_rows``."""
+    shape, stride = t.shape, t.stride()
     if len(shape) != 3 or shape[0] != n or shape[2] != d:
         raise ValueError(f"{name} {tuple(shape)} is not ({n}, heads, {d})")
     if t.dtype is not dtype or dtype not in _DT:
         raise TypeError(f"{name} has dtype {t.dtype}, {dtype if dtype in _DT else 'float32, bfloat16 or float16'} expected")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, {device} expected")
-    return t if t.stride(2) == 1 or d == 1 else t.contiguous()
+    if stride[2] != 1 and d != 1:
+        t = t.contiguous()
+        stride = t.stride()
+    return t, (t.data_ptr(), stride[0], stride[1], shape[1])
 
 
-def _out_rows(name: str, out: Optional[torch.Tensor], x: torch.Tensor) -> torch.Tensor:
+def _like(x: torch.Tensor) -> tuple:
+    """A new tensor of x's shape, dtype and device, and its ``mentat_rows``."""
+    _, h, d = x.shape
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    return out, (out.data_ptr(), h * d, d, h)
+
+
+def _check_rows(name: str, t: torch.Tensor, n: int, d: int, dtype, device) -> torch.Tensor:
+    return _operand(name, t, n, d, dtype, device)[0]
+
+
+def _out_rows(name: str, out: Optional[torch.Tensor], x: torch.Tensor) -> tuple:
     """``out`` checked as the result of a row operation on ``x``: its own rows distinct, and
-    either ``x`` itself or apart from it; a new tensor if None."""
+    either ``x`` itself or apart from it; a new tensor if None.  With its ``mentat_rows``."""
     if out is None:
-        return torch.empty_like(x, memory_format=torch.contiguous_format)
+        return _like(x)
+    _check_out(name, out, x)
+    return out, (out.data_ptr(), out.stride(0), out.stride(1), out.shape[1])
+
+
+def _check_out(name: str, out: torch.Tensor, x: torch.Tensor) -> None:
     n, h, d = x.shape
     if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
         raise ValueError(f"{name} must have the input's shape, dtype and device")
     if x.numel() == 0:
-        return out
+        return
     s0, s1 = out.stride(0), out.stride(1)
     if (d > 1 and out.stride(2) != 1) or not (
             ((h == 1 or s1 >= d) and (n == 1 or s0 >= (h - 1) * s1 * (h > 1) + d)) or
             ((n == 1 or s0 >= d) and (h == 1 or s1 >= (n - 1) * s0 * (n > 1) + d))):
         raise ValueError(f"{name} must hold rows of its own, each contiguous")
     if out.data_ptr() == x.data_ptr() and out.stride() == x.stride():
-        return out
+        return
 
     def span(t):
         a = t.data_ptr()
@@ -307,16 +323,15 @@ def _out_rows(name: str, out: Optional[torch.Tensor], x: torch.Tensor) -> torch.
     (a0, a1), (b0, b1) = span(out), span(x)
     if a0 < b1 and b0 < a1:
         raise ValueError(f"{name} must be the input itself or not overlap it")
-    return out
 
 
 def _check_positions(positions: torch.Tensor, n: int, device) -> torch.Tensor:
-    if positions.shape != (n,) or positions.dtype not in (torch.int64, torch.int32):
+    dtype = positions.dtype
+    if positions.shape != (n,) or (dtype is not torch.int64 and dtype is not torch.int32):
         raise ValueError(f"positions must be {n} int64 or int32 values")
     if positions.device != device:
         raise ValueError(f"positions are on {positions.device}, {device} expected")
-    return positions.to(torch.int64).contiguous() if positions.dtype is torch.int32 or n > 1 and positions.stride(0) != 1 \
-        else positions
+    return positions if dtype is torch.int64 and positions.is_contiguous() else positions.to(torch.int64).contiguous()
 
 
 def _check_rotary(rotary, d: int, device) -> None:
@@ -343,17 +358,18 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     Returns (q, k): new tensors, or ``q_out`` / ``k_out``, which may be the inputs
     themselves.  Any token and head strides; wraps ``mentat_rotary_apply``."""
     n, _, d = q.shape
-    q = _check_rows("q", q, n, d, q.dtype, q.device)
-    _check_rotary(rotary, d, q.device)
-    positions = _check_positions(positions, n, q.device)
-    qo = _out_rows("q_out", q_out, q)
-    ko = None
+    dtype, dev = q.dtype, q.device
+    q, rq = _operand("q", q, n, d, dtype, dev)
+    _check_rotary(rotary, d, dev)
+    positions = _check_positions(positions, n, dev)
+    qo, rqo = _out_rows("q_out", q_out, q)
+    ko, rk, rko = None, _NO_ROWS, _NO_ROWS
     if k is not None:
-        k = _check_rows("k", k, n, d, q.dtype, q.device)
-        ko = _out_rows("k_out", k_out, k)
+        k, rk = _operand("k", k, n, d, dtype, dev)
+        ko, rko = _out_rows("k_out", k_out, k)
     if n:
-        _call(q.device, "mentat_rotary_apply", _DT[q.dtype], d, n, *_rows(q, qo, k, ko),
-              positions.data_ptr(), rotary._ptrs[bool(inverse)])
+        _call(dev, "mentat_rotary_apply", _DT[dtype], d, n, *_rows(rq, rqo, rk, rko), positions.data_ptr(),
+              rotary._ptrs[bool(inverse)])
     return qo, ko
 
 
@@ -365,25 +381,26 @@ def rotary_append(cache, layer: int, rows: torch.Tensor, q: Optional[torch.Tenso
     distinct; -1 writes none.  Returns the turned queries.  The tables and lengths
     are not touched; ``PagedKVCacheManager.append_rotated`` keeps them.  Wraps
     ``mentat_rotary_append``."""
-    n, _, d = k.shape
-    dev = cache.device
-    if d != cache.head_dim or k.shape[1] != cache.num_key_value_heads or v.shape[1] != k.shape[1]:
+    n, hkv, d = k.shape
+    dev, dtype = cache.device, cache.dtype
+    if d != cache.head_dim or hkv != cache.num_key_value_heads or v.shape[1] != hkv:
         raise ValueError("k or v shape does not match the cache geometry")
     if not 0 <= layer < cache.num_layers:
         raise ValueError(f"layer {layer} is not within 0 .. {cache.num_layers - 1}")
-    k, v = _check_rows("k", k, n, d, cache.dtype, dev), _check_rows("v", v, n, d, cache.dtype, dev)
+    k, rk = _operand("k", k, n, d, dtype, dev)
+    v, rv = _operand("v", v, n, d, dtype, dev)
     _check_rotary(rotary, d, dev)
     positions = _check_positions(positions, n, dev)
-    if rows.shape != (n,) or rows.dtype != torch.int64 or rows.device != dev:
+    if rows.shape != (n,) or rows.dtype is not torch.int64 or rows.device != dev:
         raise ValueError(f"rows must be {n} int64 values on {dev}")
     rows = rows.contiguous()
-    qo = None
+    qo, rq, rqo = None, _NO_ROWS, _NO_ROWS
     if q is not None:
-        q = _check_rows("q", q, n, d, cache.dtype, dev)
-        qo = _out_rows("q_out", q_out, q)
+        q, rq = _operand("q", q, n, d, dtype, dev)
+        qo, rqo = _out_rows("q_out", q_out, q)
     if n:
-        _call(dev, "mentat_rotary_append", cache._desc_ptr, layer, n, rows.data_ptr(),
-              *_rows(q, qo, k, v), positions.data_ptr(), rotary._ptrs[0])
+        _call(dev, "mentat_rotary_append", cache._desc_ptr, layer, n, rows.data_ptr(), *_rows(rq, rqo, rk, rv),
+              positions.data_ptr(), rotary._ptrs[0])
     return qo
 
 
@@ -395,13 +412,13 @@ def _append_rotated(k_pool: torch.Tensor, v_pool: torch.Tensor, slots: torch.Ten
     mgr, rot = _cache(cache), _cache(rotary)
     n, d = k.shape[0], k.shape[2]
     dev = mgr.device
-    q, k, v = (_check_rows(name, t, n, d, mgr.dtype, dev) for name, t in (("q", q), ("k", k), ("v", v)))
-    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+    (q, rq), (k, rk), (v, rv) = (_operand(name, t, n, d, mgr.dtype, dev) for name, t in (("q", q), ("k", k), ("v", v)))
+    qo, rqo = _like(q)
+    size = q.element_size()
     for a in range(0, n, 1024):
-        b = min(n, a + 1024)
-        _call(dev, "mentat_kv_append_rotated_batched", mgr._desc_ptr, layer,
-              slots.data_ptr() + 4 * a, b - a, *_rows(*((q, qo, k, v) if n <= 1024 else (x[a:b] for x in (q, qo, k, v)))),
-              None, rot._ptrs[0])
+        part = [(p + a * s0 * size, s0, s1, h) for p, s0, s1, h in (rq, rqo, rk, rv)] if a else (rq, rqo, rk, rv)
+        _call(dev, "mentat_kv_append_rotated_batched", mgr._desc_ptr, layer, slots.data_ptr() + 4 * a, min(n - a, 1024),
+              *_rows(*part), None, rot._ptrs[0])
     if mgr.page_index is not None:
         _index_tails(mgr, layer, slots, n)
     return qo

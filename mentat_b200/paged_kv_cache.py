@@ -665,22 +665,22 @@ class PagedKVCacheManager:
         sequence, or to ``positions`` (n,) int64; returns the turned queries."""
         seq = self._sequences[seq_id]
         n, d = k.shape[0], self.head_dim
-        k, v = (ops._check_rows(name, t, n, d, self.dtype, self.device) for name, t in (("k", k), ("v", v)))
+        (k, rk), (v, rv) = (ops._operand(name, t, n, d, self.dtype, self.device) for name, t in (("k", k), ("v", v)))
         if k.shape[1] != self.num_key_value_heads or v.shape[1] != self.num_key_value_heads:
             raise ValueError("k or v shape does not match the cache geometry")
         ops._check_rotary(rotary, d, self.device)
         if positions is not None:
             positions = ops._check_positions(positions, n, self.device)
-        qo = None
+        qo, rq, rqo = None, ops._NO_ROWS, ops._NO_ROWS
         if q is not None:
-            q = ops._check_rows("q", q, n, d, self.dtype, self.device)
-            qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q, rq = ops._operand("q", q, n, d, self.dtype, self.device)
+            qo, rqo = ops._like(q)
         if n == 0:
             return qo
         first = seq.num_tokens[layer_idx]
         self._mirror_append(seq, layer_idx, n)
         ops._call(self.device, "mentat_kv_append_rotated", self._desc_ptr, layer_idx, seq.slot, n,
-                  *ops._rows(q, qo, k, v), None if positions is None else positions.data_ptr(), rotary._ptrs[0])
+                  *ops._rows(rq, rqo, rk, rv), None if positions is None else positions.data_ptr(), rotary._ptrs[0])
         self._index_appended(seq, layer_idx, first)
         self._after()
         return qo
