@@ -333,14 +333,28 @@ __global__ void __launch_bounds__(CLUSTER_THREADS) k_free_cluster(mentat_kv_cach
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = cluster.block_rank();
     int* held = reinterpret_cast<int*>(dyn) + warp * per * 32 + lane;
     uint32_t* bits = dyn + CLUSTER_WARPS * per * 32;
-    bool stop = LEAD ? *w.stop != 0 : !slots_distinct(c, slots, n, bits, &s_bad);
-    if (!LEAD && stop && threadIdx.x == 0) set_error(c, MENTAT_DEV_BAD_SLOT, s_bad);
-    if (!LEAD) stop = __syncthreads_or(stop || has_error(c));
-    // an earlier error, or this one, stops every CTA: nothing of this call is recorded before all have looked
-    if (stop) return;
     const int rows = n * c.num_layers, items = rows * chunks, me = rank * CLUSTER_WARPS + warp;
     const int y0 = min(items, me * per), y1 = min(items, y0 + per);
+    // the entries are read while the batch is checked (a slot that is out of range has none)
     const long long tail0 = c.ctrl[MENTAT_CTRL_TAIL];
+    bool stop = LEAD ? *w.stop != 0 : has_error(c);
+    for (int y = y0; y < y1; ++y) {
+        const int row = y / chunks, j = y % chunks * 32 + lane, i = row / c.num_layers, l = row - i * c.num_layers;
+        const int slot = slots[i], lead = LEAD && !stop ? w.lead[row] : 0;
+        int b = -1;
+        if (slot >= 0 && slot < c.max_seqs && j >= lead && j < c.nblocks[seq_index(c, l, slot)]) {
+            b = table_row(c, l, slot)[j];
+            if ((unsigned)b >= (unsigned)c.num_blocks) b = -2;  // recorded once all CTAs have looked at the error word
+        }
+        held[(y - y0) * 32] = b;
+    }
+    if (!LEAD) {
+        const bool bad = !slots_distinct(c, slots, n, bits, &s_bad);
+        stop = __syncthreads_or(stop || bad);
+        if (bad && threadIdx.x == 0) set_error(c, MENTAT_DEV_BAD_SLOT, s_bad);
+    }
+    // an earlier error, or this one, stops every CTA: nothing of this call is recorded before all have looked
+    if (stop) return;
     // entries past an item's first 32 (a table longer than the launch was sized for) are read again each time
     auto rest = [&](int y, auto&& f) {
         if (y % chunks != chunks - 1) return;
@@ -353,18 +367,8 @@ __global__ void __launch_bounds__(CLUSTER_THREADS) k_free_cluster(mentat_kv_cach
         }
     };
     for (int y = y0; y < y1; ++y) {
-        const int row = y / chunks, j = y % chunks * 32 + lane, i = row / c.num_layers, l = row - i * c.num_layers;
-        const int slot = slots[i], nb = c.nblocks[seq_index(c, l, slot)];
-        int b = -1;
-        if (j < nb && (!LEAD || j >= w.lead[row])) {
-            b = table_row(c, l, slot)[j];
-            if ((unsigned)b >= (unsigned)c.num_blocks) {
-                b = -2;  // recorded once all CTAs have looked at the error word
-            } else {
-                w.order[b] = 0;
-            }
-        }
-        held[(y - y0) * 32] = b;
+        const int b = held[(y - y0) * 32];
+        if (b >= 0) w.order[b] = 0;
         rest(y, [&](int, int, int b) {
             if (b >= 0) w.order[b] = 0;
         });

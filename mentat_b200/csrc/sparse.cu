@@ -277,7 +277,9 @@ __global__ void __launch_bounds__(256) k_page_bounds(mentat_kv_cache c, int laye
 // The cluster's CTAs score a slice of the pages each and write the keys to all of their
 // shared memories; each then makes the whole choice for itself, attends to an equal share
 // of the chosen pages, and they merge their partials: one launch, and no workspace.
-constexpr int SPARSE_THREADS = 128, SPARSE_WARPS = SPARSE_THREADS / 32;
+// warps of a CTA: with the tensor-core path's rings two CTAs of four fit on an SM; the other path is bound by
+// latency and takes eight
+__host__ __device__ constexpr int sparse_warps(bool mma) { return mma ? 4 : 8; }
 constexpr int SPARSE_STAGES = 3;  // groups of 16 tokens that a warp holds or has on the way
 constexpr int SPARSE_MAX_BUDGET = 8192, SPARSE_MAX_GROUP = 16, SPARSE_MAX_CLUSTER = 16;
 
@@ -312,14 +314,14 @@ __host__ __device__ inline SparseSmem sparse_smem(int G, int GM, int D, bool mma
                                                   int share) {
     SparseSmem s;
     share = (share + 3) / 4 * 4;
-    const int attend = mma ? SPARSE_WARPS * SPARSE_STAGES * 16 * D : 0, partials = SPARSE_WARPS * G * D;
+    const int warps = sparse_warps(mma), attend = mma ? warps * SPARSE_STAGES * 16 * D : 0, partials = warps * G * D;
     s.po = s.q8 = 0;
     s.keys = (GM < 8 ? 8 : GM) * 2 * D / 4;
     const int chose = listed ? 0 : s.keys + (pages + 3 + 3) / 4 * 4;
     s.qf = attend > partials ? attend : partials;
     if (chose > s.qf) s.qf = chose;
     s.ml = s.qf + (mma ? 0 : G * D);
-    s.pages = s.ml + 2 * SPARSE_WARPS * GM;
+    s.pages = s.ml + 2 * warps * GM;
     s.blocks = s.pages + share;
     s.total = s.blocks + share;
     return s;
@@ -389,7 +391,7 @@ __device__ __forceinline__ void mma_s8(int* d, int a0, int a1, int a2, int a3, i
 // keys[p] of the pages p0 .. p1, to every CTA of the cluster.  A warp takes 16 pages at a time as
 // the rows of a product, 8 query heads (16 for GM 16) as its columns; the order of the
 // channels within the product is the one that lets a lane load 16 contiguous bytes of its page.
-template <int D, int GM>
+template <int D, int GM, int WARPS>
 __device__ __forceinline__ void score_pages(const mentat_kv_cache& c, const mentat_page_index& x, const SparseArgs& a,
                                             int h, const int32_t* row, int P, int p0, int p1, const int8_t* q8,
                                             const float* unit, uint32_t* keys) {
@@ -409,7 +411,7 @@ __device__ __forceinline__ void score_pages(const mentat_kv_cache& c, const ment
         u[nt][0] = unit[nt * 8 + 2 * t];
         u[nt][1] = unit[nt * 8 + 2 * t + 1];
     }
-    for (int p = p0 + warp * 16; p < p1; p += SPARSE_WARPS * 16) {
+    for (int p = p0 + warp * 16; p < p1; p += WARPS * 16) {
         int4 v[2][CH];
         int ek[2];
         bool ok[2];
@@ -689,7 +691,7 @@ __device__ __forceinline__ void choose_cluster(const uint32_t* keys, int p0, int
 
 // A warp's partial of the share's pages, without tensor cores: 16 tokens at a time; for Q K^T lane =
 // (half of D, token), for P V lane = D / 32 channels.  Writes m, l, o to the warp's rows.
-template <typename T, int D, int GM>
+template <typename T, int D, int GM, int WARPS>
 __device__ __forceinline__ void attend_simple(const mentat_kv_cache& c, const SparseArgs& a, int h, int len,
                                               const int32_t* pages, const int32_t* blocks, int count, const float* qf,
                                               float* pm, float* pl, float* po) {
@@ -704,7 +706,7 @@ __device__ __forceinline__ void attend_simple(const mentat_kv_cache& c, const Sp
         for (int j = 0; j < DL; ++j) o[g][j] = 0.f;
     }
     const int per = (bs + 15) / 16;  // groups of 16 rows of a page
-    for (int i = warp; i < count * per; i += SPARSE_WARPS) {
+    for (int i = warp; i < count * per; i += WARPS) {
         const int p = pages[i / per], b = blocks[i / per], t0 = (i % per) * 16;
         const int live = min(min(bs - t0, 16), len - (p * bs + t0));
         if (b < 0 || live <= 0) continue;
@@ -798,6 +800,7 @@ __device__ __forceinline__ void attend_mma(const mentat_kv_cache& c, const Spars
                                            const int32_t* blocks, int count, const T* q, uint8_t* ring, uint64_t* bars,
                                            float* pm, float* pl, float* po) {
     constexpr int QC = D / 32, VC = D / 64, ST = SPARSE_STAGES, HALF = 16 * 128, TILE = 2 * VC * HALF;
+    constexpr int WARPS = sparse_warps(true);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, G = a.G, bs = c.block_size;
     uint2 qa[QC][2], qb[QC][2];  // rows g and g + 8
 #pragma unroll
@@ -832,20 +835,20 @@ __device__ __forceinline__ void attend_mma(const mentat_kv_cache& c, const Spars
         }
     };
 #pragma unroll
-    for (int s = 0; s < ST - 1; ++s) request(warp + s * SPARSE_WARPS, s);
+    for (int s = 0; s < ST - 1; ++s) request(warp + s * WARPS, s);
     int stage = 0, parity = 0;
     // a lane's reads: K rows t', t' + 8 (token of column g), V rows t, t + 4, t + 8, t + 12, chunk of column g
     const int kr = (g >> 1) + 4 * (g & 1), vc = kr;
-    for (int i = warp; i < total; i += SPARSE_WARPS) {
+    for (int i = warp; i < total; i += WARPS) {
         __syncwarp();
-        request(i + (ST - 1) * SPARSE_WARPS, stage == 0 ? ST - 1 : stage - 1);
+        request(i + (ST - 1) * WARPS, stage == 0 ? ST - 1 : stage - 1);
         if (!__all_sync(0xffffffffu, mbar_wait(bar0 + 8 * stage, parity))) {
             if (lane == 0) set_error(c, MENTAT_DEV_DECODE_TIMEOUT, 8);
             // the copies still on the way end before the shared memory is used again or given back
             for (int s = 1; s < ST; ++s) {
                 stage = stage == ST - 1 ? 0 : stage + 1;
                 parity ^= stage == 0;
-                if (i + s * SPARSE_WARPS < total) (void)mbar_wait(bar0 + 8 * stage, parity);
+                if (i + s * WARPS < total) (void)mbar_wait(bar0 + 8 * stage, parity);
             }
             break;
         }
@@ -942,9 +945,10 @@ __device__ __forceinline__ void attend_mma(const mentat_kv_cache& c, const Spars
 
 // LISTED: the choice was made before (k_score, k_choose); only the attention is left.
 template <typename T, int D, int GM, bool MMA, bool LISTED>
-__global__ void __launch_bounds__(SPARSE_THREADS) k_sparse(const __grid_constant__ CUtensorMap mk,
+__global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_constant__ CUtensorMap mk,
                                                            const __grid_constant__ CUtensorMap mv, mentat_kv_cache c,
                                                            mentat_page_index x, SparseArgs a) {
+    constexpr int SPARSE_WARPS = sparse_warps(MMA), SPARSE_THREADS = 32 * SPARSE_WARPS;
     extern __shared__ int smem_raw[];
     int* smem = smem_raw + (((smem_u32(smem_raw) + 1023) & ~1023u) - smem_u32(smem_raw)) / 4;
     __shared__ uint64_t bars[SPARSE_WARPS * SPARSE_STAGES];
@@ -996,7 +1000,7 @@ __global__ void __launch_bounds__(SPARSE_THREADS) k_sparse(const __grid_constant
             quantise<T, D>(q + g * D, g < G, q8 + 2 * g * D, s_unit + g);
         __syncthreads();
         const int each = (P + cs - 1) / cs, p0 = min(P, rank * each), p1 = min(P, p0 + each);
-        score_pages<D, GM>(c, x, a, h, row, P, p0, p1, q8, s_unit, keys);
+        score_pages<D, GM, SPARSE_WARPS>(c, x, a, h, row, P, p0, p1, q8, s_unit, keys);
         if (cs > 1) cluster.sync(); else __syncthreads();
         choose<SPARSE_THREADS>(keys, P, k, i0, i0 + count, pages, s_choose);
     }
@@ -1018,7 +1022,7 @@ __global__ void __launch_bounds__(SPARSE_THREADS) k_sparse(const __grid_constant
         attend_mma<T, D, GM>(c, a, &mk, &mv, h, len, pages, blocks, count, q, reinterpret_cast<uint8_t*>(smem), bars, pm,
                              pl, po);
     else
-        attend_simple<T, D, GM>(c, a, h, len, pages, blocks, count, qf, pm, pl, po);
+        attend_simple<T, D, GM, SPARSE_WARPS>(c, a, h, len, pages, blocks, count, qf, pm, pl, po);
     __syncthreads();
     // the warps' partials into the first one's place
     for (int i = tid; i < G * D; i += SPARSE_THREADS) {
@@ -1404,7 +1408,7 @@ static int launch_sparse(const mentat_kv_cache* c, const mentat_page_index* x, S
     const size_t smem = 4 * (size_t)sparse_smem(a.G, GM, D, MMA, LISTED, a.held, a.share).total + 1024;
     CUtensorMap mk{}, mv{};
     if (MMA && !pool_maps(c, a.layer, &mk, &mv)) return MENTAT_ERR_CUDA;
-    return launch_cluster(k_sparse<T, D, GM, MMA, LISTED>, cs, dim3(c->num_kv_heads * cs, a.n), SPARSE_THREADS, smem, s,
+    return launch_cluster(k_sparse<T, D, GM, MMA, LISTED>, cs, dim3(c->num_kv_heads * cs, a.n), 32 * sparse_warps(MMA), smem, s,
                           mk, mv, *c, *x, a);
 }
 

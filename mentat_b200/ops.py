@@ -535,7 +535,8 @@ def page_bounds(index, layer: int, blocks: torch.Tensor) -> tuple:
     c = index.cache
     blocks = _check_ids("blocks", blocks, c.device)
     n, h, d = blocks.shape[0], c.num_key_value_heads, c.head_dim
-    low, high = torch.empty((n, h, d), device=c.device), torch.empty((n, h, d), device=c.device)
+    low = torch.empty((n, h, d), dtype=torch.float32, device=c.device)
+    high = torch.empty_like(low)
     exps = torch.empty((n, h), dtype=torch.int8, device=c.device)
     _call(c.device, "mentat_page_bounds", c._desc_ptr, layer, blocks.data_ptr(), n, index._ptr,
           low.data_ptr(), high.data_ptr(), exps.data_ptr())
