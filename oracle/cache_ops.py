@@ -105,20 +105,15 @@ def index_page(k):
 
 def choose_pages(q, bounds, exps, pages, budget, sink, recent):
     """The pages one KV head attends to: q (G, D) float64, bounds (pages, 2, D), exps (pages,)."""
-    scores = np.zeros(pages)
-    for p in range(pages):
-        if p < sink or p >= pages - recent:
-            scores[p] = np.inf
-        elif exps[p] == 127:
-            scores[p] = 1e300
-        else:
-            best = -np.inf
-            for row in q:
-                row = np.where(np.isfinite(row), row, 0.0)
-                e = unit_exponent(np.abs(row).max())
-                grid = np.clip(np.rint(row / 2.0 ** e), -127, 127) * 2.0 ** e
-                best = max(best, np.maximum(grid * bounds[p, 0], grid * bounds[p, 1]).sum() * 2.0 ** float(exps[p]))
-            scores[p] = best
+    best = np.full(pages, -np.inf)
+    for row in q:
+        row = np.where(np.isfinite(row), row, 0.0)
+        e = unit_exponent(np.abs(row).max())
+        grid = np.clip(np.rint(row / 2.0 ** e), -127, 127) * 2.0 ** e
+        products = np.maximum(grid * bounds[:, 0], grid * bounds[:, 1]).sum(1)
+        best = np.maximum(best, products * 2.0 ** np.where(exps == 127, 0, exps).astype(float))
+    p = np.arange(pages)
+    scores = np.where((p < sink) | (p >= pages - recent), np.inf, np.where(exps == 127, 1e300, best))
     order = sorted(range(pages), key=lambda p: (-scores[p], p))
     return sorted(order[:budget])
 

@@ -169,6 +169,65 @@ def test_batches_of_trees():
         run_and_check(c, x, q, tables, lens, 8, 1, 2, "bf16", layer=0)
 
 
+# hq, hkv, d, bs, n, dtype: more heads than CTAs run at once and more than 600 pages, so that scores and choice
+# have launches of their own, for groups of 1 to 16 and with and without tensor cores
+LONG = [(5, 5, 128, 16, 31, "bf16"), (4, 2, 64, 16, 77, "f16"), (12, 4, 128, 32, 38, "bf16"), (25, 5, 64, 16, 31, "f16"),
+        (20, 2, 128, 16, 76, "bf16"), (16, 1, 64, 16, 150, "bf16"), (8, 4, 64, 5, 76, "f32"), (9, 3, 128, 24, 101, "f16")]
+
+
+@pytest.mark.parametrize("case", LONG, ids=lambda c: "-".join(map(str, c)))
+def test_large_batches_of_long_sequences(case):
+    hq, hkv, d, bs, n, dtype = case
+    rng = np.random.default_rng(n)
+    lens = [int(v) for v in rng.integers(580 * bs, 640 * bs, n)]
+    lens[0] = 640 * bs
+    for i in rng.choice(np.arange(1, n), n // 4, replace=False):  # short ones, some without a choice
+        lens[i] = int(rng.integers(0, 40 * bs))
+    lens[2], lens[n - 1] = 0, 639 * bs + 1
+    # a common prefix that ends inside a tile of pages, and its first pages alone
+    for shared, budget, sink, recent in ((585, 37, 1, 2), (21, 600, 0, 1)):
+        c, x, q, tables = make(lens, hq, hkv, d, bs, dtype, layers=1, shared=shared)
+        if budget == 600:  # most of the pages, for sequences in any order and more than once
+            some = rng.choice(n, 310 // hkv, replace=True)
+            run_and_check(c, x, q[torch.from_numpy(some).cuda()], tables, lens, budget, sink, recent, dtype, layer=0,
+                          slots=[int(i) for i in some])
+        else:
+            run_and_check(c, x, q, tables, lens, budget, sink, recent, dtype, layer=0)
+
+
+def test_large_batches_record_bad_state():
+    """The same with a table entry outside the pool, a bad slot and a row longer than max_len: recorded, not
+    read, and the other rows come out as before."""
+    from mentat_b200 import ops
+    n, lens = 80, [610 * 16] * 80
+    c, x, q, tables = make(lens, 4, 2, 64, 16, "bf16", layers=1, shared=600)
+    every = torch.arange(n, dtype=torch.int32, device="cuda")
+    want = ops.sparse_decode(x, 0, every, q, 610 * 16, 12)
+    c.check()
+    slots = every.clone()
+    slots[7] = n + 5
+    got = ops.sparse_decode(x, 0, slots, q, 610 * 16, 12)
+    with pytest.raises(ValueError, match="slot"):
+        c.check()
+    c._tensors["ctrl"].zero_()
+    rest = [i for i in range(n) if i != 7]
+    assert torch.equal(got[rest], want[rest]) and not got[7].any()
+    got = ops.sparse_decode(x, 0, every, q, 610 * 16 - 1, 12)
+    with pytest.raises(RuntimeError, match="overflow"):
+        c.check()
+    c._tensors["ctrl"].zero_()
+    assert not got.any()
+    for page in (300, 605):                                  # among the shared ones, and a sequence's own
+        c._tensors["tables"][0, 11, page] = c.max_blocks
+        got = ops.sparse_decode(x, 0, every, q, 610 * 16, 12)
+        with pytest.raises(AssertionError):
+            c.check()
+        c._tensors["ctrl"].zero_()
+        rest = [i for i in range(n) if i != 11]
+        assert torch.equal(got[rest], want[rest])
+        c._tensors["tables"][0, 11, page] = int(tables[0, 11, page])
+
+
 def test_ties_go_to_the_lowest_page():
     from mentat_b200 import ops
     lens = [2000]
