@@ -310,14 +310,13 @@ struct SparseArgs {
 struct SparseSmem {
     int po, q8, keys, qf, ml, pages, blocks, total;
 };
-__host__ __device__ inline SparseSmem sparse_smem(int G, int GM, int D, bool mma, bool listed, int pages,
-                                                  int share) {
+__host__ __device__ inline SparseSmem sparse_smem(int G, int GM, int D, bool mma, int pages, int share) {
     SparseSmem s;
     share = (share + 3) / 4 * 4;
     const int warps = sparse_warps(mma), attend = mma ? warps * SPARSE_STAGES * 16 * D : 0, partials = warps * G * D;
     s.po = s.q8 = 0;
     s.keys = (GM < 8 ? 8 : GM) * 2 * D / 4;
-    const int chose = listed ? 0 : s.keys + (pages + 3 + 3) / 4 * 4;
+    const int chose = pages ? s.keys + (pages + 3 + 3) / 4 * 4 : 0;
     s.qf = attend > partials ? attend : partials;
     if (chose > s.qf) s.qf = chose;
     s.ml = s.qf + (mma ? 0 : G * D);
@@ -943,8 +942,8 @@ __device__ __forceinline__ void attend_mma(const mentat_kv_cache& c, const Spars
     }
 }
 
-// LISTED: the choice was made before (k_score, k_choose); only the attention is left.
-template <typename T, int D, int GM, bool MMA, bool LISTED>
+// The scores may have been made before (a.keys), and the choice too (a.list).
+template <typename T, int D, int GM, bool MMA>
 __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_constant__ CUtensorMap mk,
                                                            const __grid_constant__ CUtensorMap mv, mentat_kv_cache c,
                                                            mentat_page_index x, SparseArgs a) {
@@ -957,7 +956,7 @@ __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, cs = cluster.num_blocks(), rank = cluster.block_rank();
     const int n = blockIdx.y, h = blockIdx.x / cs, G = a.G, H = c.num_kv_heads, bs = c.block_size;
-    const SparseSmem at = sparse_smem(G, GM, D, MMA, LISTED, a.held, a.share);
+    const SparseSmem at = sparse_smem(G, GM, D, MMA, a.held, a.share);
     float* pm = reinterpret_cast<float*>(smem + at.ml);
     float* pl = pm + SPARSE_WARPS * GM;
     float* po = reinterpret_cast<float*>(smem + at.po);
@@ -970,7 +969,8 @@ __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_
         for (int i = 0; i < SPARSE_WARPS * SPARSE_STAGES; ++i) mbar_init(smem_u32(bars + i), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (!LISTED && cs > 1) cluster.barrier_arrive();  // this CTA runs: its shared memory may be written
+    const bool spread = cs > 1 && !a.keys;
+    if (spread) cluster.barrier_arrive();  // this CTA runs: its shared memory may be written
     griddep_wait();
     griddep_launch();
 
@@ -985,7 +985,7 @@ __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_
     }
     int P = (len + bs - 1) / bs;
     if (len > a.max_len || P > c.max_blocks_per_seq) {
-        if (!LISTED && tid == 0) set_error(c, MENTAT_DEV_PLAN_OVERFLOW, slot);
+        if (tid == 0) set_error(c, MENTAT_DEV_PLAN_OVERFLOW, slot);
         P = 0;
     }
     const int32_t* row = P ? table_row(c, a.layer, slot) : nullptr;
@@ -994,20 +994,25 @@ __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_
         for (int i = tid; i < G * D; i += SPARSE_THREADS) qf[i] = Elem<T>::to_f(q[i]);
 
     const int i0 = (int)((int64_t)rank * k / cs), count = (int)((int64_t)(rank + 1) * k / cs) - i0;
-    if (!LISTED && cs > 1) cluster.barrier_wait();
-    if (!LISTED && P > k) {  // every CTA of the cluster alike
-        for (int g = warp; g < (GM < 8 ? 8 : GM); g += SPARSE_WARPS)
-            quantise<T, D>(q + g * D, g < G, q8 + 2 * g * D, s_unit + g);
-        __syncthreads();
-        const int each = (P + cs - 1) / cs, p0 = min(P, rank * each), p1 = min(P, p0 + each);
-        score_pages<D, GM, SPARSE_WARPS>(c, x, a, h, row, P, p0, p1, q8, s_unit, keys);
-        if (cs > 1) cluster.sync(); else __syncthreads();
+    if (spread) cluster.barrier_wait();
+    if (!a.list && P > k) {  // every CTA of the cluster alike
+        if (a.keys) {
+            const uint4* from = reinterpret_cast<const uint4*>(a.keys + ((int64_t)n * H + h) * a.key_stride);
+            for (int p = tid; p < (P + 3) / 4; p += SPARSE_THREADS) reinterpret_cast<uint4*>(keys)[p] = from[p];
+        } else {
+            for (int g = warp; g < (GM < 8 ? 8 : GM); g += SPARSE_WARPS)
+                quantise<T, D>(q + g * D, g < G, q8 + 2 * g * D, s_unit + g);
+            __syncthreads();
+            const int each = (P + cs - 1) / cs, p0 = min(P, rank * each), p1 = min(P, p0 + each);
+            score_pages<D, GM, SPARSE_WARPS>(c, x, a, h, row, P, p0, p1, q8, s_unit, keys);
+        }
+        if (spread) cluster.sync(); else __syncthreads();
         choose<SPARSE_THREADS>(keys, P, k, i0, i0 + count, pages, s_choose);
     }
     // this CTA's share of the chosen pages, and their blocks
-    int32_t* told = !LISTED && a.pages ? a.pages + ((int64_t)n * H + h) * a.budget : nullptr;
+    int32_t* told = !a.list && a.pages ? a.pages + ((int64_t)n * H + h) * a.budget : nullptr;
     for (int i = tid; i < count; i += SPARSE_THREADS) {
-        const int p = LISTED ? a.list[((int64_t)n * H + h) * a.budget + i0 + i] : P > k ? pages[i] : i0 + i, b = row[p];
+        const int p = a.list ? a.list[((int64_t)n * H + h) * a.budget + i0 + i] : P > k ? pages[i] : i0 + i, b = row[p];
         const bool ok = (unsigned)b < (unsigned)c.num_blocks;
         if (!ok) set_error(c, MENTAT_DEV_BAD_BLOCK, b);
         pages[i] = p;
@@ -1016,7 +1021,7 @@ __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_
     }
     if (told && rank == 0)
         for (int i = k + tid; i < a.budget; i += SPARSE_THREADS) told[i] = -1;
-    if (MMA && !LISTED) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // keys, then TMA, in one place
+    if (MMA) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // keys, then TMA, in one place
     __syncthreads();
     if constexpr (MMA)
         attend_mma<T, D, GM>(c, a, &mk, &mv, h, len, pages, blocks, count, q, reinterpret_cast<uint8_t*>(smem), bars, pm,
@@ -1071,9 +1076,11 @@ __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_
 // of them at once: the query heads of up to 16 sequences are the columns of the product (GP columns each,
 // the group rounded up to a power of two; the columns past the group have no part; at most 64 columns), and
 // where all of them have the same 16 blocks the bounds are read once.  Two warps take 16 pages, half of the
-// columns each, or, where the pages are not shared, every second sequence each; a warp has the next pages'
-// bounds and the blocks of those after them on the way while it works.
-constexpr int SCORE_THREADS = 256, SCORE_TILES = SCORE_THREADS / 64;  // tiles of 16 pages at a time
+// columns each.  Pages that are not shared are put aside, and then shared out by sequence among all warps of the
+// CTA.  A warp has the next pages' bounds and the blocks of those after them on the way while it works.
+constexpr int SCORE_THREADS = 256, SCORE_WARPS = SCORE_THREADS / 32;
+constexpr int SCORE_TILES = SCORE_WARPS / 2;  // tiles of 16 pages at a time
+constexpr int SCORE_ASIDE = 1024;             // tiles between two looks at those put aside
 
 // The query heads in 8 bits, [n][Hq][2 D], negative part and positive part, and their units.
 template <typename T, int D>
@@ -1116,6 +1123,7 @@ __global__ void __launch_bounds__(SCORE_THREADS, 2) k_score(mentat_kv_cache c, m
     __shared__ __align__(8) float s_unit[COLS];
     __shared__ int s_pages[ROWS];
     __shared__ const int32_t* s_row[ROWS];
+    __shared__ int s_aside[SCORE_ASIDE], s_count;
     griddep_wait();
     griddep_launch();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -1215,34 +1223,45 @@ __global__ void __launch_bounds__(SCORE_THREADS, 2) k_score(mentat_kv_cache c, m
     auto unit_of = [&](int nt) { return *reinterpret_cast<const float2*>(s_unit + nt * 8 + 2 * t); };
     const uint8_t* cols = smem_q + g * QS + t * 16;
 
-    int id[IDS], now[IDS], first, ek[2];  // now: the blocks of the tile in hand, if it is not shared
-    int4 v[2][CH];
-    int tl = tile0;
-    bool shared = false;
-    if (tl < tiles) {
-        fetch(tl, id);
-        shared = common(id, first);
-        if (shared) load(__shfl_sync(0xffffffffu, first, g), __shfl_sync(0xffffffffu, first, 8 + g), v, ek);
+    // the next piece of work's bounds, and the blocks of the one after it, are on the way
+    int4 v[2][CH], nv[2][CH];
+    int ek[2], nek[2];
+    auto advance = [&] {
 #pragma unroll
-        for (int e = 0; e < IDS; ++e) now[e] = id[e];
-        if (tl + step < tiles) fetch(tl + step, id);
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();
-    for (; tl < tiles; tl += step) {
-        // the next tile's bounds, and the blocks of the one after it
-        int4 nv[2][CH];
-        int nek[2] = {0, 0}, nid[IDS];
-        bool next_shared = false;
-        if (tl + step < tiles) {
-            next_shared = common(id, first);
-            if (next_shared) load(__shfl_sync(0xffffffffu, first, g), __shfl_sync(0xffffffffu, first, 8 + g), nv, nek);
+        for (int r = 0; r < 2; ++r) {
+            ek[r] = nek[r];
 #pragma unroll
-            for (int e = 0; e < IDS; ++e) nid[e] = id[e];
-            if (tl + 2 * step < tiles) fetch(tl + 2 * step, id);
+            for (int ch = 0; ch < CH; ++ch) v[r][ch] = nv[r][ch];
         }
-        const int pt = tl * 16;
-        if (shared) {
+    };
+    for (int t0 = 0; t0 < tiles; t0 += step * (SCORE_ASIDE / SCORE_TILES)) {
+        const int t1 = min(tiles, t0 + step * (SCORE_ASIDE / SCORE_TILES));
+        if (t0 > 0) __syncthreads();
+        if (tid == 0) s_count = 0;
+        int id[IDS], first, tl = t0 + tile0;
+        bool shared = false;
+        auto look = [&] {
+            shared = common(id, first);
+            if (shared) load(__shfl_sync(0xffffffffu, first, g), __shfl_sync(0xffffffffu, first, 8 + g), nv, nek);
+        };
+        if (tl < t1) {
+            fetch(tl, id);
+            look();
+            if (tl + step < t1) fetch(tl + step, id);
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+        for (; tl < t1; tl += step) {
+            const bool now = shared;
+            advance();
+            if (tl + step < t1) {
+                look();
+                if (tl + 2 * step < t1) fetch(tl + 2 * step, id);
+            }
+            if (!now) {
+                if (half == 0 && lane == 0) s_aside[atomicAdd(&s_count, 1)] = tl;
+                continue;
+            }
             int d[HALF][4];
             const int nt0 = half * HALF;
             score_product<D, HALF>(v, cols + nt0 * 8 * QS, d);
@@ -1252,7 +1271,7 @@ __global__ void __launch_bounds__(SCORE_THREADS, 2) k_score(mentat_kv_cache c, m
                 const float2 u = unit_of(nt);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const int pp = pt + r * 8 + g;
+                    const int pp = tl * 16 + r * 8 + g;
                     if (GP == 1) {  // each column is a sequence
                         put(nt * 8 + 2 * t, pp, (float)d[k][2 * r] * u.x, ek[r]);
                         put(nt * 8 + 2 * t + 1, pp, (float)d[k][2 * r + 1] * u.y, ek[r]);
@@ -1265,68 +1284,68 @@ __global__ void __launch_bounds__(SCORE_THREADS, 2) k_score(mentat_kv_cache c, m
                     }
                 }
             }
-        } else {
-            // sequence 2 e + half's blocks are in the lanes from 16 half; the next sequence's bounds are on the
-            // way while one is scored
-            constexpr int N1 = GP > 8 ? 2 : 1;
-            auto load_one = [&](int e, int4 (&v)[2][CH], int (&ek)[2]) {
-                int b[2];
+        }
+        __syncthreads();
+        // (tile, sequence) by warp
+        const int units = s_count * ROWS;
+        int b[2];
+        auto blocks_of = [&](int u) {
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    b[r] = __shfl_sync(0xffffffffu, now[e], 16 * half + 8 * r + g);
-                    if (b[r] != NONE && (unsigned)b[r] >= (unsigned)c.num_blocks) {
-                        if (t == 0) set_error(c, MENTAT_DEV_BAD_BLOCK, b[r]);
-                        b[r] = -1;
-                    }
+            for (int r = 0; r < 2; ++r) {
+                const int i = u % ROWS, pp = u < units ? s_aside[u / ROWS] * 16 + r * 8 + g : 0;
+                b[r] = u < units && pp < s_pages[i] ? s_row[i][pp] : NONE;
+            }
+        };
+        auto load_blocks = [&] {
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+                if (b[r] != NONE && (unsigned)b[r] >= (unsigned)c.num_blocks) {
+                    if (t == 0) set_error(c, MENTAT_DEV_BAD_BLOCK, b[r]);
+                    b[r] = -1;
                 }
-                load(b[0], b[1], v, ek);
-            };
-            load_one(0, v, ek);
+            load(b[0], b[1], nv, nek);
+        };
+        if (warp < units) {
+            blocks_of(warp);
+            load_blocks();
+            blocks_of(warp + SCORE_WARPS);
+        }
+        constexpr int N1 = GP > 8 ? 2 : 1;
+        for (int u = warp; u < units; u += SCORE_WARPS) {
+            advance();
+            if (u + SCORE_WARPS < units) {
+                load_blocks();
+                blocks_of(u + 2 * SCORE_WARPS);
+            }
+            const int i = u % ROWS, nt = i * GP / 8, col = i * GP % 8;  // its first column in its tile
+            int d[N1][4];
+            score_product<D, N1>(v, cols + nt * 8 * QS, d);
+            const float2 un = unit_of(nt);
 #pragma unroll
-            for (int e = 0; e < IDS; ++e) {
-                const int i = 2 * e + half, nt = i * GP / 8, col = i * GP % 8;  // its first column in its tile
-                const int ex[2] = {ek[0], ek[1]};
-                int d[N1][4];
-                score_product<D, N1>(v, cols + nt * 8 * QS, d);
-                if (e + 1 < IDS) load_one(e + 1 < IDS ? e + 1 : 0, v, ek);
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int pp = pt + r * 8 + g;
-                    const float2 u = unit_of(nt);
-                    if (GP == 1) {
-                        if (t == col / 2) put(i, pp, (float)d[0][2 * r + (col & 1)] * (col & 1 ? u.y : u.x), ex[r]);
-                    } else {
-                        float best = highest(d[0], u, r);
-                        if (GP > 8) best = fmaxf(best, highest(d[N1 - 1], unit_of(nt + N1 - 1), r));
-                        if (t == col / 2) put(i, pp, best, ex[r]);
-                    }
+            for (int r = 0; r < 2; ++r) {
+                const int pp = s_aside[u / ROWS] * 16 + r * 8 + g;
+                if (GP == 1) {
+                    if (t == col / 2) put(i, pp, (float)d[0][2 * r + (col & 1)] * (col & 1 ? un.y : un.x), ek[r]);
+                } else {
+                    float best = highest(d[0], un, r);
+                    if (GP > 8) best = fmaxf(best, highest(d[N1 - 1], unit_of(nt + N1 - 1), r));
+                    if (t == col / 2) put(i, pp, best, ek[r]);
                 }
             }
-        }
-        shared = next_shared;
-#pragma unroll
-        for (int e = 0; e < IDS; ++e) now[e] = nid[e];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            ek[r] = nek[r];
-#pragma unroll
-            for (int ch = 0; ch < CH; ++ch) v[r][ch] = nv[r][ch];
         }
     }
 }
 
-// The chosen pages from the keys: one CTA per (sequence, KV head), or a cluster where a sequence may have
-// more than HELD_PAGES pages.
+// The chosen pages from the keys where a sequence may have more than HELD_PAGES pages: a cluster per (sequence,
+// KV head).
 constexpr int CHOOSE_THREADS = 256, HELD_PAGES = 16384;
-template <bool CL>
 __global__ void __launch_bounds__(CHOOSE_THREADS) k_choose(mentat_kv_cache c, SparseArgs a) {
     extern __shared__ __align__(16) uint32_t keys[];
-    __shared__ int smem32[CL ? 32 : 1], counts[CL ? 4 * 256 : 1];
-    __shared__ Chooser s_choose;
+    __shared__ int smem32[32], counts[4 * 256];
     griddep_wait();
     griddep_launch();
     cg::cluster_group cluster = cg::this_cluster();
-    const int cs = CL ? cluster.num_blocks() : 1, rank = CL ? cluster.block_rank() : 0;
+    const int cs = cluster.num_blocks(), rank = cluster.block_rank();
     const int tid = threadIdx.x, n = blockIdx.y, h = blockIdx.x / cs, H = c.num_kv_heads, bs = c.block_size;
     const int slot = a.slots[n];
     int len = slot >= 0 && slot < c.max_seqs ? c.ntok[seq_index(c, a.layer, slot)] : 0;
@@ -1343,10 +1362,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) k_choose(mentat_kv_cache c, Sp
     const uint32_t* from = a.keys + ((int64_t)n * H + h) * a.key_stride;
     for (int p = p0 + tid; p < p1; p += CHOOSE_THREADS) keys[p - p0] = from[p];
     __syncthreads();
-    if constexpr (CL)
-        choose_cluster<CHOOSE_THREADS>(keys, p0, p1 - p0, k, counts, list, smem32);
-    else
-        choose<CHOOSE_THREADS>(keys, P, k, 0, k, list, s_choose);
+    choose_cluster<CHOOSE_THREADS>(keys, p0, p1 - p0, k, counts, list, smem32);
 }
 
 // ---------------------------------------------------------------------------
@@ -1400,35 +1416,35 @@ static int launch_cluster(void (*kernel)(KArgs...), int cs, dim3 grid, int threa
     return MENTAT_OK;
 }
 
-template <typename T, int D, int GM, bool MMA, bool LISTED>
+template <typename T, int D, int GM, bool MMA>
 static int launch_sparse(const mentat_kv_cache* c, const mentat_page_index* x, SparseArgs a, cudaStream_t s) {
     const int pages = (a.max_len + c->block_size - 1) / c->block_size, cs = sparse_cluster(a.n * c->num_kv_heads, MMA);
-    a.held = pages;
+    a.held = pages <= a.budget || a.list ? 0 : pages;
     a.share = (min(pages, a.budget) + cs - 1) / cs;
-    const size_t smem = 4 * (size_t)sparse_smem(a.G, GM, D, MMA, LISTED, a.held, a.share).total + 1024;
+    const size_t smem = 4 * (size_t)sparse_smem(a.G, GM, D, MMA, a.held, a.share).total + 1024;
     CUtensorMap mk{}, mv{};
     if (MMA && !pool_maps(c, a.layer, &mk, &mv)) return MENTAT_ERR_CUDA;
-    return launch_cluster(k_sparse<T, D, GM, MMA, LISTED>, cs, dim3(c->num_kv_heads * cs, a.n), 32 * sparse_warps(MMA), smem, s,
+    return launch_cluster(k_sparse<T, D, GM, MMA>, cs, dim3(c->num_kv_heads * cs, a.n), 32 * sparse_warps(MMA), smem, s,
                           mk, mv, *c, *x, a);
 }
 
 // 16-bit types with pages of 16 rows or a multiple run on tensor cores
-template <typename T, int D, int GM, bool LISTED>
+template <typename T, int D, int GM>
 static int launch_sparse_kind(const mentat_kv_cache* c, const mentat_page_index* x, const SparseArgs& a,
                               cudaStream_t s) {
     if constexpr (sizeof(T) == 2)
         if (sparse_mma(c) && a.qs % 4 == 0 && (uintptr_t)a.q % 8 == 0)
-            return launch_sparse<T, D, (GM > 8 ? 16 : 8), true, LISTED>(c, x, a, s);
-    return launch_sparse<T, D, GM, false, LISTED>(c, x, a, s);
+            return launch_sparse<T, D, (GM > 8 ? 16 : 8), true>(c, x, a, s);
+    return launch_sparse<T, D, GM, false>(c, x, a, s);
 }
 
-template <typename T, int D, bool LISTED>
+template <typename T, int D>
 static int launch_sparse_group(const mentat_kv_cache* c, const mentat_page_index* x, const SparseArgs& a,
                                cudaStream_t s) {
-    if (a.G <= 2) return launch_sparse_kind<T, D, 2, LISTED>(c, x, a, s);
-    if (a.G <= 4) return launch_sparse_kind<T, D, 4, LISTED>(c, x, a, s);
-    if (a.G <= 8) return launch_sparse_kind<T, D, 8, LISTED>(c, x, a, s);
-    return launch_sparse_kind<T, D, 16, LISTED>(c, x, a, s);
+    if (a.G <= 2) return launch_sparse_kind<T, D, 2>(c, x, a, s);
+    if (a.G <= 4) return launch_sparse_kind<T, D, 4>(c, x, a, s);
+    if (a.G <= 8) return launch_sparse_kind<T, D, 8>(c, x, a, s);
+    return launch_sparse_kind<T, D, 16>(c, x, a, s);
 }
 
 template <int D, int GP>
@@ -1446,7 +1462,7 @@ static int launch_score(const mentat_kv_cache* c, const mentat_page_index* x, co
 template <typename T, int D>
 static int launch_sparse_dim(const mentat_kv_cache* c, const mentat_page_index* x, const SparseArgs& a,
                              cudaStream_t s) {
-    if (!a.keys) return launch_sparse_group<T, D, false>(c, x, a, s);
+    if (!a.keys) return launch_sparse_group<T, D>(c, x, a, s);
     const int heads = a.n * a.G * c->num_kv_heads;
     MENTAT_LAUNCH(k_score_queries<T, D>, dim3((heads + 3) / 4), dim3(128), 0, s, (const T*)a.q, a.qs, heads,
                   a.G * c->num_kv_heads, a.q8, a.units);
@@ -1457,14 +1473,15 @@ static int launch_sparse_dim(const mentat_kv_cache* c, const mentat_page_index* 
     else if (a.G <= 8) sc = launch_score<D, 8>(c, x, a, s);
     else sc = launch_score<D, 16>(c, x, a, s);
     if (sc != MENTAT_OK) return sc;
-    const int pages = (a.max_len + c->block_size - 1) / c->block_size;
-    int cs = 1;
-    while (cs < SPARSE_MAX_CLUSTER && (pages + cs - 1) / cs > HELD_PAGES) cs *= 2;
-    const size_t smem = 4 * (size_t)((pages + cs - 1) / cs + 3);
-    const int st = launch_cluster(cs > 1 ? k_choose<true> : k_choose<false>, cs, dim3(c->num_kv_heads * cs, a.n),
-                                  CHOOSE_THREADS, smem, s, *c, a);
-    if (st != MENTAT_OK) return st;
-    return launch_sparse_group<T, D, true>(c, x, a, s);
+    if (a.list) {
+        const int pages = (a.max_len + c->block_size - 1) / c->block_size;
+        int cs = 2;
+        while (cs < SPARSE_MAX_CLUSTER && (pages + cs - 1) / cs > HELD_PAGES) cs *= 2;
+        const size_t smem = 4 * (size_t)((pages + cs - 1) / cs + 3);
+        const int st = launch_cluster(k_choose, cs, dim3(c->num_kv_heads * cs, a.n), CHOOSE_THREADS, smem, s, *c, a);
+        if (st != MENTAT_OK) return st;
+    }
+    return launch_sparse_group<T, D>(c, x, a, s);
 }
 
 }  // namespace mentat
@@ -1561,7 +1578,8 @@ int mentat_sparse_decode(const mentat_kv_cache* c, int32_t layer, const mentat_p
         a.q8 = reinterpret_cast<int8_t*>(next);
         next += (int64_t)n * Hq * c->head_dim / 2;
         a.units = reinterpret_cast<float*>(next);
-        a.list = pages ? pages : reinterpret_cast<int32_t*>(next + (int64_t)n * Hq);
+        if (max_len > (int64_t)HELD_PAGES * c->block_size)
+            a.list = pages ? pages : reinterpret_cast<int32_t*>(next + (int64_t)n * Hq);
     }
     int st = MENTAT_OK;
     if (c->head_dim == 128) {
