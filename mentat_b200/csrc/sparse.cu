@@ -113,7 +113,8 @@ template <> struct Extreme<__half> {
 
 // The index of all heads of one block by one CTA, 16 bytes of a row to a thread (head_dim / VEC threads to a
 // head, a power of two within a warp, every thread of which takes part); the page is read once, 8 rows of a
-// thread on the way at a time.  Bound by memory.
+// thread on the way at a time.  Bound by memory: 8,192 pages of 16 x 8 heads of 128 (285 MB) in 55 us, 5.2 TB/s (15
+// rows at a time 58; a ring of bulk copies in one CTA on an SM 61).
 template <typename T>
 __device__ __forceinline__ void index_block(const mentat_kv_cache& c, int layer, int b, const mentat_page_index& x) {
     using E = Extreme<T>;
@@ -219,7 +220,8 @@ __global__ void k_index_seqs(mentat_kv_cache c, int layer0, const int32_t* slots
     else index_page<T>(c, layer, b, blockIdx.y, x);
 }
 
-// Four pages to a CTA, each thread one piece of each of them on the way.
+// Four pages to a CTA, each thread one piece of each of them on the way.  Bound by the stores: 8,192 pages of 8 heads
+// of 128 (84 MB) take 15 us, with stores that stay in L2 22.
 constexpr int BOUNDS_PAGES = 4;
 __global__ void __launch_bounds__(256) k_page_bounds(mentat_kv_cache c, int layer, const int32_t* blocks, int n,
                                                      mentat_page_index x, float* low, float* high, int8_t* exps) {
@@ -252,10 +254,10 @@ __global__ void __launch_bounds__(256) k_page_bounds(mentat_kv_cache c, int laye
 #pragma unroll
             for (int k = 0; k < BOUNDS_PAGES; ++k)
                 if (at[k] >= 0)
-                    *reinterpret_cast<float4*>((top ? high : low) + (to + (int64_t)k * H + h) * D + d) =
-                        e[k] == EXP_ALL ? make_float4(inf, inf, inf, inf)
-                                        : make_float4(value(v[k].x, e[k]), value(v[k].y, e[k]), value(v[k].z, e[k]),
-                                                      value(v[k].w, e[k]));
+                    __stcs(reinterpret_cast<float4*>((top ? high : low) + (to + (int64_t)k * H + h) * D + d),
+                           e[k] == EXP_ALL ? make_float4(inf, inf, inf, inf)
+                                           : make_float4(value(v[k].x, e[k]), value(v[k].y, e[k]), value(v[k].z, e[k]),
+                                                         value(v[k].w, e[k])));
         }
     } else {
         for (int u = threadIdx.x; u < BOUNDS_PAGES * H * D; u += blockDim.x) {
