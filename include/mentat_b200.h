@@ -373,12 +373,13 @@ int mentat_kv_append_rotated(const mentat_kv_cache* c, int32_t layer, int32_t sl
  */
 /* fork_sequence (paged_kv_cache.py:152-170) of parents[i] into children[i].
  * The children are distinct and none is also a parent; a parent may have
- * several.  max_nblocks is the longest parent's table (a launch-size hint). */
+ * several. */
 int mentat_kv_fork_batched(const mentat_kv_cache* c, const int32_t* parents, const int32_t* children, int32_t n,
-                           int32_t max_nblocks, cudaStream_t s);
+                           cudaStream_t s);
 
 /* free_sequence (paged_kv_cache.py:172-176) of distinct slots, with the state
  * that freeing them one after another leaves, the free list's order included.
+ * max_nblocks is the longest table (a launch-size hint: any value is right).
  * workspace: mentat_pages_workspace_bytes(c, n) bytes, 16-byte aligned. */
 int64_t mentat_pages_workspace_bytes(const mentat_kv_cache* c, int32_t n);
 int mentat_kv_free_batched(const mentat_kv_cache* c, const int32_t* slots, int32_t n, int32_t max_nblocks,
@@ -388,7 +389,8 @@ int mentat_kv_free_batched(const mentat_kv_cache* c, const int32_t* slots, int32
  * paged_kv_cache.py:370-417, keeps a window of one sequence).  Sequence i keeps
  * the positions keep[layer * keep_layer_stride + cu[i] .. cu[i + 1]) of
  * src[i], in that order (any order; a position may repeat), as its positions 0,
- * 1, ...; keep_layer_stride 0 keeps the same ones in every layer.  max_keep is
+ * 1, ...; keep_layer_stride 0 keeps the same ones in every layer.  A layer has
+ * keep_total positions, which no list may pass.  max_keep is
  * the longest list, max_nblocks the longest source table (launch-size hints:
  * larger is safe).  Full pages at the front whose tokens all stay in place (all
  * pages, if the sequence keeps every token) are not copied; the others are written
@@ -400,8 +402,8 @@ int mentat_kv_free_batched(const mentat_kv_cache* c, const int32_t* slots, int32
  * turned from their old position to the new one (scale is not applied again).
  * workspace as above. */
 int mentat_kv_compact(const mentat_kv_cache* c, const int32_t* src, const int32_t* dst, int32_t n,
-                      const int32_t* keep, int64_t keep_layer_stride, const int32_t* cu, int32_t max_keep,
-                      int32_t max_nblocks, const mentat_rotary* r, void* workspace, int64_t workspace_bytes,
+                      const int32_t* keep, int64_t keep_layer_stride, int64_t keep_total, const int32_t* cu,
+                      int32_t max_keep, int32_t max_nblocks, const mentat_rotary* r, void* workspace, int64_t workspace_bytes,
                       cudaStream_t s);
 
 /*

@@ -104,10 +104,10 @@ SIGNATURES = [
     ("mentat_rotary_append", C.c_int, [_KV, _I32, _I32, _P, _ROWS, _ROWS, _ROWS, _ROWS, _P, _ROT, _P]),
     ("mentat_kv_append_rotated_batched", C.c_int, [_KV, _I32, _P, _I32, _ROWS, _ROWS, _ROWS, _ROWS, _P, _ROT, _P]),
     ("mentat_kv_append_rotated", C.c_int, [_KV, _I32, _I32, _I32, _ROWS, _ROWS, _ROWS, _ROWS, _P, _ROT, _P]),
-    ("mentat_kv_fork_batched", C.c_int, [_KV, _P, _P, _I32, _I32, _P]),
+    ("mentat_kv_fork_batched", C.c_int, [_KV, _P, _P, _I32, _P]),
     ("mentat_pages_workspace_bytes", _I64, [_KV, _I32]),
     ("mentat_kv_free_batched", C.c_int, [_KV, _P, _I32, _I32, _P, _I64, _P]),
-    ("mentat_kv_compact", C.c_int, [_KV, _P, _P, _I32, _P, _I64, _P, _I32, _I32, _ROT, _P, _I64, _P]),
+    ("mentat_kv_compact", C.c_int, [_KV, _P, _P, _I32, _P, _I64, _I64, _P, _I32, _I32, _ROT, _P, _I64, _P]),
     ("mentat_page_index_blocks", C.c_int, [_KV, _I32, _P, _I32, _IDX, _P]),
     ("mentat_page_index_seqs", C.c_int, [_KV, _I32, _P, _I32, _I32, _I32, _IDX, _P]),
     ("mentat_page_bounds", C.c_int, [_KV, _I32, _P, _I32, _IDX, _P, _P, _P, _P]),

@@ -433,7 +433,7 @@ struct CompactArgs {
     const int32_t* src;
     const int32_t* dst;  // NULL: in place
     const int32_t* keep;
-    int64_t keep_ls;
+    int64_t keep_ls, total;
     const int32_t* cu;
     int n;
 };
@@ -466,6 +466,14 @@ __global__ void __launch_bounds__(CLUSTER_THREADS) k_compact_plan(mentat_kv_cach
         }
     ok = !__syncthreads_or(no) && ok;
     if (!ok && threadIdx.x == 0) set_error(c, MENTAT_DEV_BAD_SLOT, s_bad);
+    int off = -1;  // a list that does not lie within keep: nothing of it is read
+    for (int i = threadIdx.x; i < a.n; i += CLUSTER_THREADS)
+        if (a.cu[i] < 0 || a.cu[i + 1] < a.cu[i] || a.cu[i + 1] > a.total) off = i;
+    if (off >= 0) s_bad = a.cu[off + 1];
+    if (__syncthreads_or(off >= 0)) {
+        if (ok && threadIdx.x == 0) set_error(c, MENTAT_DEV_BAD_TOKEN, s_bad);
+        ok = false;
+    }
     bool stop = __syncthreads_or(!ok || has_error(c));
     const int rows = a.n * L, per = (rows + CLUSTER_ALL_WARPS - 1) / CLUSTER_ALL_WARPS;
     const int r0 = min(rows, (rank * CLUSTER_WARPS + warp) * per), r1 = min(rows, r0 + per);
@@ -866,6 +874,7 @@ constexpr int FREE_CLUSTER_PER = 4;
 template <bool LEAD>
 static int launch_free(const mentat_kv_cache* c, const int32_t* slots, const int32_t* cu, int32_t n, int32_t max_nb,
                        const PagesWs& w, cudaStream_t s) {
+    if (max_nb > c->max_blocks_per_seq) max_nb = c->max_blocks_per_seq;
     const int rows = n * c->num_layers, chunks = max_nb < 1 ? 1 : (max_nb + 31) / 32;
     const int64_t per = ((int64_t)rows * chunks + CLUSTER_ALL_WARPS - 1) / CLUSTER_ALL_WARPS;
     const size_t held = (size_t)CLUSTER_WARPS * per * 32 * 4;
@@ -933,12 +942,10 @@ int64_t mentat_pages_workspace_bytes(const mentat_kv_cache* c, int32_t n) {
     return bad_pages(c, n) ? 0 : pages_ws(c, n, nullptr, nullptr);
 }
 
-int mentat_kv_fork_batched(const mentat_kv_cache* c, const int32_t* parents, const int32_t* children, int32_t n,
-                           int32_t max_nb, cudaStream_t s) {
-    if (bad_pages(c, n) || max_nb < 0 || (n > 0 && (!parents || !children))) return MENTAT_ERR_ARG;
+int mentat_kv_fork_batched(const mentat_kv_cache* c, const int32_t* parents, const int32_t* children, int32_t n, cudaStream_t s) {
+    if (bad_pages(c, n) || (n > 0 && (!parents || !children))) return MENTAT_ERR_ARG;
     if (n == 0) return MENTAT_OK;
     if (!pages_fit(c, n)) return MENTAT_ERR_UNSUPPORTED;
-    (void)max_nb;
     const dim3 grid((n + PAGES_WARPS - 1) / PAGES_WARPS, c->num_layers);
     MENTAT_LAUNCH(k_fork_batched, grid, dim3(PAGES_THREADS), bitmap_bytes(c), s, *c, parents, children, n);
     return MENTAT_OK;
@@ -955,10 +962,10 @@ int mentat_kv_free_batched(const mentat_kv_cache* c, const int32_t* slots, int32
 }
 
 int mentat_kv_compact(const mentat_kv_cache* c, const int32_t* src, const int32_t* dst, int32_t n, const int32_t* keep,
-                      int64_t keep_ls, const int32_t* cu, int32_t max_keep, int32_t max_nb, const mentat_rotary* r,
-                      void* workspace, int64_t workspace_bytes, cudaStream_t s) {
-    if (bad_pages(c, n) || max_keep < 0 || max_nb < 0 || keep_ls < 0 || c->head_dim <= 0 || c->num_kv_heads <= 0 ||
-        (n > 0 && (!src || !cu || !workspace || ((uintptr_t)workspace & 15) || !c->k_pool || !c->v_pool || (max_keep > 0 && !keep))) ||
+                      int64_t keep_ls, int64_t total, const int32_t* cu, int32_t max_keep, int32_t max_nb,
+                      const mentat_rotary* r, void* workspace, int64_t workspace_bytes, cudaStream_t s) {
+    if (bad_pages(c, n) || max_keep < 0 || max_nb < 0 || keep_ls < 0 || total < 0 || c->head_dim <= 0 || c->num_kv_heads <= 0 ||
+        (n > 0 && (!src || !cu || !workspace || ((uintptr_t)workspace & 15) || !c->k_pool || !c->v_pool || (total > 0 && !keep))) ||
         (r && !rotary_ok(r, c->head_dim)))
         return MENTAT_ERR_ARG;
     if (n == 0) return MENTAT_OK;
@@ -973,7 +980,7 @@ int mentat_kv_compact(const mentat_kv_cache* c, const int32_t* src, const int32_
     }
     const bool wide = c->head_dim % vec == 0 && (!r || rotary_aligned(r, c->head_dim, vec)) &&
                       ((uintptr_t)c->k_pool | (uintptr_t)c->v_pool) % 16 == 0;
-    const CompactArgs a{src, dst, keep, keep_ls, cu, n};
+    const CompactArgs a{src, dst, keep, keep_ls, total, cu, n};
     int st = launch_one_cluster(k_compact_plan, bitmap_bytes(c), s, *c, a, chunks_of(max_keep, PLAN_CHUNK, 1 << 20), w);
     if (st == MENTAT_OK)
         st = rotary_dispatch(c->dtype, wide, turn.interleaved != 0, LaunchCompactMove{*c, a, turn, w, max_keep, s});

@@ -463,23 +463,21 @@ def _workspace(cache, n: int) -> tuple:
 MAX_SEQS_PER_PAGES_CALL = 1024
 
 
-def fork_pages(cache, parents: torch.Tensor, children: torch.Tensor, max_blocks: Optional[int] = None) -> None:
+def fork_pages(cache, parents: torch.Tensor, children: torch.Tensor) -> None:
     """Every layer's table of slot ``parents[i]`` into slot ``children[i]``, with a
     reference on each page (int32 slots on the device; the children distinct, empty
-    and no parents).  ``max_blocks``: the longest parent's table, a launch-size hint.
-    ``PagedKVCacheManager.fork_sequences`` keeps the host's mirror too.  Wraps
+    and no parents).  ``PagedKVCacheManager.fork_sequences`` keeps the host's mirror too.  Wraps
     ``mentat_kv_fork_batched``."""
     dev = cache.device
     parents = _check_ids("parents", parents, dev, limit=MAX_SEQS_PER_PAGES_CALL)
     children = _check_ids("children", children, dev, parents.shape[0])
-    hint = cache.table_capacity if max_blocks is None else max_blocks
-    _call(dev, "mentat_kv_fork_batched", cache._desc_ptr, parents.data_ptr(), children.data_ptr(),
-          parents.shape[0], hint)
+    _call(dev, "mentat_kv_fork_batched", cache._desc_ptr, parents.data_ptr(), children.data_ptr(), parents.shape[0])
 
 
 def free_pages(cache, slots: torch.Tensor, max_blocks: Optional[int] = None) -> None:
     """Releases every page of the (distinct) slots, as freeing them one after another
-    would, the order of the free list included.  Wraps ``mentat_kv_free_batched``."""
+    would, the order of the free list included.  ``max_blocks``: the longest table, a
+    launch-size hint.  Wraps ``mentat_kv_free_batched``."""
     dev = cache.device
     slots = _check_ids("slots", slots, dev, limit=MAX_SEQS_PER_PAGES_CALL)
     hint = cache.table_capacity if max_blocks is None else max_blocks
@@ -514,7 +512,7 @@ def compact_pages(cache, src: torch.Tensor, dst: Optional[torch.Tensor], keep: t
     hint = cache.table_capacity if max_blocks is None else max_blocks
     ws, size = _workspace(cache, n)
     _call(dev, "mentat_kv_compact", cache._desc_ptr, src.data_ptr(),
-          None if dst is None else dst.data_ptr(), n, keep.data_ptr(), keep.stride(0) if per_layer else 0,
+          None if dst is None else dst.data_ptr(), n, keep.data_ptr(), keep.stride(0) if per_layer else 0, keep.shape[-1],
           cu.data_ptr(), max_keep, hint, None if rotary is None else rotary._ptrs[0], ws.data_ptr(), size)
 
 

@@ -469,7 +469,7 @@ class PagedKVCacheManager:
             part = slice(a, a + ops.MAX_SEQS_PER_PAGES_CALL)
             both = self._upload([p.slot for p in parents[part]] + [self._sequences[c].slot for c in kids[part]])
             n = both.numel() // 2
-            ops.fork_pages(self, both[:n], both[n:], max(max(p.num_blocks) for p in parents[part]))
+            ops.fork_pages(self, both[:n], both[n:])
         self._after()
         return kids
 

@@ -150,20 +150,20 @@ def test_c_abi_refuses_page_arguments():
     c = _desc()
     need = lib.mentat_pages_workspace_bytes(c, 4)
     assert need >= 4 * (2 * 64 + 4 * 4 * 2) and lib.mentat_pages_workspace_bytes(c, 1025) == 0
-    assert lib.mentat_kv_fork_batched(c, None, None, 0, 0, None) == 0
-    assert lib.mentat_kv_fork_batched(c, None, 4096, 1, 1, None) == ARG
-    assert lib.mentat_kv_fork_batched(c, 4096, 4096, 1025, 1, None) == ARG
-    assert lib.mentat_kv_fork_batched(_desc(max_seqs=1 << 20), 4096, 4096, 1, 1, None) == UNSUPPORTED
+    assert lib.mentat_kv_fork_batched(c, None, None, 0, None) == 0
+    assert lib.mentat_kv_fork_batched(c, None, 4096, 1, None) == ARG
+    assert lib.mentat_kv_fork_batched(c, 4096, 4096, 1025, None) == ARG
+    assert lib.mentat_kv_fork_batched(_desc(max_seqs=1 << 20), 4096, 4096, 1, None) == UNSUPPORTED
     assert lib.mentat_kv_free_batched(c, None, 0, 0, None, 0, None) == 0
     assert lib.mentat_kv_free_batched(c, 4096, 4, 1, 4096, need - 1, None) == ARG
     assert lib.mentat_kv_free_batched(c, 4096, 4, 1, None, need, None) == ARG
     big = _desc(num_layers=64, max_blocks_per_seq=1 << 20)
     assert lib.mentat_kv_free_batched(big, 4096, 1024, 1, 4096, 1 << 40, None) == UNSUPPORTED
 
-    def compact(c=c, n=4, keep=4096, cu=4096, most=5, rot=None, ws=need, ls=0):
-        return lib.mentat_kv_compact(c, 4096, None, n, keep, ls, cu, most, 3, rot, 4096, ws, None)
+    def compact(c=c, n=4, keep=4096, cu=4096, most=5, rot=None, ws=need, ls=0, total=20):
+        return lib.mentat_kv_compact(c, 4096, None, n, keep, ls, total, cu, most, 3, rot, 4096, ws, None)
     assert compact(n=0) == 0 and compact(n=1025) == ARG and compact(keep=None) == ARG and compact(cu=None) == ARG
-    assert compact(ws=need - 1) == ARG and compact(most=-1) == ARG and compact(ls=-1) == ARG
+    assert compact(ws=need - 1) == ARG and compact(most=-1) == ARG and compact(ls=-1) == ARG and compact(total=-1) == ARG
     assert compact(rot=C.byref(_lib.Rotary(4096, 33, 0, 0, 0, 1.0))) == ARG
 
 

@@ -111,6 +111,69 @@ def test_large_batches_of_shared_pages():
     same(m, o)
 
 
+def test_large_compaction_in_place():
+    """More table entries than one cluster releases; pages at the front shared by all sequences."""
+    rng = np.random.default_rng(11)
+    m, o = pair(L=3, hkv=1, d=2, pool=40000, bs=2, dtype="f32")
+    (root,) = start(m, o, [463], rng, "f32")
+    ids = [root] + m.fork_sequences([root] * 59)
+    for _ in range(59):
+        o.fork_sequence(root)
+    keep = [np.r_[0:100, 100 + np.sort(rng.permutation(363)[: int(rng.integers(0, 363))])] for _ in ids]
+    keep[7], keep[8], keep[9] = np.arange(463), np.arange(0), np.arange(462)
+    m.compact_sequences(ids, keep)
+    compact(o, ids, keep)
+    same(m, o)
+    m.free_sequences(ids)
+    for s in ids:
+        o.free_sequence(s)
+    same(m, o)
+
+
+@pytest.mark.parametrize("dtype,hkv,d,bs", [("f32", 8, 128, 32), ("bf16", 1, 64, 24), ("f16", 16, 256, 16), ("f32", 64, 256, 2),
+                                            ("bf16", 8, 128, 1), ("bf16", 3, 8, 7), ("f16", 1, 8, 40)])
+def test_compaction_of_all_row_sizes(dtype, hkv, d, bs):
+    """Rows of 16 bytes to 64 KB (one token to a stage of the copies, or too long for them), with keys turned too."""
+    from mentat_b200 import Rotary
+    rng = np.random.default_rng(12)
+    m, o = pair(L=1, hkv=hkv, d=d, bs=bs, pool=400, dtype=dtype)
+    ids = start(m, o, [3, 71, 100], rng, dtype)
+    keep = [[2, 0], np.r_[0:2, 30:71], np.sort(rng.permutation(100)[:57])]
+    new = m.compact_sequences(ids, keep, into_new=True)
+    assert new == compact(o, ids, keep, into_new=True)
+    same(m, o)
+    rot = Rotary(d)
+    f, eps = rot.inv_freq.cpu().numpy(), torch.finfo(m.dtype).eps
+    m.compact_sequences(ids, keep, rotary=rot)
+    compact(o, ids, keep, turn_keys=lambda k, shift: turn(k, shift, f))
+    same(m, o, lambda want: 1.5 * turn_tolerance(want, f, eps)(want) + (2.0 ** -25 if dtype == "f16" else 0))
+
+
+def test_sizes_are_only_hints():
+    from mentat_b200 import ops
+    rng = np.random.default_rng(13)
+    m, o = pair(L=2, pool=2000, bs=2)
+    a, b = ids = start(m, o, [431, 700], rng)
+    slots = torch.tensor([m._sequences[s].slot for s in ids], dtype=torch.int32, device="cuda")
+    keep = [np.arange(1, 431, 2), np.arange(700)[::-1][:600]]
+    flat = torch.from_numpy(np.concatenate(keep)).int().cuda()
+    ops.compact_pages(m, slots, None, flat, torch.tensor([0, 215, 815], dtype=torch.int32, device="cuda"), 1, max_blocks=1)
+    compact(o, ids, keep)
+    for layer in range(2):
+        for s in ids:
+            st, w = m._sequences[s], o._sequences[s]
+            st.num_tokens[layer], st.num_blocks[layer] = w.num_tokens[layer], len(w.page_table[layer])
+            st.tokens_in_last_block[layer] = w.tokens_in_last_block[layer]
+    same(m, o)
+    for hint in (0, 1 << 30):
+        (c,) = m.fork_sequences([a])
+        assert c == o.fork_sequence(a)
+        ops.free_pages(m, torch.tensor([m._sequences[c].slot], dtype=torch.int32, device="cuda"), max_blocks=hint)
+        m.free_sequence(c)
+        o.free_sequence(c)
+        same(m, o)
+
+
 def test_batched_refusals_change_nothing():
     rng = np.random.default_rng(2)
     m, o = pair(max_seqs=5)
@@ -163,6 +226,11 @@ def test_device_refusals_change_nothing():
         (ValueError, lambda: ops.compact_pages(m, ids(sa), ids(sa), ids(0, 1, 2), cu1, 3)),
         (IndexError, lambda: ops.compact_pages(m, ids(sa, sb), None, ids(0, 1, 2, 4, 5), cu2, 3)),
         (IndexError, lambda: ops.compact_pages(m, ids(sa), None, ids(-1, 1, 2), cu1, 3)),
+        # lists that leave keep, or end before they begin
+        (IndexError, lambda: ops.compact_pages(m, ids(sa), None, ids(0, 1, 2), ids(0, 4), 3)),
+        (IndexError, lambda: ops.compact_pages(m, ids(sa, sb), None, ids(0, 1, 2, 0, 1), ids(0, 1 << 30, 5), 3)),
+        (IndexError, lambda: ops.compact_pages(m, ids(sa, sb), None, ids(0, 1, 2, 0, 1), ids(-3, 3, 5), 3)),
+        (IndexError, lambda: ops.compact_pages(m, ids(sa, sb), ids(free_slot, 50), ids(0, 1, 2, 0, 1), ids(0, 3, 2), 3)),
         (RuntimeError, lambda: ops.compact_pages(m, ids(sa), ids(free_slot), torch.arange(20, 3, -1, **i32), ids(0, 17), 17)),
     ]
     for k, (exc, call) in enumerate(bad):
