@@ -194,7 +194,7 @@ __global__ void k_index_blocks(mentat_kv_cache c, int layer, const int32_t* bloc
 }
 
 template <typename T, bool WIDE>
-__global__ void k_index_seqs(mentat_kv_cache c, int layer0, const int32_t* slots, int first, mentat_page_index x,
+__global__ void k_index_seqs(mentat_kv_cache c, int layer0, const int32_t* slots, int n, int first, mentat_page_index x,
                              int max_pages) {
     griddep_wait();
     griddep_launch();
@@ -207,8 +207,12 @@ __global__ void k_index_seqs(mentat_kv_cache c, int layer0, const int32_t* slots
     const int full = min(len / c.block_size, c.max_blocks_per_seq);
     int p = first + blockIdx.x % max_pages;
     if (first < 0) {
-        if (len == 0 || len % c.block_size) return;
-        p = full - 1;
+        // the page that ends with entry i's token: a sequence that occurs again behind i got later ones too
+        int later = 0;
+        for (int j = i + 1 + (threadIdx.x & 31); j < n; j += 32) later += slots[j] == slot;
+        const int mine = len - __reduce_add_sync(0xffffffffu, later);
+        if (mine <= 0 || mine % c.block_size) return;
+        p = mine / c.block_size - 1;
     }
     if (p >= full) return;
     const int b = table_row(c, layer, slot)[p];
@@ -1528,11 +1532,11 @@ int mentat_page_index_seqs(const mentat_kv_cache* c, int32_t layer, const int32_
     const int l0 = layer < 0 ? 0 : layer, layers = layer < 0 ? c->num_layers : 1;
     if (const int threads = index_block_threads(c)) {
         MENTAT_BY_DTYPE(MENTAT_LAUNCH((k_index_seqs<T, true>), dim3(n * max_pages, 1, layers), dim3(threads), 0, s, *c, l0,
-                                      slots, first, *x, max_pages))
+                                      slots, n, first, *x, max_pages))
         return MENTAT_OK;
     }
     const dim3 grid(n * max_pages, c->num_kv_heads, layers), block((c->head_dim + 31) / 32 * 32);
-    MENTAT_BY_DTYPE(MENTAT_LAUNCH((k_index_seqs<T, false>), grid, block, 0, s, *c, l0, slots, first, *x, max_pages))
+    MENTAT_BY_DTYPE(MENTAT_LAUNCH((k_index_seqs<T, false>), grid, block, 0, s, *c, l0, slots, n, first, *x, max_pages))
     return MENTAT_OK;
 }
 

@@ -314,15 +314,34 @@ def _check_out(name: str, out: torch.Tensor, x: torch.Tensor) -> None:
             ((h == 1 or s1 >= d) and (n == 1 or s0 >= (h - 1) * s1 * (h > 1) + d)) or
             ((n == 1 or s0 >= d) and (h == 1 or s1 >= (n - 1) * s0 * (n > 1) + d))):
         raise ValueError(f"{name} must hold rows of its own, each contiguous")
-    if out.data_ptr() == x.data_ptr() and out.stride() == x.stride():
-        return
-
-    def span(t):
-        a = t.data_ptr()
-        return a, a + t.element_size() * (sum((m - 1) * s for m, s in zip(t.shape, t.stride())) + 1)
-    (a0, a1), (b0, b1) = span(out), span(x)
-    if a0 < b1 and b0 < a1:
+    if not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride() or _apart(out, x)):
         raise ValueError(f"{name} must be the input itself or not overlap it")
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of rows share no byte: separate ranges of memory, or separate parts of
+    the rows of one buffer (equal token strides)."""
+    if a.numel() == 0 or b.numel() == 0:
+        return True
+
+    def reach(t, dims):
+        return t.element_size() * (sum((m - 1) * s for m, s in zip(t.shape[dims:], t.stride()[dims:])) + 1)
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    if a0 + reach(a, 0) <= b0 or b0 + reach(b, 0) <= a0:
+        return True
+    row = a.stride(0) * a.element_size()
+    if row <= 0 or row != b.stride(0) * b.element_size():
+        return False
+    at = (b0 - a0) % row  # b's part, from the start of one of a's
+    return reach(a, 1) <= at and at + reach(b, 1) <= row
+
+
+def _check_apart(**tensors) -> None:
+    """Refuses an output (the first, if given) that shares memory with another operand."""
+    (name, out), *others = tensors.items()
+    for other, t in others:
+        if out is not None and t is not None and not _apart(out, t):
+            raise ValueError(f"{name} must not overlap {other}")
 
 
 def _check_positions(positions: torch.Tensor, n: int, device) -> torch.Tensor:
@@ -367,6 +386,9 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     if k is not None:
         k, rk = _operand("k", k, n, d, dtype, dev)
         ko, rko = _out_rows("k_out", k_out, k)
+        if q_out is not None or k_out is not None:
+            _check_apart(q_out=q_out, k=k, k_out=k_out)
+            _check_apart(k_out=k_out, q=q)
     if n:
         _call(dev, "mentat_rotary_apply", _DT[dtype], d, n, *_rows(rq, rqo, rk, rko), positions.data_ptr(),
               rotary._ptrs[bool(inverse)])
@@ -398,6 +420,7 @@ def rotary_append(cache, layer: int, rows: torch.Tensor, q: Optional[torch.Tenso
     if q is not None:
         q, rq = _operand("q", q, n, d, dtype, dev)
         qo, rqo = _out_rows("q_out", q_out, q)
+        _check_apart(q_out=q_out, k=k, v=v)
     if n:
         _call(dev, "mentat_rotary_append", cache._desc_ptr, layer, n, rows.data_ptr(), *_rows(rq, rqo, rk, rv),
               positions.data_ptr(), rotary._ptrs[0])
@@ -440,7 +463,7 @@ def append_rotated(k_pool, v_pool, slots, q, k, v, cache, layer, rotary):
 
 
 def _index_tails(mgr, layer: int, slots: torch.Tensor, n: int) -> None:
-    """Indexes each sequence's last page, if it is full (after a batched append)."""
+    """Indexes the pages that a batched append to ``slots`` has filled."""
     _call(mgr.device, "mentat_page_index_seqs", mgr._desc_ptr, layer, slots.data_ptr(),
           n, -1, 1, mgr.page_index._ptr)
 

@@ -517,7 +517,12 @@ class PagedKVCacheManager:
         lists, counts, per_layer = [], [], False
         for seq, k in zip(seqs, keep):
             if on_device:
-                k = torch.as_tensor(k).to(device=self.device, dtype=torch.int32)
+                k = torch.as_tensor(k)
+                if k.numel() and (k.dtype == torch.bool or k.is_floating_point() or k.is_complex()):
+                    raise TypeError("kept positions must be whole numbers")
+                if k.dtype == torch.int64:
+                    k = k.clamp(-1, 0x7fffffff)  # stay outside when cut to 32 bits
+                k = k.to(device=self.device, dtype=torch.int32)
                 ndim, shape = k.dim(), tuple(k.shape)
             else:
                 k = np.asarray(k)
@@ -580,7 +585,8 @@ class PagedKVCacheManager:
     def enable_page_index(self) -> PageIndex:
         """The cache's :class:`PageIndex`: made at the first call, from the pages of
         every live sequence, and from then on kept by every append, trim and
-        compaction of this class (a page is indexed when it is full)."""
+        compaction of this class (a page is indexed when it is full).  A graph of appends
+        that was captured before does not keep it."""
         if self.page_index is None:
             self.page_index = PageIndex(self)
             live = list(self._sequences.values())

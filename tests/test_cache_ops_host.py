@@ -92,6 +92,20 @@ def test_row_operands_refused():
     base = torch.zeros(4, 4, 64)
     with pytest.raises(ValueError, match="not overlap"):
         ops.rotary(base[:3], None, p, r, q_out=base[1:])
+    both = torch.zeros(3, 6, 64)
+    for outs in (dict(q_out=both[:, :4], k_out=both[:, 3:5]), dict(q_out=torch.zeros(1), k_out=q[:, 1:3]),
+                 dict(q_out=q, k_out=q[:, :2])):
+        with pytest.raises(ValueError):
+            ops.rotary(q, k, p, r, **outs)
+    with pytest.raises(ValueError, match="q_out must not overlap k"):
+        ops.rotary(q, q.clone()[:, :2], p, r, q_out=both[:, :4], k_out=both[:, 2:4])
+    with pytest.raises(ValueError, match="q_out must not overlap k"):
+        ops.rotary(both[:, 2:6].clone(), both[:, :4], p, r, q_out=both[:, :4])
+    # parts of one buffer's rows are apart
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.rotary(both[:, :4], both[:, 4:], p, r, q_out=both[:, :4], k_out=both[:, 4:])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.rotary(q, k, p, r, q_out=both[:, 2:], k_out=both[:, :2])
     with pytest.raises(TypeError):
         ops.rotary(q, k.double(), p, r)
     with pytest.raises(TypeError):

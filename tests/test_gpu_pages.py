@@ -195,6 +195,10 @@ def test_batched_refusals_change_nothing():
         m.compact_sequences([a, b], [[0]])
     with pytest.raises(TypeError):
         m.compact_sequences([a], [[0.5]])
+    for mask in (torch.ones(9, dtype=torch.bool, device="cuda"), torch.zeros(3, device="cuda")):
+        with pytest.raises(TypeError):
+            m.compact_sequences([a], [mask])
+    assert m.get_kv_length(a) == 9
     assert m.fork_sequences([]) == [] and m.free_sequences([]) is None and m.compact_sequences([], []) is None
     same(m, o)
 
@@ -320,6 +324,57 @@ def test_compaction_of_device_positions_on_another_stream():
     torch.cuda.current_stream().wait_stream(s)
     compact(o, ids, [k.cpu().numpy() for k in keep])
     same(m, o)
+
+
+def test_captured_page_operators():
+    """Forks, a compaction into new slots, one in place and releases in one graph, replayed: the state that the
+    same calls leave one after another."""
+    from mentat_b200 import ops
+    rng = np.random.default_rng(14)
+    m, o = pair(L=2, pool=400)
+    a, b = ids = start(m, o, [41, 18], rng)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    slots = torch.tensor([m._sequences[s].slot for s in ids], **i32)
+    kids = torch.tensor(m._free_slots[-4:][::-1], **i32)  # the slots that the next sequences get
+    keep = [np.r_[0:4, 9:30], np.r_[5:18]]
+    flat = torch.from_numpy(np.concatenate(keep)).to(**i32)
+    cu = torch.tensor([0, 25, 38], **i32)
+
+    def step():
+        ops.fork_pages(m, slots, kids[:2])
+        ops.compact_pages(m, slots, kids[2:], flat, cu, 25)
+        ops.free_pages(m, kids[:2])
+        ops.free_pages(m, kids[2:])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    for _ in range(3):
+        g.replay()
+        fork = [o.fork_sequence(s) for s in ids]
+        new = compact(o, ids, keep, into_new=True)
+        for s in fork + new:
+            o.free_sequence(s)
+    same(m, o)
+    # in place: two graphs over one cache
+    g2 = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g2):
+        ops.compact_pages(m, slots[1:], None, torch.arange(12, -1, -1, **i32), torch.tensor([0, 13], **i32), 13)
+    for graph in (g2, g, g2):
+        if graph is g:  # what g keeps of b: its positions 0 .. 12
+            flat[25:] = torch.arange(13, **i32)
+            keep[1] = np.arange(13)
+            g.replay()
+            fork = [o.fork_sequence(s) for s in ids]
+            for s in fork + compact(o, ids, keep, into_new=True):
+                o.free_sequence(s)
+        else:
+            g2.replay()
+            compact(o, [b], [np.arange(13)[::-1]])
+        for layer in range(2):
+            st, w = m._sequences[b], o._sequences[b]
+            st.num_tokens[layer], st.num_blocks[layer] = w.num_tokens[layer], len(w.page_table[layer])
+            st.tokens_in_last_block[layer] = w.tokens_in_last_block[layer]
+        same(m, o)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])

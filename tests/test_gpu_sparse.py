@@ -367,6 +367,35 @@ def test_index_is_kept_by_the_cache():
     check()
 
 
+def test_index_of_a_sequence_twice_in_a_batch():
+    """A page that fills in the middle of a batch, under a repeated sequence, holds the bounds of its new keys."""
+    from mentat_b200 import PagedKVCacheManager, Rotary
+    m = PagedKVCacheManager(1, 2, 64, max_blocks=40, block_size=4, device="cuda", dtype=torch.bfloat16, max_seqs=32)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rot = Rotary(64)
+
+    def rows(n):
+        return torch.randn((n, 2, 64), generator=g, device="cuda").bfloat16()
+    m.enable_page_index()
+    for _ in range(2):  # the second time over blocks whose old bounds are in the index
+        a, b = m.allocate_sequence(), m.allocate_sequence()
+        m.append_tokens(a, 0, rows(2), rows(2))
+        m.append_tokens_batched([a, b, a, a, b], 0, rows(5), rows(5))                       # a 5, b 2
+        m.append_rotated_batched([b] + [a] * 8 + [b] * 7, 0, rows(16), rows(16), rows(16), rot)  # a 13, b 10
+        for s in (a, b):
+            st = m._sequences[s]
+            for block in m._tables[0, st.slot, : st.num_tokens[0] // 4].tolist():
+                bounds, e = index_page(m.k_pools[0][block].double().cpu().numpy())
+                np.testing.assert_array_equal(m.page_index.bounds[0, block].cpu().numpy(), bounds)
+                np.testing.assert_array_equal(m.page_index.exps[0, block].cpu().numpy(), e)
+        m.free_sequences([a, b])
+        for s in range(20):  # the ring comes round to the same blocks
+            c = m.allocate_sequence()
+            m.append_tokens(c, 0, rows(8), rows(8))
+            m.free_sequence(c)
+    m.check()
+
+
 def test_captured_and_on_another_stream():
     from mentat_b200 import ops
     lens = [900, 70]
