@@ -17,6 +17,10 @@
 //
 // The steps of one call depend on one another across all rows.  Where they are small, one cluster
 // of CTAs takes them all, with cluster barriers between them; else each step is a launch.
+//
+// Forks and frees are bound by latency: chains of dependent loads and barriers.  Fork and free of 64 x 3 children of 130
+// to 160 pages in 32 layers: 8 + 23 us, against 1 us of bytes; of 6 of 30 pages: 4 + 11 us.  A compaction is bound by the
+// rows that it moves.
 
 #include <cooperative_groups.h>
 
@@ -440,18 +444,20 @@ struct CompactArgs {
 
 constexpr int PLAN_CHUNK = 512;  // kept positions of a warp's step; the last chunk goes on to the end of a list
 // The plan, in one cluster, a warp a range of rows: the batch is checked, the kept positions are inside their
-// sequences; how many pages at the front stay, and the fresh blocks of the others.  (The lists are a
-// thousandth of the bytes that are moved.)
+// sequences; how many pages at the front stay, and the fresh blocks of the others.  Bound by latency (the lists
+// are a thousandth of the bytes that are moved): 12 us for 8 sequences in 4 layers, 21 for 12 of 16,000 tokens in 2.
 __global__ void __launch_bounds__(CLUSTER_THREADS) k_compact_plan(mentat_kv_cache c, CompactArgs a, int chunks,
                                                                   PagesWs w) {
     extern __shared__ uint32_t bits[];
-    __shared__ int s_bad, s_total[CLUSTER_WARPS];
+    __shared__ int s_bad, s_list, s_is_list, s_total[CLUSTER_WARPS];
     cg::cluster_group cluster = cg::this_cluster();
+    if (threadIdx.x == 0) s_is_list = 0;  // (slots_distinct synchronises)
     griddep_wait();
     griddep_launch();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = cluster.block_rank(), L = c.num_layers;
     // every CTA checks the whole batch
-    bool ok = slots_distinct(c, a.dst ? a.dst : a.src, a.n, bits, &s_bad);
+    const bool ok = slots_distinct(c, a.dst ? a.dst : a.src, a.n, bits, &s_bad);
+    const bool before = has_error(c);
     int no = 0;
     if (a.dst && ok)  // sources in range, destinations empty in every layer (so none is a source with tokens)
         for (int64_t x = threadIdx.x; x < (int64_t)a.n * L; x += CLUSTER_THREADS) {
@@ -464,17 +470,17 @@ __global__ void __launch_bounds__(CLUSTER_THREADS) k_compact_plan(mentat_kv_cach
                 s_bad = a.dst[i];
             }
         }
-    ok = !__syncthreads_or(no) && ok;
-    if (!ok && threadIdx.x == 0) set_error(c, MENTAT_DEV_BAD_SLOT, s_bad);
-    int off = -1;  // a list that does not lie within keep: nothing of it is read
-    for (int i = threadIdx.x; i < a.n; i += CLUSTER_THREADS)
-        if (a.cu[i] < 0 || a.cu[i + 1] < a.cu[i] || a.cu[i + 1] > a.total) off = i;
-    if (off >= 0) s_bad = a.cu[off + 1];
-    if (__syncthreads_or(off >= 0)) {
-        if (ok && threadIdx.x == 0) set_error(c, MENTAT_DEV_BAD_TOKEN, s_bad);
-        ok = false;
+    for (int i = threadIdx.x; i < a.n; i += CLUSTER_THREADS)  // lists within keep: nothing of another is read
+        if (a.cu[i] < 0 || a.cu[i + 1] < a.cu[i] || a.cu[i + 1] > a.total) {
+            no = 1;
+            s_list = a.cu[i + 1];
+            s_is_list = 1;
+        }
+    bool stop = __syncthreads_or(no || !ok || before);
+    if (stop && threadIdx.x == 0 && !before) {
+        if (s_is_list) set_error(c, MENTAT_DEV_BAD_TOKEN, s_list);
+        else set_error(c, MENTAT_DEV_BAD_SLOT, s_bad);
     }
-    bool stop = __syncthreads_or(!ok || has_error(c));
     const int rows = a.n * L, per = (rows + CLUSTER_ALL_WARPS - 1) / CLUSTER_ALL_WARPS;
     const int r0 = min(rows, (rank * CLUSTER_WARPS + warp) * per), r1 = min(rows, r0 + per);
     if (!stop)
@@ -545,10 +551,16 @@ __global__ void __launch_bounds__(CLUSTER_THREADS) k_compact_plan(mentat_kv_cach
         const int first = w.first[row] + base, count = w.count[row];
         __syncwarp();
         if (lane == 0) w.first[row] = first;
-        for (int j = lane; j < count; j += 32) {
-            const int b = c.free_ring[(head + first + j) % c.num_blocks];
-            w.fresh[first + j] = b;
-            c.refcounts[b] = 1;
+        for (int j = lane; j < count; j += 256) {
+            int b[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) b[u] = j + 32 * u < count ? c.free_ring[(head + first + j + 32 * u) % c.num_blocks] : -1;
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (b[u] >= 0) {
+                    w.fresh[first + j + 32 * u] = b[u];
+                    c.refcounts[b[u]] = 1;
+                }
         }
     }
 }
@@ -684,7 +696,8 @@ __device__ __forceinline__ void turn_row(T* row, int H, int D, const mentat_rota
 // through a ring of stages.  A producer warp looks up where the rows come from and copies them in with bulk
 // copies, K and V, a stage ahead or more; eight warps turn K in place; the stage, which is contiguous in the
 // fresh page, leaves as two bulk copies.  So the bytes pass through registers only where they change, and the
-// next rows are always on the way.  Bound by memory.
+// next rows are always on the way.  Bound by memory: 1.3 GB in 223 us, 5.9 TB/s (through registers, a CTA a page: 3.0);
+// 75 MB in 19 us, of which the first and last stages, which nothing covers, are 6.
 constexpr int STREAM_WORKERS = 256, STREAM_THREADS = STREAM_WORKERS + 32, STREAM_MAX_STAGES = 4;
 template <typename T, int VEC, bool IL>
 __global__ void __launch_bounds__(STREAM_THREADS) k_compact_stream(mentat_kv_cache c, CompactArgs a, mentat_rotary r,
@@ -868,7 +881,11 @@ static int launch_one_cluster(void (*kernel)(KArgs...), size_t smem, cudaStream_
     return MENTAT_OK;
 }
 
-// Releases are one cluster's work while a warp has at most this many groups of 32 table entries.
+// Releases are one cluster's work while a warp has at most this many groups of 32 table entries.  One launch instead
+// of four saves the host 6 us (fork and free of 6 sequences: 16.5 and 22.4).  On the device both are as fast at 1 a
+// warp (8 siblings of 30 pages in 32 layers: 15.3); at 3 the cluster takes 22 us and four launches 40 for 12
+// sequences of 440 pages of their own, at 4 it is 25 and 17 for 16 siblings of 60 pages, which k_free_mark takes
+// in runs; 32 of them, 8 a warp, 40 and 19.
 constexpr int FREE_CLUSTER_PER = 4;
 
 template <bool LEAD>
@@ -905,7 +922,9 @@ struct LaunchCompactMove {
         const int64_t rows = (int64_t)a.n * c.num_layers, most = rows * ((max_keep + c.block_size - 1) / c.block_size);
         const size_t table = (size_t)MOVE_TOKENS * 2 * r.pairs * sizeof(float);
         if constexpr (VEC > 1) {
-            // stages of up to 16 tokens and 64 KB, three of them or four; several CTAs on an SM where they are small
+            // stages of up to 16 tokens and 64 KB, three of them or four; several CTAs on an SM where they are small.
+            // 12 sequences, 1.3 GB (64 KB for 16 tokens): 277 us with 16 tokens, 308 with 8, 320 with 4; 3 or 4
+            // stages are alike, 2 take 438.
             const int64_t row = (int64_t)c.num_kv_heads * c.head_dim * sizeof(T);
             int tokens = c.block_size < MOVE_TOKENS ? c.block_size : MOVE_TOKENS;
             while (tokens > 1 && 2 * tokens * row > 64 * 1024) tokens /= 2;

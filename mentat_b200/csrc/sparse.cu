@@ -282,11 +282,13 @@ __global__ void __launch_bounds__(256) k_page_bounds(mentat_kv_cache c, int laye
 // ---------------------------------------------------------------------------
 // The cluster's CTAs score a slice of the pages each and write the keys to all of their
 // shared memories; each then makes the whole choice for itself, attends to an equal share
-// of the chosen pages, and they merge their partials: one launch, and no workspace.
+// of the chosen pages, and they merge their partials: one launch, and no workspace.  Bound by latency: one sequence of
+// 4,000 tokens takes 10 us (slots, lengths, table, bounds, the choice and the pages wait for one another).
 // warps of a CTA: with the tensor-core path's rings two CTAs of four fit on an SM; the other path is bound by
 // latency and takes eight
 __host__ __device__ constexpr int sparse_warps(bool mma) { return mma ? 4 : 8; }
-constexpr int SPARSE_STAGES = 3;  // groups of 16 tokens that a warp holds or has on the way
+// groups of 16 tokens that a warp holds or has on the way: as many as leave room for two CTAs on an SM (96 KB)
+constexpr int SPARSE_STAGES = 3;
 constexpr int SPARSE_MAX_BUDGET = 8192, SPARSE_MAX_GROUP = 16, SPARSE_MAX_CLUSTER = 16;
 
 struct SparseArgs {
@@ -316,13 +318,14 @@ struct SparseArgs {
 struct SparseSmem {
     int po, q8, keys, qf, ml, pages, blocks, total;
 };
-__host__ __device__ inline SparseSmem sparse_smem(int G, int GM, int D, bool mma, int pages, int share) {
+__host__ __device__ inline SparseSmem sparse_smem(int G, int GM, int D, bool mma, bool listed, int pages,
+                                                  int share) {
     SparseSmem s;
     share = (share + 3) / 4 * 4;
     const int warps = sparse_warps(mma), attend = mma ? warps * SPARSE_STAGES * 16 * D : 0, partials = warps * G * D;
     s.po = s.q8 = 0;
     s.keys = (GM < 8 ? 8 : GM) * 2 * D / 4;
-    const int chose = pages ? s.keys + (pages + 3 + 3) / 4 * 4 : 0;
+    const int chose = listed ? 0 : s.keys + (pages + 3 + 3) / 4 * 4;
     s.qf = attend > partials ? attend : partials;
     if (chose > s.qf) s.qf = chose;
     s.ml = s.qf + (mma ? 0 : G * D);
@@ -799,6 +802,10 @@ __device__ __forceinline__ void attend_simple(const mentat_kv_cache& c, const Sp
 //
 // P is rounded to the element type for the product; the sum of P is taken of the rounded values, so the
 // weights sum to one.
+//
+// Bound by memory: 64 sequences with 128 pages each for 8 KV heads of 128 (540 MB of different rows, 1.07 GB with
+// those that several sequences chose) take 80 us, 6.7 TB/s of the former.  A tile of the larger tensor-core
+// instruction has 128 rows, of which a KV head's group would fill at most 16.
 template <typename T, int D, int GM>
 __device__ __forceinline__ void attend_mma(const mentat_kv_cache& c, const SparseArgs& a, const CUtensorMap* mk,
                                            const CUtensorMap* mv, int h, int len, const int32_t* pages,
@@ -948,8 +955,8 @@ __device__ __forceinline__ void attend_mma(const mentat_kv_cache& c, const Spars
     }
 }
 
-// The scores may have been made before (a.keys), and the choice too (a.list).
-template <typename T, int D, int GM, bool MMA>
+// LISTED: the choice was made before (k_score, k_choose); only the attention is left.
+template <typename T, int D, int GM, bool MMA, bool LISTED>
 __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_constant__ CUtensorMap mk,
                                                            const __grid_constant__ CUtensorMap mv, mentat_kv_cache c,
                                                            mentat_page_index x, SparseArgs a) {
@@ -962,7 +969,7 @@ __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, warp = tid >> 5, cs = cluster.num_blocks(), rank = cluster.block_rank();
     const int n = blockIdx.y, h = blockIdx.x / cs, G = a.G, H = c.num_kv_heads, bs = c.block_size;
-    const SparseSmem at = sparse_smem(G, GM, D, MMA, a.held, a.share);
+    const SparseSmem at = sparse_smem(G, GM, D, MMA, LISTED, a.held, a.share);
     float* pm = reinterpret_cast<float*>(smem + at.ml);
     float* pl = pm + SPARSE_WARPS * GM;
     float* po = reinterpret_cast<float*>(smem + at.po);
@@ -975,8 +982,7 @@ __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_
         for (int i = 0; i < SPARSE_WARPS * SPARSE_STAGES; ++i) mbar_init(smem_u32(bars + i), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const bool spread = cs > 1 && !a.keys;
-    if (spread) cluster.barrier_arrive();  // this CTA runs: its shared memory may be written
+    if (!LISTED && cs > 1) cluster.barrier_arrive();  // this CTA runs: its shared memory may be written
     griddep_wait();
     griddep_launch();
 
@@ -991,7 +997,7 @@ __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_
     }
     int P = (len + bs - 1) / bs;
     if (len > a.max_len || P > c.max_blocks_per_seq) {
-        if (tid == 0) set_error(c, MENTAT_DEV_PLAN_OVERFLOW, slot);
+        if (!LISTED && tid == 0) set_error(c, MENTAT_DEV_PLAN_OVERFLOW, slot);
         P = 0;
     }
     const int32_t* row = P ? table_row(c, a.layer, slot) : nullptr;
@@ -1000,25 +1006,20 @@ __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_
         for (int i = tid; i < G * D; i += SPARSE_THREADS) qf[i] = Elem<T>::to_f(q[i]);
 
     const int i0 = (int)((int64_t)rank * k / cs), count = (int)((int64_t)(rank + 1) * k / cs) - i0;
-    if (spread) cluster.barrier_wait();
-    if (!a.list && P > k) {  // every CTA of the cluster alike
-        if (a.keys) {
-            const uint4* from = reinterpret_cast<const uint4*>(a.keys + ((int64_t)n * H + h) * a.key_stride);
-            for (int p = tid; p < (P + 3) / 4; p += SPARSE_THREADS) reinterpret_cast<uint4*>(keys)[p] = from[p];
-        } else {
-            for (int g = warp; g < (GM < 8 ? 8 : GM); g += SPARSE_WARPS)
-                quantise<T, D>(q + g * D, g < G, q8 + 2 * g * D, s_unit + g);
-            __syncthreads();
-            const int each = (P + cs - 1) / cs, p0 = min(P, rank * each), p1 = min(P, p0 + each);
-            score_pages<D, GM, SPARSE_WARPS>(c, x, a, h, row, P, p0, p1, q8, s_unit, keys);
-        }
-        if (spread) cluster.sync(); else __syncthreads();
+    if (!LISTED && cs > 1) cluster.barrier_wait();
+    if (!LISTED && P > k) {  // every CTA of the cluster alike
+        for (int g = warp; g < (GM < 8 ? 8 : GM); g += SPARSE_WARPS)
+            quantise<T, D>(q + g * D, g < G, q8 + 2 * g * D, s_unit + g);
+        __syncthreads();
+        const int each = (P + cs - 1) / cs, p0 = min(P, rank * each), p1 = min(P, p0 + each);
+        score_pages<D, GM, SPARSE_WARPS>(c, x, a, h, row, P, p0, p1, q8, s_unit, keys);
+        if (cs > 1) cluster.sync(); else __syncthreads();
         choose<SPARSE_THREADS>(keys, P, k, i0, i0 + count, pages, s_choose);
     }
     // this CTA's share of the chosen pages, and their blocks
-    int32_t* told = !a.list && a.pages ? a.pages + ((int64_t)n * H + h) * a.budget : nullptr;
+    int32_t* told = !LISTED && a.pages ? a.pages + ((int64_t)n * H + h) * a.budget : nullptr;
     for (int i = tid; i < count; i += SPARSE_THREADS) {
-        const int p = a.list ? a.list[((int64_t)n * H + h) * a.budget + i0 + i] : P > k ? pages[i] : i0 + i, b = row[p];
+        const int p = LISTED ? a.list[((int64_t)n * H + h) * a.budget + i0 + i] : P > k ? pages[i] : i0 + i, b = row[p];
         const bool ok = (unsigned)b < (unsigned)c.num_blocks;
         if (!ok) set_error(c, MENTAT_DEV_BAD_BLOCK, b);
         pages[i] = p;
@@ -1027,7 +1028,7 @@ __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_
     }
     if (told && rank == 0)
         for (int i = k + tid; i < a.budget; i += SPARSE_THREADS) told[i] = -1;
-    if (MMA) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // keys, then TMA, in one place
+    if (MMA && !LISTED) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // keys, then TMA, in one place
     __syncthreads();
     if constexpr (MMA)
         attend_mma<T, D, GM>(c, a, &mk, &mv, h, len, pages, blocks, count, q, reinterpret_cast<uint8_t*>(smem), bars, pm,
@@ -1076,7 +1077,7 @@ __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_
 }
 
 // ---------------------------------------------------------------------------
-// large batches: scores, choice and attention in three launches
+// large batches: scores, choice and attention in launches of their own
 // ---------------------------------------------------------------------------
 // Adjacent sequences of a tree share most of their pages, so a CTA scores its pages for several
 // of them at once: the query heads of up to 16 sequences are the columns of the product (GP columns each,
@@ -1084,6 +1085,8 @@ __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_
 // where all of them have the same 16 blocks the bounds are read once.  Two warps take 16 pages, half of the
 // columns each.  Pages that are not shared are put aside, and then shared out by sequence among all warps of the
 // CTA.  A warp has the next pages' bounds and the blocks of those after them on the way while it works.
+// Bound by latency and issue: 64 sequences of 2,050 to 2,300 pages, 2,048 in common, 8 KV heads of 4 query heads: 19 us
+// (the bounds are 4 MB, the byte products 3 us); 24 where each warp pair scored its own unshared tiles.
 constexpr int SCORE_THREADS = 256, SCORE_WARPS = SCORE_THREADS / 32;
 constexpr int SCORE_TILES = SCORE_WARPS / 2;  // tiles of 16 pages at a time
 constexpr int SCORE_ASIDE = 1024;             // tiles between two looks at those put aside
@@ -1342,16 +1345,19 @@ __global__ void __launch_bounds__(SCORE_THREADS, 2) k_score(mentat_kv_cache c, m
     }
 }
 
-// The chosen pages from the keys where a sequence may have more than HELD_PAGES pages: a cluster per (sequence,
-// KV head).
+// The chosen pages from the keys (12 us for 512 of 2,200 pages; made by the attention's CTAs instead, the same batch
+// takes 126 us in all, not 121): one CTA per (sequence, KV head), or a cluster where a sequence may have
+// more than HELD_PAGES pages.
 constexpr int CHOOSE_THREADS = 256, HELD_PAGES = 16384;
+template <bool CL>
 __global__ void __launch_bounds__(CHOOSE_THREADS) k_choose(mentat_kv_cache c, SparseArgs a) {
     extern __shared__ __align__(16) uint32_t keys[];
-    __shared__ int smem32[32], counts[4 * 256];
+    __shared__ int smem32[CL ? 32 : 1], counts[CL ? 4 * 256 : 1];
+    __shared__ Chooser s_choose;
     griddep_wait();
     griddep_launch();
     cg::cluster_group cluster = cg::this_cluster();
-    const int cs = cluster.num_blocks(), rank = cluster.block_rank();
+    const int cs = CL ? cluster.num_blocks() : 1, rank = CL ? cluster.block_rank() : 0;
     const int tid = threadIdx.x, n = blockIdx.y, h = blockIdx.x / cs, H = c.num_kv_heads, bs = c.block_size;
     const int slot = a.slots[n];
     int len = slot >= 0 && slot < c.max_seqs ? c.ntok[seq_index(c, a.layer, slot)] : 0;
@@ -1368,30 +1374,34 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) k_choose(mentat_kv_cache c, Sp
     const uint32_t* from = a.keys + ((int64_t)n * H + h) * a.key_stride;
     for (int p = p0 + tid; p < p1; p += CHOOSE_THREADS) keys[p - p0] = from[p];
     __syncthreads();
-    choose_cluster<CHOOSE_THREADS>(keys, p0, p1 - p0, k, counts, list, smem32);
+    if constexpr (CL)
+        choose_cluster<CHOOSE_THREADS>(keys, p0, p1 - p0, k, counts, list, smem32);
+    else
+        choose<CHOOSE_THREADS>(keys, P, k, 0, k, list, s_choose);
 }
 
 // ---------------------------------------------------------------------------
 // launch
 // ---------------------------------------------------------------------------
 // How many CTAs share one (sequence, KV head): the largest power of two up to 8 that still runs all CTAs at
-// once (two on an SM with the rings of the tensor-core path, four without).  One sequence of 4,000 tokens,
-// 8 KV heads, budget 64: 24.9 / 17.3 / 13.1 / 11.4 us with 1 / 2 / 4 / 8; 16 sequences: 28.6 / 21.8 / 29.6 / 50.
-static int sparse_cluster(int heads, bool mma) {
+// once, two on an SM.  Budget 64, 8 KV heads of 128 in bf16, sequences of up to 1,000 pages, with 1 / 2 / 4 / 8: one
+// 31.8 / 21.6 / 15.4 / 12.8 us, 8 of them 36.8 / 25.7 / 19.5 / 31.0, 16 of them 41.8 / 33.1 / 40.1 / 62.6.  Of
+// 2 heads of 64 in fp32, 500 pages, 32 of them 48.6 / 29.3 / 25.0 / 33.6.
+static int sparse_cluster(int heads) {
     int cs = 1;
-    while (cs < 8 && (int64_t)heads * cs * 2 <= 148 * (mma ? 2 : 4)) cs *= 2;
+    while (cs < 8 && (int64_t)heads * cs * 2 <= 2 * 148) cs *= 2;
     return cs;
 }
 static bool sparse_mma(const mentat_kv_cache* c) { return c->dtype != MENTAT_F32 && c->block_size % 16 == 0; }
 
 // Whether the scores and the choice get launches of their own: from 600 pages for each CTA to score (and past
-// what k_sparse can hold).  Sequences of up to 1,000 pages, budget 64: 16 of them 33.6 us in one launch and 35.7
-// in several, 24 of them 56 and 50; with a 32,768-token prefix in common 8 of them 28.8 and 29.6, 16 of
-// them 43 and 39, 64 of them 159 and 91.
+// what k_sparse can hold).  In one launch and in several, as above: 16 sequences of up to 1,000 pages (500 a CTA)
+// 33.2 and 35.7 us, 24 of them (1,000) 56.6 and 46.7; behind a prefix of 32,768 tokens in common, 2,170 pages,
+// 8 of them (540) 28.9 and 29.8, 16 of them (1,090) 43 and 36, 64 of them 160 and 79.
 static bool sparse_listed(const mentat_kv_cache* c, int n, int max_len, int budget) {
     const int64_t pages = ((int64_t)max_len + c->block_size - 1) / c->block_size;
     if (pages <= budget) return false;
-    return pages > HELD_PAGES || pages > 600 * sparse_cluster(n * c->num_kv_heads, sparse_mma(c));
+    return pages > HELD_PAGES || pages > 600 * sparse_cluster(n * c->num_kv_heads);
 }
 
 // A kernel over clusters of cs CTAs.
@@ -1422,35 +1432,35 @@ static int launch_cluster(void (*kernel)(KArgs...), int cs, dim3 grid, int threa
     return MENTAT_OK;
 }
 
-template <typename T, int D, int GM, bool MMA>
+template <typename T, int D, int GM, bool MMA, bool LISTED>
 static int launch_sparse(const mentat_kv_cache* c, const mentat_page_index* x, SparseArgs a, cudaStream_t s) {
-    const int pages = (a.max_len + c->block_size - 1) / c->block_size, cs = sparse_cluster(a.n * c->num_kv_heads, MMA);
-    a.held = pages <= a.budget || a.list ? 0 : pages;
+    const int pages = (a.max_len + c->block_size - 1) / c->block_size, cs = sparse_cluster(a.n * c->num_kv_heads);
+    a.held = pages;
     a.share = (min(pages, a.budget) + cs - 1) / cs;
-    const size_t smem = 4 * (size_t)sparse_smem(a.G, GM, D, MMA, a.held, a.share).total + 1024;
+    const size_t smem = 4 * (size_t)sparse_smem(a.G, GM, D, MMA, LISTED, a.held, a.share).total + 1024;
     CUtensorMap mk{}, mv{};
     if (MMA && !pool_maps(c, a.layer, &mk, &mv)) return MENTAT_ERR_CUDA;
-    return launch_cluster(k_sparse<T, D, GM, MMA>, cs, dim3(c->num_kv_heads * cs, a.n), 32 * sparse_warps(MMA), smem, s,
+    return launch_cluster(k_sparse<T, D, GM, MMA, LISTED>, cs, dim3(c->num_kv_heads * cs, a.n), 32 * sparse_warps(MMA), smem, s,
                           mk, mv, *c, *x, a);
 }
 
 // 16-bit types with pages of 16 rows or a multiple run on tensor cores
-template <typename T, int D, int GM>
+template <typename T, int D, int GM, bool LISTED>
 static int launch_sparse_kind(const mentat_kv_cache* c, const mentat_page_index* x, const SparseArgs& a,
                               cudaStream_t s) {
     if constexpr (sizeof(T) == 2)
         if (sparse_mma(c) && a.qs % 4 == 0 && (uintptr_t)a.q % 8 == 0)
-            return launch_sparse<T, D, (GM > 8 ? 16 : 8), true>(c, x, a, s);
-    return launch_sparse<T, D, GM, false>(c, x, a, s);
+            return launch_sparse<T, D, (GM > 8 ? 16 : 8), true, LISTED>(c, x, a, s);
+    return launch_sparse<T, D, GM, false, LISTED>(c, x, a, s);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool LISTED>
 static int launch_sparse_group(const mentat_kv_cache* c, const mentat_page_index* x, const SparseArgs& a,
                                cudaStream_t s) {
-    if (a.G <= 2) return launch_sparse_kind<T, D, 2>(c, x, a, s);
-    if (a.G <= 4) return launch_sparse_kind<T, D, 4>(c, x, a, s);
-    if (a.G <= 8) return launch_sparse_kind<T, D, 8>(c, x, a, s);
-    return launch_sparse_kind<T, D, 16>(c, x, a, s);
+    if (a.G <= 2) return launch_sparse_kind<T, D, 2, LISTED>(c, x, a, s);
+    if (a.G <= 4) return launch_sparse_kind<T, D, 4, LISTED>(c, x, a, s);
+    if (a.G <= 8) return launch_sparse_kind<T, D, 8, LISTED>(c, x, a, s);
+    return launch_sparse_kind<T, D, 16, LISTED>(c, x, a, s);
 }
 
 template <int D, int GP>
@@ -1468,7 +1478,7 @@ static int launch_score(const mentat_kv_cache* c, const mentat_page_index* x, co
 template <typename T, int D>
 static int launch_sparse_dim(const mentat_kv_cache* c, const mentat_page_index* x, const SparseArgs& a,
                              cudaStream_t s) {
-    if (!a.keys) return launch_sparse_group<T, D>(c, x, a, s);
+    if (!a.keys) return launch_sparse_group<T, D, false>(c, x, a, s);
     const int heads = a.n * a.G * c->num_kv_heads;
     MENTAT_LAUNCH(k_score_queries<T, D>, dim3((heads + 3) / 4), dim3(128), 0, s, (const T*)a.q, a.qs, heads,
                   a.G * c->num_kv_heads, a.q8, a.units);
@@ -1479,15 +1489,14 @@ static int launch_sparse_dim(const mentat_kv_cache* c, const mentat_page_index* 
     else if (a.G <= 8) sc = launch_score<D, 8>(c, x, a, s);
     else sc = launch_score<D, 16>(c, x, a, s);
     if (sc != MENTAT_OK) return sc;
-    if (a.list) {
-        const int pages = (a.max_len + c->block_size - 1) / c->block_size;
-        int cs = 2;
-        while (cs < SPARSE_MAX_CLUSTER && (pages + cs - 1) / cs > HELD_PAGES) cs *= 2;
-        const size_t smem = 4 * (size_t)((pages + cs - 1) / cs + 3);
-        const int st = launch_cluster(k_choose, cs, dim3(c->num_kv_heads * cs, a.n), CHOOSE_THREADS, smem, s, *c, a);
-        if (st != MENTAT_OK) return st;
-    }
-    return launch_sparse_group<T, D>(c, x, a, s);
+    const int pages = (a.max_len + c->block_size - 1) / c->block_size;
+    int cs = 1;
+    while (cs < SPARSE_MAX_CLUSTER && (pages + cs - 1) / cs > HELD_PAGES) cs *= 2;
+    const size_t smem = 4 * (size_t)((pages + cs - 1) / cs + 3);
+    const int st = launch_cluster(cs > 1 ? k_choose<true> : k_choose<false>, cs, dim3(c->num_kv_heads * cs, a.n),
+                                  CHOOSE_THREADS, smem, s, *c, a);
+    if (st != MENTAT_OK) return st;
+    return launch_sparse_group<T, D, true>(c, x, a, s);
 }
 
 }  // namespace mentat
@@ -1584,8 +1593,7 @@ int mentat_sparse_decode(const mentat_kv_cache* c, int32_t layer, const mentat_p
         a.q8 = reinterpret_cast<int8_t*>(next);
         next += (int64_t)n * Hq * c->head_dim / 2;
         a.units = reinterpret_cast<float*>(next);
-        if (max_len > (int64_t)HELD_PAGES * c->block_size)
-            a.list = pages ? pages : reinterpret_cast<int32_t*>(next + (int64_t)n * Hq);
+        a.list = pages ? pages : reinterpret_cast<int32_t*>(next + (int64_t)n * Hq);
     }
     int st = MENTAT_OK;
     if (c->head_dim == 128) {

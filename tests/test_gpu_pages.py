@@ -357,8 +357,9 @@ def test_captured_page_operators():
     same(m, o)
     # in place: two graphs over one cache
     g2 = torch.cuda.CUDAGraph()
+    back, cu2 = torch.arange(12, -1, -1, **i32), torch.tensor([0, 13], **i32)
     with torch.cuda.graph(g2):
-        ops.compact_pages(m, slots[1:], None, torch.arange(12, -1, -1, **i32), torch.tensor([0, 13], **i32), 13)
+        ops.compact_pages(m, slots[1:], None, back, cu2, 13)
     for graph in (g2, g, g2):
         if graph is g:  # what g keeps of b: its positions 0 .. 12
             flat[25:] = torch.arange(13, **i32)
