@@ -487,3 +487,58 @@ def test_rollout_with_fused_rotary_and_all_pages(mode):
                 np.testing.assert_allclose([x["log_prob"] for x in got], [x["log_prob"] for x in want["results"]],
                                            rtol=1e-4, atol=1e-4)
             assert r.cache.get_stats()["blocks_used"] == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 8, 128), (10, 2, 64), (8, 1, 128), (16, 1, 64), (24, 2, 128)])
+def test_weights_keep_more_bits_than_the_element_type(hq, hkv, d, dtype):
+    """Off by the rounding of the output and 32-bit sums, not by weights rounded to the element type.
+
+    Keys and queries have one channel, so the scores' products are exact.  A weight: the exponent |s| < 8 after the
+    scale, its rounding and the difference from the maximum, 4 roundings of 8 2^-24 ln 2 < 2^-19.4; exp2 and at most 4
+    factors between partials, 2^-21 each; 20 tokens' sums 20 2^-24, and as much again in the product unit.  Below
+    2^-17.5, in numerator and denominator: 2^-16.5 of sum w |v|.  What two parts of a weight leave: (eps / 2)^2."""
+    from mentat_b200 import ops
+    lens = [1, 2, 5, 17, 20]
+    c, x, q, tables = make(lens, hq, hkv, d, 16, dtype, layers=1)
+    k, v = c._tensors["k_pool"], c._tensors["v_pool"]
+    k[..., 1:] = 0
+    q[..., 1:] = 0
+    k.clamp_(-2, 2)
+    q.clamp_(-2, 2)
+    slots = torch.arange(len(lens), dtype=torch.int32, device="cuda")
+    got = ops.sparse_decode(x, 0, slots, q, 20, 4, scale=1.0).double().cpu().numpy()
+    c.check()
+    half = torch.finfo(c.dtype).eps / 2
+    kd, vd, qd = (t.double().cpu().numpy() for t in (k[0], v[0], q))
+    for i, n in enumerate(lens):
+        rows = tables[0, i][np.arange(n) // 16], np.arange(n) % 16
+        for h in range(hq):
+            s = kd[rows][:, h // (hq // hkv), 0] * qd[i, h, 0]
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            vals = vd[rows][:, h // (hq // hkv)]
+            want, size = w @ vals, w @ np.abs(vals)
+            wide = (half * half + 2.0 ** -16.5) * size
+            tol = wide + half * (np.abs(want) + wide) + (2.0 ** -25 if dtype == "f16" else 0.0)
+            off = np.abs(got[i, h] - want) - tol
+            assert off.max() <= 0, (n, h, off.max(), tol[off.argmax()])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("hq", [8, 16])
+def test_infinite_values_show_as_such(hq, dtype):
+    """A value of infinity gives infinity in its channel, whatever part of its weight is 0; behind the last token it
+    is not seen."""
+    from mentat_b200 import ops
+    lens = [1, 20]
+    c, x, q, tables = make(lens, hq, 1, 64, 16, dtype, layers=1)
+    v = c._tensors["v_pool"]
+    v[0, int(tables[0, 0, 0]), 0, 0, 3] = float("inf")
+    v[0, int(tables[0, 0, 0]), 5, 0, 4] = float("inf")          # no token of the sequence
+    v[0, int(tables[0, 1, 1]), 2, 0, 60] = -float("inf")
+    slots = torch.arange(2, dtype=torch.int32, device="cuda")
+    out = ops.sparse_decode(x, 0, slots, q, 20, 4)
+    assert (out[0, :, 3] == float("inf")).all() and (out[1, :, 60] == -float("inf")).all()
+    out[0, :, 3] = out[1, :, 60] = 0
+    assert torch.isfinite(out).all()
