@@ -149,7 +149,15 @@ class Rotary:
     @classmethod
     def from_module(cls, rotary_emb, head_dim: int) -> "Rotary":
         """The angles of a Hugging Face rotary module (its ``inv_freq`` and
-        ``attention_scaling``; Llama and Qwen3 pair i with i + rotary_dim / 2)."""
+        ``attention_scaling``; Llama and Qwen3 pair i with i + rotary_dim / 2).
+        A module of type ``dynamic`` or ``longrope`` is refused: it replaces its
+        frequencies while it runs, when a sequence passes the original context, and
+        what it holds now is right for some lengths only.  For one length its
+        angles are ``Rotary(head_dim, base=..., scaling=..., seq_len=...)``."""
+        kind = getattr(rotary_emb, "rope_type", None)
+        if kind in ("dynamic", "longrope"):
+            raise ValueError(f"rope_type {kind!r} changes its frequencies with the length of the sequence: "
+                             "give Rotary its base, scaling and seq_len instead")
         return cls(head_dim, inv_freq=rotary_emb.inv_freq,
                    attention_scaling=getattr(rotary_emb, "attention_scaling", 1.0))
 

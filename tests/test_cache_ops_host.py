@@ -61,6 +61,45 @@ def test_dynamic_and_longrope():
     assert scale == pytest.approx(math.sqrt(1 + math.log(16) / math.log(4096)))
 
 
+@pytest.mark.parametrize("kind,extra", [
+    ("dynamic", dict(factor=2.0)),
+    ("longrope", dict(factor=4.0, short_factor=[1.0] * 32, long_factor=[2.0] * 32, original_max_position_embeddings=512)),
+])
+def test_modules_that_change_with_the_length_are_refused(kind, extra):
+    transformers = pytest.importorskip("transformers")
+    from transformers.models.llama.modeling_llama import LlamaRotaryEmbedding
+    cfg = transformers.LlamaConfig(hidden_size=128, num_attention_heads=2, head_dim=64,
+                                   max_position_embeddings=512 if kind == "dynamic" else 2048,
+                                   rope_parameters=dict(rope_type=kind, rope_theta=1e4, **extra))
+    module = LlamaRotaryEmbedding(cfg)
+    before = module.inv_freq.clone()
+    with pytest.raises(ValueError, match="seq_len"):
+        Rotary.from_module(module, 64)
+    module(torch.zeros(1, 2048, 128), torch.arange(2048)[None])
+    assert not torch.equal(module.inv_freq, before)  # the reason
+    with pytest.raises(ValueError, match="seq_len"):
+        Rotary.from_module(module, 64)
+    if kind == "dynamic":  # one length's angles, in float: as the comparison with the model's own above
+        r = Rotary(64, base=1e4, scaling=dict(extra, rope_type=kind, original_max_position_embeddings=512), seq_len=2048,
+                   device="cpu")
+        np.testing.assert_allclose(r.inv_freq.numpy(), module.inv_freq.double().numpy(), rtol=32 * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("kind,extra", [
+    ("default", {}), ("linear", dict(factor=4.0)),
+    ("llama3", dict(factor=8.0, low_freq_factor=1.0, high_freq_factor=4.0, original_max_position_embeddings=512)),
+    ("yarn", dict(factor=4.0, original_max_position_embeddings=512)),
+])
+def test_modules_with_fixed_angles(kind, extra):
+    transformers = pytest.importorskip("transformers")
+    from transformers.models.llama.modeling_llama import LlamaRotaryEmbedding
+    cfg = transformers.LlamaConfig(hidden_size=128, num_attention_heads=2, head_dim=64, max_position_embeddings=2048,
+                                   rope_parameters=dict(rope_type=kind, rope_theta=1e4, **extra))
+    module = LlamaRotaryEmbedding(cfg)
+    r = Rotary.from_module(module, 64)
+    assert torch.equal(r.inv_freq, module.inv_freq.double()) and r.attention_scaling == module.attention_scaling
+
+
 def test_rotary_refusals():
     for bad in (dict(rotary_dim=7), dict(rotary_dim=0), dict(rotary_dim=72), dict(offset=-1),
                 dict(rotary_dim=64, offset=1), dict(base=0.0), dict(scaling={"rope_type": "none such"}),
