@@ -72,6 +72,56 @@ static cudaError_t launch(bool pdl, void (*kernel)(KArgs...), dim3 grid, dim3 bl
         MENTAT_CHECK_LAUNCH();                                           \
     } while (0)
 
+// The most dynamic shared memory that a kernel may be launched with, set once for each device to what the device
+// has beside the kernel's static one.  The limit is the kernel's, not the launch's: a call that set it to its own size could
+// lower it between another host thread's setting and launch, whose launch would then be refused.
+template <auto KERNEL>
+static cudaError_t reserve_smem() {
+    static std::atomic<bool> done[64] = {};
+    int dev = 0, most = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64 && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+    cudaFuncAttributes f;
+    if ((e = cudaFuncGetAttributes(&f, KERNEL)) != cudaSuccess ||
+        (e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev)) != cudaSuccess ||
+        (e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)f.sharedSizeBytes)) !=
+            cudaSuccess)
+        return e;
+    if (dev < 64) done[dev].store(true, std::memory_order_release);
+    return cudaSuccess;
+}
+
+// KERNEL over clusters of cs CTAs, as a status: counted, with programmatic stream serialization as launch().
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_ex(const cudaLaunchConfig_t* cfg, void (*kernel)(KArgs...), Args... args) {
+    return cudaLaunchKernelEx(cfg, kernel, static_cast<KArgs>(args)...);
+}
+template <auto KERNEL, typename... Args>
+static int launch_cluster(int cs, dim3 grid, int threads, size_t smem, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cs;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    if (reserve_smem<KERNEL>() != cudaSuccess ||
+        (cs > 8 && cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
+        launch_ex(&cfg, KERNEL, args...) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return MENTAT_ERR_CUDA;
+    }
+    MENTAT_CHECK_LAUNCH();
+    return MENTAT_OK;
+}
+
 // device timeline of one call (trace builds only): nanosecond stamps, first and
 // last over the CTAs of a kernel
 #ifdef MENTAT_TC_TRACE

@@ -856,29 +856,9 @@ static int chunks_of(int64_t work, int64_t each, int64_t most) {
 }
 
 // a kernel over one cluster of CLUSTER_CTAS
-template <typename... KArgs, typename... Args>
-static int launch_one_cluster(void (*kernel)(KArgs...), size_t smem, cudaStream_t s, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(CLUSTER_CTAS);
-    cfg.blockDim = dim3(CLUSTER_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = CLUSTER_CTAS;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    if ((smem > 40 * 1024 &&
-         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) ||
-        cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...) != cudaSuccess) {
-        (void)cudaGetLastError();
-        return MENTAT_ERR_CUDA;
-    }
-    MENTAT_CHECK_LAUNCH();
-    return MENTAT_OK;
+template <auto KERNEL, typename... Args>
+static int launch_one_cluster(size_t smem, cudaStream_t s, Args... args) {
+    return launch_cluster<KERNEL>(CLUSTER_CTAS, dim3(CLUSTER_CTAS), CLUSTER_THREADS, smem, s, args...);
 }
 
 // Releases are one cluster's work while a warp has at most this many groups of 32 table entries.  One launch instead
@@ -896,7 +876,7 @@ static int launch_free(const mentat_kv_cache* c, const int32_t* slots, const int
     const int64_t per = ((int64_t)rows * chunks + CLUSTER_ALL_WARPS - 1) / CLUSTER_ALL_WARPS;
     const size_t held = (size_t)CLUSTER_WARPS * per * 32 * 4;
     if (per <= FREE_CLUSTER_PER && held + bitmap_bytes(c) <= 100 * 1024)
-        return launch_one_cluster(k_free_cluster<LEAD>, held + bitmap_bytes(c), s, *c, slots, cu, n, chunks, (int)per, w);
+        return launch_one_cluster<k_free_cluster<LEAD>>(held + bitmap_bytes(c), s, *c, slots, cu, n, chunks, (int)per, w);
     const dim3 clear(chunks_of(c->num_blocks, 1024, 148)), by_row((rows + PAGES_WARPS - 1) / PAGES_WARPS);
     if (!LEAD)
         MENTAT_LAUNCH(k_pages_begin, clear, dim3(256), bitmap_bytes(c), s, *c, slots, n, (int)by_row.x, w);
@@ -910,6 +890,8 @@ static int launch_free(const mentat_kv_cache* c, const int32_t* slots, const int
 }
 
 namespace {
+// The launch that moves the rows.  With `ready`, only what may refuse it: asked before the plan, whose fresh blocks
+// would belong to no table if the rows could not be moved.
 struct LaunchCompactMove {
     const mentat_kv_cache& c;
     const CompactArgs& a;
@@ -917,6 +899,13 @@ struct LaunchCompactMove {
     const PagesWs& w;
     int max_keep;
     cudaStream_t s;
+    bool ready;
+    template <auto KERNEL>
+    static int reserve() {
+        if (reserve_smem<KERNEL>() == cudaSuccess) return MENTAT_OK;
+        (void)cudaGetLastError();
+        return MENTAT_ERR_CUDA;
+    }
     template <typename T, int VEC, bool IL>
     int operator()() {
         const int64_t rows = (int64_t)a.n * c.num_layers, most = rows * ((max_keep + c.block_size - 1) / c.block_size);
@@ -934,21 +923,13 @@ struct LaunchCompactMove {
                 const size_t smem = stages * stage + table;
                 int per_sm = (int)(220 * 1024 / (smem + 2048));
                 per_sm = per_sm < 1 ? 1 : per_sm > 6 ? 6 : per_sm;
-                const auto kernel = k_compact_stream<T, VEC, IL>;
-                if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
-                    (void)cudaGetLastError();
-                    return MENTAT_ERR_CUDA;
-                }
-                MENTAT_LAUNCH(kernel, dim3(chunks_of(most, 1, 148 * per_sm)), dim3(STREAM_THREADS), smem, s, c, a, r, tokens,
+                if (ready) return reserve<k_compact_stream<T, VEC, IL>>();
+                MENTAT_LAUNCH((k_compact_stream<T, VEC, IL>), dim3(chunks_of(most, 1, 148 * per_sm)), dim3(STREAM_THREADS), smem, s, c, a, r, tokens,
                               stages, w);
                 return MENTAT_OK;
             }
         }
-        if (table > 40 * 1024 && cudaFuncSetAttribute(k_compact_move<T, IL>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                      (int)table) != cudaSuccess) {
-            (void)cudaGetLastError();
-            return MENTAT_ERR_CUDA;
-        }
+        if (ready) return reserve<k_compact_move<T, IL>>();
         MENTAT_LAUNCH((k_compact_move<T, IL>), dim3(chunks_of(most, 1, 148 * 8)), dim3(MOVE_THREADS), table, s, c, a, r, w);
         return MENTAT_OK;
     }
@@ -1000,9 +981,17 @@ int mentat_kv_compact(const mentat_kv_cache* c, const int32_t* src, const int32_
     const bool wide = c->head_dim % vec == 0 && (!r || rotary_aligned(r, c->head_dim, vec)) &&
                       ((uintptr_t)c->k_pool | (uintptr_t)c->v_pool) % 16 == 0;
     const CompactArgs a{src, dst, keep, keep_ls, total, cu, n};
-    int st = launch_one_cluster(k_compact_plan, bitmap_bytes(c), s, *c, a, chunks_of(max_keep, PLAN_CHUNK, 1 << 20), w);
+    const auto move = [&](bool ready) {
+        return rotary_dispatch(c->dtype, wide, turn.interleaved != 0, LaunchCompactMove{*c, a, turn, w, max_keep, s, ready});
+    };
+    if (!dst && reserve_smem<k_free_cluster<true>>() != cudaSuccess) {
+        (void)cudaGetLastError();
+        return MENTAT_ERR_CUDA;
+    }
+    int st = move(true);
     if (st == MENTAT_OK)
-        st = rotary_dispatch(c->dtype, wide, turn.interleaved != 0, LaunchCompactMove{*c, a, turn, w, max_keep, s});
+        st = launch_one_cluster<k_compact_plan>(bitmap_bytes(c), s, *c, a, chunks_of(max_keep, PLAN_CHUNK, 1 << 20), w);
+    if (st == MENTAT_OK) st = move(false);
     return st != MENTAT_OK || dst ? st : launch_free<true>(c, src, cu, n, max_nb, w, s);
 }
 

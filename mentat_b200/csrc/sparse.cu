@@ -1436,34 +1436,6 @@ static bool sparse_listed(const mentat_kv_cache* c, int n, int max_len, int budg
     return pages > HELD_PAGES || pages > 600 * sparse_cluster(n * c->num_kv_heads);
 }
 
-// A kernel over clusters of cs CTAs.
-template <typename... KArgs, typename... Args>
-static int launch_cluster(void (*kernel)(KArgs...), int cs, dim3 grid, int threads, size_t smem, cudaStream_t s,
-                          Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = cs;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    if ((smem > 40 * 1024 &&
-         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) ||
-        (cs > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
-        cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...) != cudaSuccess) {
-        (void)cudaGetLastError();
-        return MENTAT_ERR_CUDA;
-    }
-    MENTAT_CHECK_LAUNCH();
-    return MENTAT_OK;
-}
-
 template <typename T, int D, int GM, bool MMA, bool LISTED>
 static int launch_sparse(const mentat_kv_cache* c, const mentat_page_index* x, SparseArgs a, cudaStream_t s) {
     const int pages = (a.max_len + c->block_size - 1) / c->block_size, cs = sparse_cluster(a.n * c->num_kv_heads);
@@ -1472,8 +1444,8 @@ static int launch_sparse(const mentat_kv_cache* c, const mentat_page_index* x, S
     const size_t smem = 4 * (size_t)sparse_smem(a.G, GM, D, MMA, LISTED, a.held, a.share).total + 1024;
     CUtensorMap mk{}, mv{};
     if (MMA && !pool_maps(c, a.layer, &mk, &mv)) return MENTAT_ERR_CUDA;
-    return launch_cluster(k_sparse<T, D, GM, MMA, LISTED>, cs, dim3(c->num_kv_heads * cs, a.n), 32 * sparse_warps(MMA), smem, s,
-                          mk, mv, *c, *x, a);
+    return launch_cluster<k_sparse<T, D, GM, MMA, LISTED>>(cs, dim3(c->num_kv_heads * cs, a.n), 32 * sparse_warps(MMA), smem,
+                                                           s, mk, mv, *c, *x, a);
 }
 
 // 16-bit types with pages of 16 rows or a multiple run on tensor cores
@@ -1525,8 +1497,9 @@ static int launch_sparse_dim(const mentat_kv_cache* c, const mentat_page_index* 
     int cs = 1;
     while (cs < SPARSE_MAX_CLUSTER && (pages + cs - 1) / cs > HELD_PAGES) cs *= 2;
     const size_t smem = 4 * (size_t)((pages + cs - 1) / cs + 3);
-    const int st = launch_cluster(cs > 1 ? k_choose<true> : k_choose<false>, cs, dim3(c->num_kv_heads * cs, a.n),
-                                  CHOOSE_THREADS, smem, s, *c, a);
+    const dim3 grid(c->num_kv_heads * cs, a.n);
+    const int st = cs > 1 ? launch_cluster<k_choose<true>>(cs, grid, CHOOSE_THREADS, smem, s, *c, a)
+                          : launch_cluster<k_choose<false>>(1, grid, CHOOSE_THREADS, smem, s, *c, a);
     if (st != MENTAT_OK) return st;
     return launch_sparse_group<T, D, true>(c, x, a, s);
 }
