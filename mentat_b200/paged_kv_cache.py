@@ -452,25 +452,51 @@ class PagedKVCacheManager:
         self._cache.clear()
         self._after()
 
+    def _new_sequence(self, num_tokens, tokens_in_last_block, num_blocks) -> int:
+        sid = self._next_seq_id
+        self._next_seq_id += 1
+        self._sequences[sid] = SequenceState(sid, self.num_layers, self._free_slots.pop(), num_tokens,
+                                             tokens_in_last_block, num_blocks)
+        return sid
+
+    def _release(self, seqs) -> None:
+        """Frees sequences on the device and forgets them."""
+        step = ops.MAX_SEQS_PER_PAGES_CALL
+        for a in range(0, len(seqs), step):
+            part = seqs[a: a + step]
+            ops.free_pages(self, self._upload([s.slot for s in part]), max(max(s.num_blocks) for s in part))
+            for s in part:
+                del self._sequences[s.seq_id]
+                self._free_slots.append(s.slot)
+        self._cache.clear()
+
+    def _take_back(self, ids, launched: int) -> None:
+        """Removes the new sequences of a call that failed: the caller has no ids of them.  The device has begun with
+        the first ``launched``."""
+        for c in reversed(ids[launched:]):
+            self._free_slots.append(self._sequences.pop(c).slot)
+        self._release([self._sequences[c] for c in reversed(ids[:launched])])
+
     def fork_sequences(self, parent_ids) -> list:
         """``[fork_sequence(p) for p in parent_ids]`` in one launch (a parent may occur
-        several times).  An unknown id or a lack of slots raises before any change."""
+        several times).  An unknown id or a lack of slots raises before any change; if the
+        call fails later, no child is left."""
         parents = [self._sequences[p] for p in parent_ids]
         if len(parents) > len(self._free_slots):
             raise RuntimeError(f"PagedKVCache: out of sequence slots (max_seqs={self.max_seqs})")
-        kids = []
-        for p in parents:
-            cid = self._next_seq_id
-            self._next_seq_id += 1
-            self._sequences[cid] = SequenceState(cid, self.num_layers, self._free_slots.pop(), list(p.num_tokens),
-                                                 list(p.tokens_in_last_block), list(p.num_blocks))
-            kids.append(cid)
-        for a in range(0, len(parents), ops.MAX_SEQS_PER_PAGES_CALL):
-            part = slice(a, a + ops.MAX_SEQS_PER_PAGES_CALL)
-            both = self._upload([p.slot for p in parents[part]] + [self._sequences[c].slot for c in kids[part]])
-            n = both.numel() // 2
-            ops.fork_pages(self, both[:n], both[n:])
-        self._after()
+        kids = [self._new_sequence(list(p.num_tokens), list(p.tokens_in_last_block), list(p.num_blocks)) for p in parents]
+        done = 0
+        try:
+            for a in range(0, len(parents), ops.MAX_SEQS_PER_PAGES_CALL):
+                part = slice(a, a + ops.MAX_SEQS_PER_PAGES_CALL)
+                both = self._upload([p.slot for p in parents[part]] + [self._sequences[c].slot for c in kids[part]])
+                n = both.numel() // 2
+                ops.fork_pages(self, both[:n], both[n:])
+                done = a + n
+            self._after()
+        except Exception:
+            self._take_back(kids, done)
+            raise
         return kids
 
     def free_sequences(self, seq_ids) -> None:
@@ -480,13 +506,7 @@ class PagedKVCacheManager:
         seqs = [self._sequences[s] for s in ids]
         if len(set(ids)) < len(ids):
             raise KeyError(next(s for i, s in enumerate(ids) if s in ids[:i]))
-        for a in range(0, len(seqs), ops.MAX_SEQS_PER_PAGES_CALL):
-            part = seqs[a: a + ops.MAX_SEQS_PER_PAGES_CALL]
-            ops.free_pages(self, self._upload([s.slot for s in part]), max(max(s.num_blocks) for s in part))
-        for s in seqs:
-            del self._sequences[s.seq_id]
-            self._free_slots.append(s.slot)
-        self._cache.clear()
+        self._release(seqs)
         self._after()
 
     def compact_sequences(self, seq_ids, keep, *, rotary=None, into_new: bool = False):
@@ -512,6 +532,8 @@ class PagedKVCacheManager:
             raise KeyError(next(s for i, s in enumerate(ids) if s in ids[:i]))
         if into_new and len(ids) > len(self._free_slots):
             raise RuntimeError(f"PagedKVCache: out of sequence slots (max_seqs={self.max_seqs})")
+        if rotary is not None:
+            ops._check_rotary(rotary, self.head_dim, self.device)
         L, bs = self.num_layers, self.block_size
         on_device = any(isinstance(k, torch.Tensor) and k.device.type != "cpu" for k in keep)
         lists, counts, per_layer = [], [], False
@@ -545,37 +567,36 @@ class PagedKVCacheManager:
             per_layer |= ndim == 2
             lists.append(k)
             counts.append(m)
-        out = []
-        for seq, m in zip(seqs, counts):
+        def state(m):  # of a sequence of m tokens
             nb = -(-m // bs)
-            new = ([m] * L, [m - (nb - 1) * bs if m else 0] * L, [nb] * L)
-            if into_new:
-                cid = self._next_seq_id
-                self._next_seq_id += 1
-                self._sequences[cid] = SequenceState(cid, L, self._free_slots.pop(), *new)
-                out.append(cid)
-        step = ops.MAX_SEQS_PER_PAGES_CALL
-        for a in range(0, len(seqs), step):
-            part, ks, cs = seqs[a: a + step], lists[a: a + step], counts[a: a + step]
-            if per_layer:
-                ks = [k.expand(L, -1) if on_device and k.dim() == 1 else
-                      np.broadcast_to(k, (L, k.shape[-1])) if not on_device else k for k in ks]
-            flat = torch.cat(ks, dim=-1) if on_device else \
-                self._upload(np.concatenate(ks, axis=-1)).view((L, -1) if per_layer else (-1,))
-            slots = self._upload([s.slot for s in part])
-            dst = self._upload([self._sequences[c].slot for c in out[a: a + step]]) if into_new else None
-            cu = self._upload(np.concatenate([[0], np.cumsum(cs)]))
-            ops.compact_pages(self, slots, dst, flat, cu, max(cs), rotary=rotary,
-                              max_blocks=max(max(s.num_blocks) for s in part))
-            if self.page_index is not None and max(cs) >= bs:
-                ops.index_sequences(self, slots if dst is None else dst, 0, max(cs) // bs)
-        if not into_new:
-            for seq, m in zip(seqs, counts):
-                nb = -(-m // bs)
-                seq.num_tokens, seq.num_blocks = [m] * L, [nb] * L
-                seq.tokens_in_last_block = [m - (nb - 1) * bs if m else 0] * L
-        self._cache.clear()
-        self._after()
+            return [m] * L, [m - (nb - 1) * bs if m else 0] * L, [nb] * L
+
+        out = [self._new_sequence(*state(m)) for m in counts] if into_new else []
+        step, done = ops.MAX_SEQS_PER_PAGES_CALL, 0
+        try:
+            for a in range(0, len(seqs), step):
+                part, ks, cs = seqs[a: a + step], lists[a: a + step], counts[a: a + step]
+                if per_layer:
+                    ks = [k.expand(L, -1) if on_device and k.dim() == 1 else
+                          np.broadcast_to(k, (L, k.shape[-1])) if not on_device else k for k in ks]
+                flat = torch.cat(ks, dim=-1) if on_device else \
+                    self._upload(np.concatenate(ks, axis=-1)).view((L, -1) if per_layer else (-1,))
+                slots = self._upload([s.slot for s in part])
+                dst = self._upload([self._sequences[c].slot for c in out[a: a + step]]) if into_new else None
+                cu = self._upload(np.concatenate([[0], np.cumsum(cs)]))
+                ops.compact_pages(self, slots, dst, flat, cu, max(cs), rotary=rotary,
+                                  max_blocks=max(max(s.num_blocks) for s in part))
+                done = a + len(part)
+                if not into_new:
+                    for seq, m in zip(part, cs):
+                        seq.num_tokens, seq.tokens_in_last_block, seq.num_blocks = state(m)
+                if self.page_index is not None and max(cs) >= bs:
+                    ops.index_sequences(self, slots if dst is None else dst, 0, max(cs) // bs)
+            self._cache.clear()
+            self._after()
+        except Exception:
+            self._take_back(out, done)
+            raise
         return out if into_new else None
 
     def _upload(self, values) -> torch.Tensor:

@@ -421,3 +421,65 @@ def test_rotated_appends(dtype, d, rd, il, bs):
             check_q(m.append_rotated_batched(batch, layer, tq, tk, tv, rot), q, pos)
             o.append_tokens_batched(batch, layer, turn(k, pos, f, interleaved=il), v)
     same(m, o, lambda want: 1.5 * turn_tolerance(want, f, eps, interleaved=il)(want))
+
+
+def test_failed_batches_leave_no_sequence(monkeypatch):
+    """A call that fails after its new sequences have slots (another model's rotary, a launch that is refused, too few
+    blocks) leaves the host's mirror, the slots and the device as they were, whatever part of it had run."""
+    from mentat_b200 import Rotary, ops
+    rng = np.random.default_rng(21)
+    m, o = pair(L=2, d=64, pool=40, max_seqs=9)
+    a, b = start(m, o, [33, 9], rng)  # 24 of 40 blocks
+    slots = list(m._free_slots)
+
+    def unchanged(exc, call, **kw):
+        with pytest.raises(exc, **kw):
+            call()
+        m.clear_error()
+        assert m._free_slots == slots and sorted(m._sequences) == [a, b]
+        same(m, o)
+    for new in (False, True):
+        unchanged(ValueError, lambda: m.compact_sequences([a], [[1, 2]], rotary=Rotary(128), into_new=new), match="heads of 128")
+    # 17 fresh blocks a layer do not fit; nor, in the second call, does what the first one's chunk left
+    unchanged(RuntimeError, lambda: m.compact_sequences([a, a], [list(range(32, 0, -1))] * 2, into_new=True), match="out of blocks")
+
+    def refuse_at(name, k):
+        real, calls = getattr(ops, name), []
+
+        def call(*args, **kw):
+            calls.append(0)
+            if len(calls) == k:
+                raise RuntimeError("refused on the host")
+            return real(*args, **kw)
+        monkeypatch.setattr(ops, name, call)
+        return real
+    monkeypatch.setattr(ops, "MAX_SEQS_PER_PAGES_CALL", 2)
+    for k in (1, 2):
+        real = refuse_at("fork_pages", k)
+        with pytest.raises(RuntimeError, match="refused"):
+            m.fork_sequences([a, b, a, b])
+        monkeypatch.setattr(ops, "fork_pages", real)
+        assert sorted(m._free_slots) == sorted(slots) and sorted(m._sequences) == [a, b]
+        same(m, o)  # (forks and their releases leave the free list as it was)
+    slots = list(m._free_slots)
+    for new in (False, True):
+        real = refuse_at("compact_pages", 1)
+        unchanged(RuntimeError, lambda: m.compact_sequences([a], [[1, 2]], into_new=new), match="refused")
+        monkeypatch.setattr(ops, "compact_pages", real)
+    # in place, the second part refused: the first is compacted, on the host too
+    real = refuse_at("compact_pages", 2)
+    c = m.allocate_sequence()
+    assert c > b
+    while o.allocate_sequence() < c:  # the ids that failed calls used up
+        pass
+    for sid in [s for s in o._sequences if s not in (a, b, c)]:
+        o.free_sequence(sid)
+    with pytest.raises(RuntimeError, match="refused"):
+        m.compact_sequences([a, b, c], [[3, 2, 1], [8], []])
+    monkeypatch.setattr(ops, "compact_pages", real)
+    compact(o, [a, b], [np.array([3, 2, 1]), np.array([8])])
+    same(m, o)
+    # and what succeeds in several parts
+    kids = m.fork_sequences([a, b, a])
+    m.free_sequences([kids[2], kids[0], kids[1]])
+    same(m, o)
