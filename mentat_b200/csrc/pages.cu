@@ -846,9 +846,11 @@ static bool bad_pages(const mentat_kv_cache* c, int32_t n) {
            !c->tables || !c->nblocks || !c->ntok || !c->tail || n < 0 || n > PAGES_MAX_SEQS;
 }
 static size_t bitmap_bytes(const mentat_kv_cache* c) { return ((size_t)c->max_seqs + 31) / 32 * 4; }
-// the bitmap fits in shared memory, and a release's index in 32 bits
+// the bitmap fits in shared memory
+static bool slots_fit(const mentat_kv_cache* c) { return bitmap_bytes(c) <= 48 * 1024; }
+// and a release's index in 32 bits
 static bool pages_fit(const mentat_kv_cache* c, int32_t n) {
-    return bitmap_bytes(c) <= 48 * 1024 && (int64_t)n * c->num_layers * c->max_blocks_per_seq < 0xffffffffll;
+    return slots_fit(c) && (int64_t)n * c->num_layers * c->max_blocks_per_seq < 0xffffffffll;
 }
 static int chunks_of(int64_t work, int64_t each, int64_t most) {
     const int64_t x = (work + each - 1) / each;
@@ -945,7 +947,7 @@ int64_t mentat_pages_workspace_bytes(const mentat_kv_cache* c, int32_t n) {
 int mentat_kv_fork_batched(const mentat_kv_cache* c, const int32_t* parents, const int32_t* children, int32_t n, cudaStream_t s) {
     if (bad_pages(c, n) || (n > 0 && (!parents || !children))) return MENTAT_ERR_ARG;
     if (n == 0) return MENTAT_OK;
-    if (!pages_fit(c, n)) return MENTAT_ERR_UNSUPPORTED;
+    if (!slots_fit(c)) return MENTAT_ERR_UNSUPPORTED;
     const dim3 grid((n + PAGES_WARPS - 1) / PAGES_WARPS, c->num_layers);
     MENTAT_LAUNCH(k_fork_batched, grid, dim3(PAGES_THREADS), bitmap_bytes(c), s, *c, parents, children, n);
     return MENTAT_OK;

@@ -452,6 +452,10 @@ class PagedKVCacheManager:
         self._cache.clear()
         self._after()
 
+    def _pages_step(self) -> int:
+        """Sequences of one call of the batched page operators (they number the releases of a call in 32 bits)."""
+        return max(1, min(ops.MAX_SEQS_PER_PAGES_CALL, 0xfffffffe // (self.num_layers * self._table_stride)))
+
     def _new_sequence(self, num_tokens, tokens_in_last_block, num_blocks) -> int:
         sid = self._next_seq_id
         self._next_seq_id += 1
@@ -461,7 +465,7 @@ class PagedKVCacheManager:
 
     def _release(self, seqs) -> None:
         """Frees sequences on the device and forgets them."""
-        step = ops.MAX_SEQS_PER_PAGES_CALL
+        step = self._pages_step()
         for a in range(0, len(seqs), step):
             part = seqs[a: a + step]
             ops.free_pages(self, self._upload([s.slot for s in part]), max(max(s.num_blocks) for s in part))
@@ -572,7 +576,7 @@ class PagedKVCacheManager:
             return [m] * L, [m - (nb - 1) * bs if m else 0] * L, [nb] * L
 
         out = [self._new_sequence(*state(m)) for m in counts] if into_new else []
-        step, done = ops.MAX_SEQS_PER_PAGES_CALL, 0
+        step, done = self._pages_step(), 0
         try:
             for a in range(0, len(seqs), step):
                 part, ks, cs = seqs[a: a + step], lists[a: a + step], counts[a: a + step]

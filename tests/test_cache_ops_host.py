@@ -220,6 +220,22 @@ def test_c_abi_refuses_page_arguments():
     assert compact(rot=C.byref(_lib.Rotary(4096, 33, 0, 0, 0, 1.0))) == ARG
 
 
+def test_batches_are_split_where_a_call_cannot_take_them():
+    """Releases of one call are numbered in 32 bits; a fork has no such limit."""
+    from types import SimpleNamespace
+
+    from mentat_b200 import PagedKVCacheManager
+    lib = _lib.load()
+    for layers, cap in ((80, 65536), (64, 1 << 20), (2, 16), (126, 33333332)):
+        step = PagedKVCacheManager._pages_step(SimpleNamespace(num_layers=layers, _table_stride=cap))
+        d = _desc(num_layers=layers, max_blocks_per_seq=cap)
+        assert lib.mentat_kv_free_batched(d, 4096, step, 1, 4096, 0, None) == ARG  # only its workspace is missing
+        if step < 1024:
+            assert lib.mentat_kv_free_batched(d, 4096, step + 1, 1, 4096, 0, None) == UNSUPPORTED
+        else:
+            assert step == 1024
+
+
 def test_c_abi_refuses_sparse_arguments():
     lib = _lib.load()
     x = _lib.PageIndex(4096, 4096)
