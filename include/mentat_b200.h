@@ -372,8 +372,8 @@ int mentat_kv_append_rotated(const mentat_kv_cache* c, int32_t layer, int32_t sl
  * twice, changes nothing and records MENTAT_DEV_BAD_SLOT.
  */
 /* fork_sequence (paged_kv_cache.py:152-170) of parents[i] into children[i].
- * The children are distinct and none is also a parent; a parent may have
- * several. */
+ * The children are distinct and empty (in every layer) and none is also a
+ * parent; a parent may have several. */
 int mentat_kv_fork_batched(const mentat_kv_cache* c, const int32_t* parents, const int32_t* children, int32_t n,
                            cudaStream_t s);
 

@@ -77,31 +77,44 @@ __device__ __forceinline__ bool has_bit(const uint32_t* bits, int s) { return (b
 // ---------------------------------------------------------------------------
 // fork
 // ---------------------------------------------------------------------------
-// Every CTA checks the whole batch for itself, so all of them agree whether to go on.  A warp takes one
-// (layer, run of children of one parent that follow one another): the parent's table is read once and each
-// page's count rises by the run's length in one atomic.
+// The batch is checked in a launch before: no CTA of the fork could see whether a child is empty, since another one may
+// have filled it.  What is wrong is recorded, and the fork does nothing after an error.  CTA 0 looks at the slots, all of them at
+// the children's counters.
 constexpr int PAGES_THREADS = 256, PAGES_WARPS = PAGES_THREADS / 32;
-__global__ void __launch_bounds__(PAGES_THREADS) k_fork_batched(mentat_kv_cache c, const int32_t* parents,
-                                                                const int32_t* children, int n) {
+__global__ void __launch_bounds__(PAGES_THREADS) k_fork_check(mentat_kv_cache c, const int32_t* parents,
+                                                              const int32_t* children, int n) {
     extern __shared__ uint32_t bits[];
     __shared__ int s_bad;
     griddep_wait();
     griddep_launch();
-    const bool ok = slots_distinct(c, children, n, bits, &s_bad);
-    int no = 0;
-    if (ok)
-        for (int i = threadIdx.x; i < n; i += blockDim.x) {
-            const int p = parents[i];
-            if (p < 0 || p >= c.max_seqs || has_bit(bits, p)) {
-                no = 1;
-                s_bad = p;
-            }
-        }
-    if (__syncthreads_or(no) || !ok) {
+    for (int64_t x = blockIdx.x * (int64_t)PAGES_THREADS + threadIdx.x; x < (int64_t)n * c.num_layers;
+         x += (int64_t)gridDim.x * PAGES_THREADS) {
+        const int s = children[x % n];
+        if (s < 0 || s >= c.max_seqs) continue;
+        const int64_t si = seq_index(c, (int)(x / n), s);
+        if (c.nblocks[si] || c.ntok[si]) set_error(c, MENTAT_DEV_BAD_SLOT, s);
+    }
+    if (blockIdx.x) return;
+    if (!slots_distinct(c, children, n, bits, &s_bad)) {
         if (threadIdx.x == 0) set_error(c, MENTAT_DEV_BAD_SLOT, s_bad);
         return;
     }
-    if (has_error(c)) return;
+    for (int i = threadIdx.x; i < n; i += PAGES_THREADS) {
+        const int p = parents[i];
+        if (p < 0 || p >= c.max_seqs || has_bit(bits, p)) set_error(c, MENTAT_DEV_BAD_SLOT, p);
+    }
+}
+
+// A warp takes one (layer, run of children of one parent that follow one another): the parent's table is read once
+// and each page's count rises by the run's length in one atomic.
+__global__ void __launch_bounds__(PAGES_THREADS) k_fork_batched(mentat_kv_cache c, const int32_t* parents,
+                                                                const int32_t* children, int n) {
+    __shared__ int s_stop;
+    griddep_wait();
+    griddep_launch();
+    if (threadIdx.x == 0) s_stop = has_error(c);
+    __syncthreads();
+    if (s_stop) return;
     const int lane = threadIdx.x & 31, l = blockIdx.y, i = blockIdx.x * PAGES_WARPS + (threadIdx.x >> 5);
     if (i >= n) return;
     const int parent = parents[i];
@@ -949,7 +962,9 @@ int mentat_kv_fork_batched(const mentat_kv_cache* c, const int32_t* parents, con
     if (n == 0) return MENTAT_OK;
     if (!slots_fit(c)) return MENTAT_ERR_UNSUPPORTED;
     const dim3 grid((n + PAGES_WARPS - 1) / PAGES_WARPS, c->num_layers);
-    MENTAT_LAUNCH(k_fork_batched, grid, dim3(PAGES_THREADS), bitmap_bytes(c), s, *c, parents, children, n);
+    MENTAT_LAUNCH(k_fork_check, dim3(chunks_of((int64_t)n * c->num_layers, 4 * PAGES_THREADS, 148)), dim3(PAGES_THREADS),
+                  bitmap_bytes(c), s, *c, parents, children, n);
+    MENTAT_LAUNCH(k_fork_batched, grid, dim3(PAGES_THREADS), 0, s, *c, parents, children, n);
     return MENTAT_OK;
 }
 

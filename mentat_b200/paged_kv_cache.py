@@ -390,8 +390,17 @@ class PagedKVCacheManager:
         raise_device_error(err, arg, self.max_blocks, self.max_blocks_per_seq)
 
     def clear_error(self) -> None:
-        """Forget the recorded device error (after the caller has handled it)."""
+        """Forget the recorded device error (after the caller has handled it).  Sequences that were freed in the
+        meantime, when the device did nothing, are released now, so that every free slot is empty."""
         self._ctrl[_lib.CTRL_ERROR:_lib.CTRL_ERRARG + 1].zero_()
+        held = (self._nblocks != 0).any(dim=0).tolist()
+        left = [s for s in self._free_slots if held[s]]
+        if left:
+            step = self._pages_step()
+            for a in range(0, len(left), step):
+                ops.free_pages(self, self._upload(left[a: a + step]))
+            # pages that the error had left wrong are part of what the caller has handled
+            self._ctrl[_lib.CTRL_ERROR:_lib.CTRL_ERRARG + 1].zero_()
 
     def _after(self):
         if self.strict:

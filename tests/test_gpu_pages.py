@@ -483,3 +483,61 @@ def test_failed_batches_leave_no_sequence(monkeypatch):
     kids = m.fork_sequences([a, b, a])
     m.free_sequences([kids[2], kids[0], kids[1]])
     same(m, o)
+
+
+def test_fork_into_a_slot_in_use_changes_nothing():
+    """A child that has pages, one that has tokens in one layer alone, among children that are empty: recorded, and no
+    table, count or child of the batch has changed."""
+    from mentat_b200 import ops
+    rng = np.random.default_rng(22)
+    m, o = pair(L=3, pool=400, max_seqs=300, strict=False)
+    a, b = start(m, o, [45, 7], rng)
+    c = m.allocate_sequence()
+    assert c == o.allocate_sequence()
+    k, v = (round_np(rng.standard_normal((2, 2, 64), dtype=np.float32), "bf16") for _ in range(2))
+    m.append_tokens(c, 2, *(torch.from_numpy(t).cuda().to(m.dtype) for t in (k, v)))  # its last layer alone
+    o.append_tokens(c, 2, k, v)
+    sa, sb, sc = (m._sequences[s].slot for s in (a, b, c))
+    empty = m._free_slots[::-1]
+    for used in (sb, sc):
+        for n, at in ((1, 0), (9, 8), (200, 77)):
+            kids = empty[:n]
+            kids[at] = used
+            ops.fork_pages(m, *(torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([sa] * n, kids)))
+            with pytest.raises(ValueError, match=f"slot {used} "):
+                m.check()
+            m.clear_error()
+            assert not m._nblocks[:, empty].any() and not m._ntok[:, empty].any()
+            same(m, o)
+    # the slots that were empty take the same batch
+    n = 200
+    ops.fork_pages(m, *(torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([sa] * n, empty[:n])))
+    ops.free_pages(m, torch.tensor(empty[:n], dtype=torch.int32, device="cuda"))
+    m.check()
+    same(m, o)
+
+
+def test_slots_freed_after_an_error_are_empty_when_it_is_cleared():
+    """A free after an error does nothing on the device; clearing the error makes up for it, so the slot can be forked
+    into and no page is lost."""
+    rng = np.random.default_rng(23)
+    m, o = pair(L=2, pool=60, strict=False)
+    a, b, c = start(m, o, [21, 9, 13], rng)
+    kid = m.fork_sequence(a)
+    assert kid == o.fork_sequence(a)
+    from mentat_b200 import ops
+    ops.free_pages(m, torch.tensor([-1], dtype=torch.int32, device="cuda"))
+    m.free_sequence(b)
+    m.free_sequences([kid, c])
+    with pytest.raises(ValueError):
+        m.check()
+    m.clear_error()
+    m.check()
+    for s in (c, kid, b):  # the order in which the free slots were left
+        o.free_sequence(s)
+    assert m.allocator.refcounts == o.snapshot()["refcounts"]
+    assert sorted(m.allocator.free_list()) == sorted(o.snapshot()["free"])
+    assert not m._nblocks[:, m._free_slots].any()
+    assert sorted(m.fork_sequences([a, a, a])) == sorted(o.fork_sequence(a) for _ in range(3))
+    m.check()
+    assert m.allocator.refcounts == o.snapshot()["refcounts"]
