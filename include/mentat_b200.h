@@ -369,7 +369,9 @@ int mentat_kv_append_rotated(const mentat_kv_cache* c, int32_t layer, int32_t sl
 /*
  * Pages of several sequences at once.  The slots are device int32[n], n <= 1024.
  * A batch that names a slot outside [0, max_seqs), or one that must be distinct
- * twice, changes nothing and records MENTAT_DEV_BAD_SLOT.
+ * twice, changes nothing and records MENTAT_DEV_BAD_SLOT.  A sequence that is
+ * longer than its table has room for is recorded as MENTAT_DEV_TABLE_OVERFLOW:
+ * a fork of it or a compaction changes nothing, a free releases what the table holds.
  */
 /* fork_sequence (paged_kv_cache.py:152-170) of parents[i] into children[i].
  * The children are distinct and empty (in every layer) and none is also a

@@ -72,6 +72,12 @@ __device__ __forceinline__ bool slots_distinct(const mentat_kv_cache& c, const i
     }
     return !__syncthreads_or(no);
 }
+// Entries of a table, no more than it has room for: the counters of a KVCacheView are the caller's.
+__device__ __forceinline__ int table_len(const mentat_kv_cache& c, int64_t si) { return min(c.nblocks[si], c.max_blocks_per_seq); }
+__device__ __forceinline__ bool table_overflows(const mentat_kv_cache& c, int64_t si) {
+    const int nb = c.nblocks[si], len = c.ntok[si];
+    return nb > c.max_blocks_per_seq || len > (int64_t)c.max_blocks_per_seq * c.block_size;
+}
 __device__ __forceinline__ bool has_bit(const uint32_t* bits, int s) { return (bits[s >> 5] >> (s & 31)) & 1; }
 
 // ---------------------------------------------------------------------------
@@ -79,7 +85,7 @@ __device__ __forceinline__ bool has_bit(const uint32_t* bits, int s) { return (b
 // ---------------------------------------------------------------------------
 // The batch is checked in a launch before: no CTA of the fork could see whether a child is empty, since another one may
 // have filled it.  What is wrong is recorded, and the fork does nothing after an error.  CTA 0 looks at the slots, all of them at
-// the children's counters.
+// the counters.
 constexpr int PAGES_THREADS = 256, PAGES_WARPS = PAGES_THREADS / 32;
 __global__ void __launch_bounds__(PAGES_THREADS) k_fork_check(mentat_kv_cache c, const int32_t* parents,
                                                               const int32_t* children, int n) {
@@ -89,10 +95,12 @@ __global__ void __launch_bounds__(PAGES_THREADS) k_fork_check(mentat_kv_cache c,
     griddep_launch();
     for (int64_t x = blockIdx.x * (int64_t)PAGES_THREADS + threadIdx.x; x < (int64_t)n * c.num_layers;
          x += (int64_t)gridDim.x * PAGES_THREADS) {
-        const int s = children[x % n];
-        if (s < 0 || s >= c.max_seqs) continue;
-        const int64_t si = seq_index(c, (int)(x / n), s);
-        if (c.nblocks[si] || c.ntok[si]) set_error(c, MENTAT_DEV_BAD_SLOT, s);
+        const int s = children[x % n], p = parents[x % n], l = (int)(x / n);
+        const bool child = s >= 0 && s < c.max_seqs, parent = p >= 0 && p < c.max_seqs;
+        const int64_t si = seq_index(c, l, child ? s : 0), pi = seq_index(c, l, parent ? p : 0);
+        const bool used = (c.nblocks[si] | c.ntok[si]) != 0, over = table_overflows(c, pi);
+        if (child && used) set_error(c, MENTAT_DEV_BAD_SLOT, s);
+        if (parent && over) set_error(c, MENTAT_DEV_TABLE_OVERFLOW, p);
     }
     if (blockIdx.x) return;
     if (!slots_distinct(c, children, n, bits, &s_bad)) {
@@ -197,7 +205,10 @@ __global__ void __launch_bounds__(256) k_free_mark(mentat_kv_cache c, const int3
     int nb[MARK_SEQS], most = 0;
 #pragma unroll
     for (int k = 0; k < MARK_SEQS; ++k) {
-        nb[k] = k < count ? c.nblocks[seq_index(c, l, slots[i0 + k])] : 0;
+        const int64_t si = seq_index(c, l, slots[i0 + min(k, count - 1)]);
+        nb[k] = k < count ? table_len(c, si) : 0;
+        if (!LEAD && blockIdx.y == 0 && threadIdx.x == 0 && k < count && c.nblocks[si] > c.max_blocks_per_seq)
+            set_error(c, MENTAT_DEV_TABLE_OVERFLOW, slots[i0 + k]);
         most = max(most, nb[k]);
     }
     for (int j = blockIdx.y * blockDim.x + threadIdx.x; j < most; j += gridDim.y * blockDim.x) {
@@ -240,7 +251,7 @@ __global__ void __launch_bounds__(PAGES_THREADS) k_free_count(mentat_kv_cache c,
     const int lane = threadIdx.x & 31, row = blockIdx.x * PAGES_WARPS + (threadIdx.x >> 5);
     if (row >= rows || *w.stop) return;
     const int i = row / c.num_layers, l = row - i * c.num_layers;
-    const int nb = c.nblocks[seq_index(c, l, slots[i])];
+    const int nb = table_len(c, seq_index(c, l, slots[i]));
     const int32_t* t = table_row(c, l, slots[i]);
     int n = 0;
     for (int j0 = LEAD ? w.lead[row] : 0; j0 < nb; j0 += 128) {
@@ -300,7 +311,7 @@ __global__ void __launch_bounds__(PAGES_THREADS) k_free_push(mentat_kv_cache c, 
     const int64_t si = seq_index(c, l, slots[i]);
     int32_t* t = table_row(c, l, slots[i]);
     if (s_count[warp]) {
-        const int nb = c.nblocks[si];
+        const int nb = table_len(c, si);
         for (int j0 = LEAD ? w.lead[row] : 0; j0 < nb; j0 += 32) {
             const int j = j0 + lane, b = j < nb ? t[j] : -1;
             const bool go = frees(c, w, b, row, j);
@@ -355,13 +366,18 @@ __global__ void __launch_bounds__(CLUSTER_THREADS) k_free_cluster(mentat_kv_cach
     // the entries are read while the batch is checked (a slot that is out of range has none)
     const long long tail0 = c.ctrl[MENTAT_CTRL_TAIL];
     bool stop = LEAD ? *w.stop != 0 : has_error(c);
+    int over = -1;  // a slot whose table is longer than its room
     for (int y = y0; y < y1; ++y) {
         const int row = y / chunks, j = y % chunks * 32 + lane, i = row / c.num_layers, l = row - i * c.num_layers;
         const int slot = slots[i], lead = LEAD && !stop ? w.lead[row] : 0;
         int b = -1;
-        if (slot >= 0 && slot < c.max_seqs && j >= lead && j < c.nblocks[seq_index(c, l, slot)]) {
-            b = table_row(c, l, slot)[j];
-            if ((unsigned)b >= (unsigned)c.num_blocks) b = -2;  // recorded once all CTAs have looked at the error word
+        if (slot >= 0 && slot < c.max_seqs) {
+            const int nb = c.nblocks[seq_index(c, l, slot)];
+            if (nb > c.max_blocks_per_seq) over = slot;
+            if (j >= lead && j < min(nb, c.max_blocks_per_seq)) {
+                b = table_row(c, l, slot)[j];
+                if ((unsigned)b >= (unsigned)c.num_blocks) b = -2;  // recorded once all CTAs have looked at the error word
+            }
         }
         held[(y - y0) * 32] = b;
     }
@@ -376,7 +392,7 @@ __global__ void __launch_bounds__(CLUSTER_THREADS) k_free_cluster(mentat_kv_cach
     auto rest = [&](int y, auto&& f) {
         if (y % chunks != chunks - 1) return;
         const int row = y / chunks, i = row / c.num_layers, l = row - i * c.num_layers;
-        const int nb = c.nblocks[seq_index(c, l, slots[i])], lead = LEAD ? w.lead[row] : 0;
+        const int nb = table_len(c, seq_index(c, l, slots[i])), lead = LEAD ? w.lead[row] : 0;
         const int32_t* t = table_row(c, l, slots[i]);
         for (int j0 = chunks * 32; j0 < nb; j0 += 32) {
             const int j = j0 + lane, b = j < nb && j >= lead ? t[j] : -1;
@@ -391,6 +407,7 @@ __global__ void __launch_bounds__(CLUSTER_THREADS) k_free_cluster(mentat_kv_cach
         });
     }
     cluster.sync();
+    if (!LEAD && over >= 0 && lane == 0) set_error(c, MENTAT_DEV_TABLE_OVERFLOW, over);
     auto mark = [&](int row, int j, int b) {
         if (b < 0) return;
         if (atomicSub(&c.refcounts[b], 1) <= 0) {
@@ -532,7 +549,8 @@ __global__ void __launch_bounds__(CLUSTER_THREADS) k_compact_plan(mentat_kv_cach
             // block have tails of one length (the batched append relies on it)
             const int lead = first == m && m == len ? pages : first / c.block_size;
             if (lane == 0) {
-                if (m < 0 || pages > c.max_blocks_per_seq) set_error(c, MENTAT_DEV_TABLE_OVERFLOW, a.src[i]);
+                if (pages > c.max_blocks_per_seq || table_overflows(c, seq_index(c, l, a.src[i])))
+                    set_error(c, MENTAT_DEV_TABLE_OVERFLOW, a.src[i]);
                 w.lead[row] = lead;
                 w.first[row] = demand;  // within the warp, so far
                 w.count[row] = pages - lead;
@@ -962,7 +980,7 @@ int mentat_kv_fork_batched(const mentat_kv_cache* c, const int32_t* parents, con
     if (n == 0) return MENTAT_OK;
     if (!slots_fit(c)) return MENTAT_ERR_UNSUPPORTED;
     const dim3 grid((n + PAGES_WARPS - 1) / PAGES_WARPS, c->num_layers);
-    MENTAT_LAUNCH(k_fork_check, dim3(chunks_of((int64_t)n * c->num_layers, 4 * PAGES_THREADS, 148)), dim3(PAGES_THREADS),
+    MENTAT_LAUNCH(k_fork_check, dim3(chunks_of((int64_t)n * c->num_layers, PAGES_THREADS, 148)), dim3(PAGES_THREADS),
                   bitmap_bytes(c), s, *c, parents, children, n);
     MENTAT_LAUNCH(k_fork_batched, grid, dim3(PAGES_THREADS), 0, s, *c, parents, children, n);
     return MENTAT_OK;

@@ -541,3 +541,51 @@ def test_slots_freed_after_an_error_are_empty_when_it_is_cleared():
     assert sorted(m.fork_sequences([a, a, a])) == sorted(o.fork_sequence(a) for _ in range(3))
     m.check()
     assert m.allocator.refcounts == o.snapshot()["refcounts"]
+
+
+@pytest.mark.parametrize("together", [1, 600], ids=["one", "many"])  # one cluster's work, and launches of their own
+def test_lengths_beyond_the_table_are_recorded(together):
+    """Counters of a caller's view that say more than its tables have room for, in the very last row: recorded, and no
+    entry behind the table is read.  A fork and a compaction change nothing; a free releases what the table holds."""
+    from mentat_b200 import KVCacheView, ops
+    L, S, cap, bs, pool = 2, 600, 4, 4, 32
+    i32 = dict(dtype=torch.int32, device="cuda")
+    kv = torch.randn((L, pool, bs, 1, 64), device="cuda")
+    tables = torch.full((L, S, cap), -1, **i32)
+    tables[:, S - 1] = torch.arange(2 * cap, **i32).view(L, cap)
+    nblocks, ntok, tail = (torch.zeros((L, S), **i32) for _ in range(3))
+    nblocks[:, S - 1], ntok[:, S - 1], tail[:, S - 1] = cap, cap * bs, bs
+    refs = torch.zeros(pool, **i32)
+    refs[: 2 * cap] = 1
+    ring = torch.arange(pool, **i32)
+    ctrl = torch.zeros(16, dtype=torch.int64, device="cuda")
+    ctrl[0], ctrl[1] = 2 * cap, pool  # what follows the blocks in use is free
+    c = KVCacheView(kv, kv.clone(), tables, ntok, nblocks=nblocks, tail=tail, refcounts=refs, free_ring=ring, ctrl=ctrl)
+    last, other = (torch.tensor([x], **i32) for x in (S - 1, 0))
+
+    def recorded(call, *unchanged):
+        before = [t.clone() for t in unchanged]
+        call()
+        with pytest.raises(RuntimeError, match=f"table overflow .slot {S - 1}"):
+            c.check()
+        ctrl[3:5] = 0
+        for t, w in zip(unchanged, before):
+            assert torch.equal(t, w)
+    state = (tables, nblocks, ntok, tail, refs, ring, ctrl, kv)
+    keep, cu = torch.arange(15, -1, -1, **i32), torch.tensor([0, 16], **i32)  # positions that the table holds
+    beyond = torch.stack([keep, keep + 25])                                    # and that the last layer claims to hold
+    nblocks[1, S - 1] = cap + 5
+    recorded(lambda: ops.fork_pages(c, last, other), *state)
+    for dst in (None, other):
+        recorded(lambda: ops.compact_pages(c, last, dst, keep, cu, 16), *state)
+    nblocks[1, S - 1] = cap
+    ntok[1, S - 1] = 50
+    recorded(lambda: ops.fork_pages(c, last, other), *state)
+    for dst in (None, other):
+        for k in (keep, beyond):
+            recorded(lambda: ops.compact_pages(c, last, dst, k, cu, 16), *state)
+    ntok[1, S - 1] = cap * bs
+    nblocks[1, S - 1] = 1 << 30
+    recorded(lambda: ops.free_pages(c, torch.arange(S - together, S, **i32)), tables, ring[2 * cap:])
+    assert not refs.any() and not nblocks.any() and not ntok.any() and not tail.any()
+    assert ctrl[:2].tolist() == [2 * cap, pool + 2 * cap] and ring[: 2 * cap].tolist() == list(range(2 * cap))
