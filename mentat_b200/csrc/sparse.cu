@@ -31,6 +31,7 @@ namespace mentat {
 // index
 // ---------------------------------------------------------------------------
 constexpr int EXP_MIN = -50, EXP_MAX = 50, EXP_ALL = 127;
+constexpr int EXP_UNREADABLE = -128;  // in no index: the table's entry is outside the pool
 
 // the least e with top <= 127 * 2^e, within EXP_MIN .. EXP_MAX; top finite, >= 0
 __device__ __forceinline__ int unit_exponent(float top) {
@@ -1259,6 +1260,7 @@ __global__ void __launch_bounds__(SCORE_THREADS, 2) k_score(mentat_kv_cache c, m
         if (pp >= P) return;
         uint32_t key = ek == EXP_ALL ? 0xfffffffeu : ordered(best * pow2(ek));
         if (pp < a.sink || pp >= P - a.recent) key = 0xffffffffu;
+        if (ek == EXP_UNREADABLE) key = 0u;  // behind all others
         out[i * out_step + pp] = key;
     };
     auto unit_of = [&](int nt) { return *reinterpret_cast<const float2*>(s_unit + nt * 8 + 2 * t); };
@@ -1345,6 +1347,9 @@ __global__ void __launch_bounds__(SCORE_THREADS, 2) k_score(mentat_kv_cache c, m
                     b[r] = -1;
                 }
             load(b[0], b[1], nv, nek);
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+                if (b[r] == -1) nek[r] = EXP_UNREADABLE;
         };
         if (warp < units) {
             blocks_of(warp);

@@ -542,3 +542,34 @@ def test_infinite_values_show_as_such(hq, dtype):
     assert (out[0, :, 3] == float("inf")).all() and (out[1, :, 60] == -float("inf")).all()
     out[0, :, 3] = out[1, :, 60] = 0
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("page", [0, 300, 605, 609])
+def test_large_batches_choose_unreadable_pages_last(page):
+    """A page whose table entry is outside the pool, even one that is always chosen otherwise, has the key that it
+    has where one launch does it all: the sequence alone chooses the same pages, and not this one."""
+    from mentat_b200 import ops
+    n, lens = 80, [610 * 16] * 80  # 610 pages for each of 160 heads: scores and choice have launches of their own
+    c, x, q, tables = make(lens, 4, 2, 64, 16, "bf16", layers=1, shared=600)
+    c._tensors["tables"][0, 11, page] = c.max_blocks
+    every = torch.arange(n, dtype=torch.int32, device="cuda")
+    assert x.workspace_bytes(n, 610 * 16, 12) > 0 and x.workspace_bytes(1, 610 * 16, 12) == 0
+    _, many = ops.sparse_decode(x, 0, every, q, 610 * 16, 12, return_pages=True)
+    with pytest.raises(AssertionError):
+        c.check()
+    c._tensors["ctrl"].zero_()
+    _, one = ops.sparse_decode(x, 0, every[11:12], q[11:12], 610 * 16, 12, return_pages=True)
+    assert torch.equal(many[11:12], one)
+    assert (one >= 0).all() and not (one == page).any()
+
+
+def test_large_batches_of_trees():
+    """Batches that have launches of their own for the scores and the choice: rows that share all, some or none of
+    their pages, rows without a choice and an empty one among them, groups that do not divide the columns."""
+    rng = np.random.default_rng(6)
+    for hq, hkv, d, n in ((24, 8, 64, 41), (10, 2, 128, 90)):
+        lens = [int(v) for v in rng.integers(1, 9900, n)]
+        lens[3], lens[5], lens[n - 1] = 0, 17, 9897
+        c, x, q, tables = make(lens, hq, hkv, d, 16, "bf16", layers=1, shared=400)
+        assert x.workspace_bytes(n, 9897, 8) > 0
+        run_and_check(c, x, q, tables, lens, 8, 1, 2, "bf16", layer=0)
