@@ -645,11 +645,14 @@ __device__ __forceinline__ void choose_cluster(const uint32_t* keys, int p0, int
     for (int pass = 0; pass < 4; ++pass) {
         const int shift = 24 - 8 * pass;
         int* cnt = counts + 256 * pass;
-        for (int p = tid; p < m; p += THREADS) {
-            const uint32_t key = keys[p];
-            if ((key & mask) == prefix) {
+        for (int w0 = tid & ~31; w0 < m; w0 += THREADS) {  // whole warps
+            const int p = w0 + (tid & 31);
+            const uint32_t key = p < m ? keys[p] : 0u;
+            const bool in = p < m && (key & mask) == prefix;
+            const uint32_t who = __ballot_sync(0xffffffffu, in);
+            if (in) {
                 // one addition for each digit that the warp's lanes have
-                const uint32_t digit = (key >> shift) & 255, peers = __match_any_sync(__activemask(), digit);
+                const uint32_t digit = (key >> shift) & 255, peers = __match_any_sync(who, digit);
                 if ((peers & ((1u << (tid & 31)) - 1)) == 0) atomicAdd(&cnt[digit], __popc(peers));
             }
         }
