@@ -316,9 +316,9 @@ int mentat_prune_similar(const void* sim, int32_t dtype, int64_t sim_stride, con
  * offset + 2 pairs of every head are taken as pairs (i, i + pairs), or
  * (2i, 2i + 1) if interleaved, and pair i is turned by position * inv_freq[i]
  * (by its negative if inverse) and multiplied by scale; the other dimensions
- * are copied.  Angles are reduced to one turn in 64 bits, so positions may be
- * any int64 (negative ones turn backwards); the pairs are turned in 32 bits and
- * rounded once.
+ * are copied.  Positions may be any int64 (negative ones turn backwards): for
+ * inv_freq up to 1 the fraction of a turn is known to 2^-42 at every one of them.
+ * The pairs are turned in 32 bits and rounded once.
  */
 typedef struct mentat_rotary {
     const double* inv_freq;      /* device [pairs], radians per position */

@@ -3,11 +3,14 @@
 //
 // Pair i of a token at position p is turned by p * inv_freq[i]: (x1, x2) ->
 // scale * (x1 cos - x2 sin, x1 sin + x2 cos).  The angle is taken in turns,
-// p * (inv_freq / 2 pi), in double: at p = 2^20 and one radian per position that
-// is 2^17.3 turns, known to 2^-36 of a turn, where a float would be off by
-// 2^-7.  The fraction left after rint() is at most half a turn, exact as a
-// double, and goes to the float sincospif.  Products and sums are float, one
-// rounding to the element type at the end.
+// p * (inv_freq / 2 pi), as a sum of two doubles: one double would know 2^60 turns to 2^7 of
+// a turn, and 2^17 (p = 2^20 at one radian per position) to 2^-35.  The factor
+// 1 / 2 pi and its product with inv_freq have an error of 2^-104 of themselves, the products
+// with p leave their rounding in a fused multiply-add, and whole turns are dropped
+// before the parts are added.  So the fraction of a turn is off by less than 2^-42 for every int64
+// position and every inv_freq up to one radian.  It goes to the float sincospif as the nearest float;
+// what that leaves (up to 2^-26 of a turn) is added to first order, the second being below 2^-47.
+// Products and sums are float, one rounding to the element type at the end.
 #pragma once
 
 #include "common.cuh"
@@ -17,13 +20,24 @@ namespace mentat {
 constexpr int ROTARY_THREADS = 128;   // most threads that share a token
 constexpr int ROTARY_MAX_DIM = 1024;  // largest head_dim of the rotary entry points
 
+// p * (fh + fl) without whole turns; p exact
+__device__ __forceinline__ double rotary_turns(double p, double fh, double fl) {
+    const double a = __dmul_rn(p, fh);  // rounded: not to be fused with the difference
+    return (a - rint(a)) + fma(p, fl, fma(p, fh, -a));
+}
 __device__ __forceinline__ void rotary_angle(const mentat_rotary& r, int i, int64_t pos, float* c, float* s) {
-    double t = (double)pos * (r.inv_freq[i] * 0.15915494309189533577);
+    constexpr double H = 0.15915494309189535, L = -9.839338337591243e-18;  // 1 / 2 pi
+    const double f = r.inv_freq[i], fh = __dmul_rn(f, H), fl = fma(f, L, fma(f, H, -fh));
+    double t = rotary_turns((double)(uint32_t)pos, fh, fl);
+    const int high = (int)(pos >> 32);
+    if (high) t += rotary_turns((double)high * 4294967296.0, fh, fl);
     t -= rint(t);
+    const float th = (float)t, d = 6.2831853f * (float)(t - (double)th);
     float sn, cs;
-    sincospif(2.0f * (float)t, &sn, &cs);
-    *c = cs * r.scale;
-    *s = r.inverse ? -sn * r.scale : sn * r.scale;
+    sincospif(2.0f * th, &sn, &cs);
+    *c = (cs - sn * d) * r.scale;
+    const float turned = (sn + cs * d) * r.scale;
+    *s = r.inverse ? -turned : turned;
 }
 
 // cos and sin of every pair of one token, to cs[0 .. pairs) and cs[pairs ..); the caller synchronises

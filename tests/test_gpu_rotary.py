@@ -1,5 +1,7 @@
 """Rotary positions on the device against the definition in 64 bits (``oracle.cache_ops``)."""
 
+from fractions import Fraction
+
 import numpy as np
 import pytest
 import torch
@@ -162,3 +164,36 @@ def test_rotary_on_another_stream_and_in_a_graph():
     pos.add_(1000)
     graph.replay()
     assert torch.equal(out, ops.rotary(q, None, pos, rot)[0]) and not torch.equal(out, want)
+
+
+# 1 / 2 pi to 60 digits
+INV_TWO_PI = Fraction(159154943091895335768883763372514362034459645740456448747667, 10 ** 60)
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.5])
+def test_angles_of_any_position(scale):
+    """Cosines and sines (the turn of (1, 0) and of (0, 1)) of near and far positions against exact arithmetic.
+
+    The fraction of a turn is off by 2^-42, the angle by 2^-39.3.  sincospif is off by at most 2 units in the last
+    place (2^-23 for values up to 1), the added remainder's product and sum by 2^-24 each of at most 1 and a second-order
+    term of 2^-47; a power of two as the factor adds nothing and the products with 0 and 1 are exact.  Below
+    2^-23 + 2^-24 + 2^-24 + 2^-38."""
+    from mentat_b200 import Rotary, ops
+    d = 128
+    rot = Rotary(d, base=5e5, attention_scaling=scale)
+    rng = np.random.default_rng(0)
+    pos = [0, 1, -1, 7, 4095, 131071, 1 << 20, -(1 << 20) - 3, (1 << 31) - 1, 1 << 31, (1 << 32) - 1, 1 << 32, -(1 << 32) - 1,
+           (1 << 40) + 12345, (1 << 53) + 1, -(1 << 53) - 1, (1 << 62) + 987654321, (1 << 63) - 1, -(1 << 63)]
+    pos += [int(v) for v in rng.integers(-(1 << 62), 1 << 62, 20)] + [int(v) for v in rng.integers(0, 1 << 20, 200)]
+    x = torch.zeros((len(pos), 2, d), device="cuda")
+    x[:, 0, : d // 2] = 1.0
+    x[:, 1, d // 2:] = 1.0
+    got = ops.rotary(x, None, torch.tensor(pos, dtype=torch.int64, device="cuda"), rot)[0].double().cpu().numpy()
+    back = ops.rotary(x, None, torch.tensor(pos, dtype=torch.int64, device="cuda"), rot, inverse=True)[0].double().cpu().numpy()
+    turns = np.array([[float((lambda t: t - round(t))(p * Fraction(f) * INV_TWO_PI)) for f in rot.inv_freq.tolist()] for p in pos])
+    cos, sin = np.cos(2 * np.pi * turns) * scale, np.sin(2 * np.pi * turns) * scale
+    tol = (2.0 ** -23 + 2.0 ** -23 + 2.0 ** -38) * scale
+    h = d // 2
+    for out, s in ((got, sin), (back, -sin)):
+        for part, want in ((out[:, 0, :h], cos), (out[:, 0, h:], s), (out[:, 1, :h], -s), (out[:, 1, h:], cos)):
+            assert np.abs(part - want).max() <= tol, np.unravel_index(np.abs(part - want).argmax(), part.shape)
