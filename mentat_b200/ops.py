@@ -375,7 +375,13 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     """Turns ``q`` (N, Hq, D) and ``k`` (N, Hkv, D; may be None) to ``positions`` (N,)
     (``Rotary``); ``inverse`` turns back, which is also the gradient of the turn.
     Returns (q, k): new tensors, or ``q_out`` / ``k_out``, which may be the inputs
-    themselves.  Any token and head strides; wraps ``mentat_rotary_apply``."""
+    themselves.  Any token and head strides; wraps ``mentat_rotary_apply``.  Gradients
+    pass to ``q`` and ``k``; with outputs given, which torch could not follow, an input that
+    requires one is refused."""
+    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
+        if q_out is not None or k_out is not None:
+            raise RuntimeError("rotary: q_out and k_out pass no gradients on, and an input requires one")
+        return _Turn.apply(q, k, positions, rotary, bool(inverse))
     n, _, d = q.shape
     dtype, dev = q.dtype, q.device
     q, rq = _operand("q", q, n, d, dtype, dev)
@@ -395,14 +401,34 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     return qo, ko
 
 
+class _Turn(torch.autograd.Function):
+    """``rotary`` with gradients: the turn is linear, and turning back (with the same factor) is its transpose."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, rot, inverse):
+        ctx.save_for_backward(positions)
+        ctx.rot, ctx.inverse = rot, inverse
+        ctx.set_materialize_grads(False)
+        return rotary(q, k, positions, rot, inverse=inverse)
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        positions, = ctx.saved_tensors
+        gq, gk = (g if need else None for g, need in zip((gq, gk), ctx.needs_input_grad))
+        if gq is None and gk is None:
+            return (None,) * 5
+        a, b = rotary(gk if gq is None else gq, None if gq is None else gk, positions, ctx.rot, inverse=not ctx.inverse)
+        return (None, a, None, None, None) if gq is None else (a, b, None, None, None)
+
+
 def rotary_append(cache, layer: int, rows: torch.Tensor, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
                   positions: torch.Tensor, rotary, *, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Turns ``q`` (N, Hq, D; may be None) and ``k`` (N, Hkv, D) to ``positions`` (N,) and
     writes the keys and ``v`` into rows ``rows`` (N,) int64 of layer ``layer``
     of ``cache`` (a manager or a ``KVCacheView``): block * block_size + offset,
     distinct; -1 writes none.  Returns the turned queries.  The tables and lengths
-    are not touched; ``PagedKVCacheManager.append_rotated`` keeps them.  Wraps
-    ``mentat_rotary_append``."""
+    are not touched; ``PagedKVCacheManager.append_rotated`` keeps them.  Passes no
+    gradients on, like every operator of a cache.  Wraps ``mentat_rotary_append``."""
     n, hkv, d = k.shape
     dev, dtype = cache.device, cache.dtype
     if d != cache.head_dim or hkv != cache.num_key_value_heads or v.shape[1] != hkv:

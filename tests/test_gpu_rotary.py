@@ -197,3 +197,54 @@ def test_angles_of_any_position(scale):
     for out, s in ((got, sin), (back, -sin)):
         for part, want in ((out[:, 0, :h], cos), (out[:, 0, h:], s), (out[:, 1, :h], -s), (out[:, 1, h:], cos)):
             assert np.abs(part - want).max() <= tol, np.unravel_index(np.abs(part - want).argmax(), part.shape)
+
+
+def test_rotary_passes_gradients_on():
+    """Against the formula's transpose in 64 bits and against differences; q alone, k alone, both, neither."""
+    from mentat_b200 import Rotary, ops
+    g = torch.Generator(device="cuda").manual_seed(2)
+    rot = Rotary(32, rotary_dim=24, offset=4, interleaved=True, attention_scaling=1.3)
+    pos = torch.tensor([0, 5, 70000], device="cuda")
+    q, gq = (torch.randn((3, 4, 32), generator=g, device="cuda") for _ in range(2))
+    k, gk = (torch.randn((3, 2, 32), generator=g, device="cuda") for _ in range(2))
+    plain = ops.rotary(q, k, pos, rot)
+    for need_q, need_k in ((True, True), (True, False), (False, True)):
+        a, b = q.clone().requires_grad_(need_q), k.clone().requires_grad_(need_k)
+        oq, ok = ops.rotary(a, b, pos, rot)
+        assert torch.equal(oq, plain[0]) and torch.equal(ok, plain[1])
+        torch.autograd.backward([oq, ok] if need_q and need_k else [oq] if need_q else [ok],
+                                [gq, gk] if need_q and need_k else [gq] if need_q else [gk])
+        for x, up in ((a, gq), (b, gk)):
+            if x.requires_grad:
+                _near(x.grad, up, pos, rot, inverse=True, what="gradient")
+            else:
+                assert x.grad is None
+    # turned back, alone, a gradient of stride zero, and one output that nothing uses
+    a = q.clone().requires_grad_()
+    out, none = ops.rotary(a, None, pos, rot, inverse=True)
+    assert none is None
+    out.sum().backward()
+    _near(a.grad, torch.ones_like(q), pos, rot, what="gradient of the turn back")
+    a, b = q.clone().requires_grad_(), k.clone().requires_grad_()
+    ops.rotary(a, b, pos, rot)[1].backward(gk)
+    assert a.grad is None
+    _near(b.grad, gk, pos, rot, inverse=True)
+    # the slope by differences: the turn is linear, so any step; 384 products of values below 6 * 1.3 * 2, each turned
+    # value off by less than 10 2^-24 of that, and the inputs' sums by 2^-24 * 9, over the step
+    a = q.clone().requires_grad_()
+    (ops.rotary(a, None, pos, rot)[0] * gq).sum().backward()
+    dx, h = torch.randn((3, 4, 32), generator=g, device="cuda"), 0.5
+    up, down = (ops.rotary(q + s * h * dx, None, pos, rot)[0].double() for s in (1, -1))
+    slope = ((up - down) * gq.double()).sum() / (2 * h)
+    assert abs(slope - (dx.double() * a.grad.double()).sum()) < 3 * 384 * 6 * 10 * 2.0 ** -24 * 12 * 1.3 / h
+    # second order: the gradient is a turn of its own
+    a = q.clone().requires_grad_()
+    y = gq.clone().requires_grad_()
+    grad, = torch.autograd.grad((ops.rotary(a, None, pos, rot)[0] * y).sum(), a, create_graph=True)
+    again, = torch.autograd.grad((grad * dx).sum(), y)
+    _near(again, dx, pos, rot, what="second order")
+    # outputs of the caller's take none; without gradients they are as before
+    with pytest.raises(RuntimeError, match="q_out"):
+        ops.rotary(q.clone().requires_grad_(), None, pos, rot, q_out=torch.empty_like(q))
+    with torch.no_grad():
+        assert torch.equal(ops.rotary(q.clone().requires_grad_(), None, pos, rot, q_out=torch.empty_like(q))[0], plain[0])
