@@ -1547,7 +1547,8 @@ int mentat_page_index_blocks(const mentat_kv_cache* c, int32_t layer, const int3
 int mentat_page_index_seqs(const mentat_kv_cache* c, int32_t layer, const int32_t* slots, int32_t n, int32_t first,
                            int32_t max_pages, const mentat_page_index* x, cudaStream_t s) {
     if (bad_index(c, x) || layer < -1 || layer >= c->num_layers || n < 0 || first < -1 || max_pages < 0 ||
-        !c->tables || !c->ntok || c->num_layers > 65535 || (n > 0 && !slots) || (int64_t)n * max_pages > 0x7fffffff)
+        !c->tables || !c->ntok || c->num_layers > 65535 || (n > 0 && !slots) || (int64_t)n * max_pages > 0x7fffffff ||
+        (int64_t)first + max_pages > 0x7fffffff)  // a page's number is an int
         return MENTAT_ERR_ARG;
     if (first < 0) max_pages = 1;
     if (n == 0 || max_pages == 0) return MENTAT_OK;

@@ -353,6 +353,11 @@ def _check_positions(positions: torch.Tensor, n: int, device) -> torch.Tensor:
     return positions if dtype is torch.int64 and positions.is_contiguous() else positions.to(torch.int64).contiguous()
 
 
+def _check_layer(layer: int, cache) -> None:
+    if not 0 <= layer < cache.num_layers:
+        raise ValueError(f"layer {layer} is not within 0 .. {cache.num_layers - 1}")
+
+
 def _check_rotary(rotary, d: int, device) -> None:
     if rotary.head_dim != d:
         raise ValueError(f"the rotary is for heads of {rotary.head_dim}, not {d}")
@@ -433,8 +438,7 @@ def rotary_append(cache, layer: int, rows: torch.Tensor, q: Optional[torch.Tenso
     dev, dtype = cache.device, cache.dtype
     if d != cache.head_dim or hkv != cache.num_key_value_heads or v.shape[1] != hkv:
         raise ValueError("k or v shape does not match the cache geometry")
-    if not 0 <= layer < cache.num_layers:
-        raise ValueError(f"layer {layer} is not within 0 .. {cache.num_layers - 1}")
+    _check_layer(layer, cache)
     k, rk = _operand("k", k, n, d, dtype, dev)
     v, rv = _operand("v", v, n, d, dtype, dev)
     _check_rotary(rotary, d, dev)
@@ -461,6 +465,8 @@ def _append_rotated(k_pool: torch.Tensor, v_pool: torch.Tensor, slots: torch.Ten
     mgr, rot = _cache(cache), _cache(rotary)
     n, d = k.shape[0], k.shape[2]
     dev = mgr.device
+    _check_rotary(rot, mgr.head_dim, dev)
+    slots = _check_ids("slots", slots, dev, n)
     (q, rq), (k, rk), (v, rv) = (_operand(name, t, n, d, mgr.dtype, dev) for name, t in (("q", q), ("k", k), ("v", v)))
     qo, rqo = _like(q)
     size = q.element_size()
@@ -497,11 +503,16 @@ def _index_tails(mgr, layer: int, slots: torch.Tensor, n: int) -> None:
 def index_sequences(mgr, slots: torch.Tensor, first_page: int, max_pages: int, layer: int = -1) -> None:
     """Indexes the full pages ``first_page .. first_page + max_pages`` of the slots' sequences
     in ``layer`` (-1: every layer) into the cache's index.  Wraps ``mentat_page_index_seqs``."""
+    index = _index_of(mgr)
+    slots = _check_ids("slots", slots, mgr.device)
+    if first_page < 0 or max_pages < 0:
+        raise ValueError(f"pages {first_page} .. {first_page} + {max_pages} are no range of pages")
+    first_page, max_pages = min(first_page, mgr.table_capacity), min(max_pages, mgr.table_capacity)  # no table has more
     step = max(1, 0x7fffffff // max(1, max_pages))
     for a in range(0, slots.shape[0], step):
         part = slots[a: a + step]
         _call(mgr.device, "mentat_page_index_seqs", mgr._desc_ptr, layer,
-              part.data_ptr(), part.shape[0], first_page, max_pages, mgr.page_index._ptr)
+              part.data_ptr(), part.shape[0], first_page, max_pages, index._ptr)
 
 
 def _workspace(cache, n: int) -> tuple:

@@ -709,6 +709,7 @@ class PagedKVCacheManager:
         if k.shape[1] != self.num_key_value_heads or v.shape[1] != self.num_key_value_heads:
             raise ValueError("k or v shape does not match the cache geometry")
         ops._check_rotary(rotary, d, self.device)
+        ops._check_layer(layer_idx, self)
         if positions is not None:
             positions = ops._check_positions(positions, n, self.device)
         qo, rq, rqo = None, ops._NO_ROWS, ops._NO_ROWS
@@ -736,6 +737,7 @@ class PagedKVCacheManager:
         if k.shape[1] != self.num_key_value_heads or v.shape[1] != self.num_key_value_heads:
             raise ValueError("k or v shape does not match the cache geometry")
         ops._check_rotary(rotary, self.head_dim, self.device)
+        ops._check_layer(layer_idx, self)
         if N == 0:
             return torch.empty(q.shape, dtype=q.dtype, device=q.device)
         self._mirror_append_batched(seqs, layer_idx)

@@ -259,7 +259,43 @@ def test_c_abi_refuses_sparse_arguments():
     assert lib.mentat_page_index_blocks(_desc(), 0, None, 0, x, None) == 0
     assert lib.mentat_page_index_seqs(_desc(), -2, 4096, 1, 0, 1, x, None) == ARG
     assert lib.mentat_page_index_seqs(_desc(), -1, 4096, 1, 0, 0, x, None) == 0
+    for first, pages in ((0x7fffffff, 1), (0x7fffff00, 0x100), (1, 0x7fffffff)):  # a page's number would pass an int
+        assert lib.mentat_page_index_seqs(_desc(), 0, 4096, 1, first, pages, x, None) == ARG
     assert lib.mentat_page_bounds(_desc(), 0, 4096, 1, x, None, 4096, 4096, None) == ARG
+
+
+def test_rotated_appends_and_index_refuse_their_arguments():
+    """What the kernels would read by: another model's rotary, slots of another type, length or shape, no index."""
+    class Cache:  # what the checks look at
+        def __init__(self, **kw):
+            self.__dict__.update(kw)
+    cpu = torch.device("cpu")
+    cache = Cache(device=cpu, dtype=torch.bfloat16, head_dim=64, num_layers=2, num_key_value_heads=2,
+                  page_index=None, table_capacity=16, _desc_ptr=0)
+    cid = ops.register_cache(cache)
+    rot, wide = Rotary(64, device="cpu"), Rotary(128, device="cpu")
+    q, k = torch.zeros(4, 8, 64, dtype=torch.bfloat16), torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    slots = torch.arange(4, dtype=torch.int32)
+
+    def append(slots=slots, q=q, rot=rot):
+        return ops.append_rotated(k, k, slots, q, k, k, cid, 0, rot.op_id)
+    with pytest.raises(RuntimeError, match="CUDA"):  # nothing to refuse but the device
+        append()
+    with pytest.raises(ValueError, match="heads of 128"):
+        append(rot=wide)
+    for bad in (slots.long(), slots[:3], slots.view(2, 2), torch.zeros(5, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="slots"):
+            append(slots=bad)
+    with pytest.raises(RuntimeError, match="enable_page_index"):
+        ops.index_sequences(cache, slots, 0, 1)
+    cache.page_index = Cache(_ptr=0)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.index_sequences(cache, slots, 0, 1)
+    with pytest.raises(ValueError, match="slots"):
+        ops.index_sequences(cache, slots.long(), 0, 1)
+    for first, pages in ((-1, 1), (0, -1)):
+        with pytest.raises(ValueError, match="range of pages"):
+            ops.index_sequences(cache, slots, first, pages)
 
 
 def test_operator_schemas():

@@ -589,3 +589,18 @@ def test_lengths_beyond_the_table_are_recorded(together):
     recorded(lambda: ops.free_pages(c, torch.arange(S - together, S, **i32)), tables, ring[2 * cap:])
     assert not refs.any() and not nblocks.any() and not ntok.any() and not tail.any()
     assert ctrl[:2].tolist() == [2 * cap, pool + 2 * cap] and ring[: 2 * cap].tolist() == list(range(2 * cap))
+
+
+def test_rotated_appends_to_no_layer_change_nothing():
+    from mentat_b200 import Rotary
+    rng = np.random.default_rng(24)
+    m, o = pair(L=2)
+    a, = start(m, o, [5], rng)
+    rot = Rotary(64)
+    x = torch.zeros((1, 2, 64), dtype=torch.bfloat16, device="cuda")
+    for layer in (-1, 2):
+        with pytest.raises(ValueError, match="layer"):
+            m.append_rotated(a, layer, x, x, x, rot)
+        with pytest.raises(ValueError, match="layer"):
+            m.append_rotated_batched([a], layer, x, x, x, rot)
+    same(m, o)
