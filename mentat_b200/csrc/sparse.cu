@@ -43,6 +43,15 @@ __device__ __forceinline__ int unit_exponent(float top) {
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 
+// A bound in units of 1 / inv, rounded outwards.  The product is exact but for keys below 2^-99 beside one above 127,
+// where it can underflow: a bound that is not zero keeps its side.
+__device__ __forceinline__ int8_t bound_low(float v, float inv) {
+    return (int8_t)fminf(fmaxf(floorf(v * inv), -127.f), v < 0.f ? -1.f : 127.f);
+}
+__device__ __forceinline__ int8_t bound_high(float v, float inv) {
+    return (int8_t)fmaxf(fminf(ceilf(v * inv), 127.f), v > 0.f ? 1.f : -127.f);
+}
+
 // One CTA of head_dim threads per (block, KV head).
 template <typename T>
 __device__ __forceinline__ void index_page(const mentat_kv_cache& c, int layer, int b, int h, const mentat_page_index& x) {
@@ -75,8 +84,8 @@ __device__ __forceinline__ void index_page(const mentat_kv_cache& c, int layer, 
     const int64_t at = ((int64_t)layer * c.num_blocks + b) * c.num_kv_heads + h;
     if (d < D) {
         int8_t* o = x.bounds + at * 2 * D + d;
-        o[0] = bad ? 0 : (int8_t)fminf(fmaxf(floorf(lo * inv), -127.f), 127.f);
-        o[D] = bad ? 0 : (int8_t)fminf(fmaxf(ceilf(hi * inv), -127.f), 127.f);
+        o[0] = bad ? (int8_t)0 : bound_low(lo, inv);
+        o[D] = bad ? (int8_t)0 : bound_high(hi, inv);
     }
     if (d == 0) x.exps[at] = (int8_t)(bad ? EXP_ALL : e);
     __syncthreads();
@@ -161,8 +170,8 @@ __device__ __forceinline__ void index_block(const mentat_kv_cache& c, int layer,
 #pragma unroll
             for (int i = 0; i < E::N; ++i) {
                 const float l = E::get(lo.v[w], i), g = E::get(hi.v[w], i);
-                ol.v[w * E::N + i] = bad ? 0 : (int8_t)fminf(fmaxf(floorf(l * inv), -127.f), 127.f);
-                oh.v[w * E::N + i] = bad ? 0 : (int8_t)fminf(fmaxf(ceilf(g * inv), -127.f), 127.f);
+                ol.v[w * E::N + i] = bad ? (int8_t)0 : bound_low(l, inv);
+                oh.v[w * E::N + i] = bad ? (int8_t)0 : bound_high(g, inv);
             }
         if (u < n) {
             const int h = u / per, d = (u - h * per) * VEC;

@@ -573,3 +573,20 @@ def test_large_batches_of_trees():
         c, x, q, tables = make(lens, hq, hkv, d, 16, "bf16", layers=1, shared=400)
         assert x.workspace_bytes(n, 9897, 8) > 0
         run_and_check(c, x, q, tables, lens, 8, 1, 2, "bf16", layer=0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 40])
+def test_bounds_of_the_smallest_keys_keep_their_side(d, dtype):
+    """Keys of 2^-133 beside one of 2^40 or 2^57: in units of the page they underflow, and their bounds are still on the
+    outer side of them."""
+    from mentat_b200 import KVCacheView, PageIndex, ops
+    k = torch.zeros((1, 3, 16, 1, d), dtype=TORCH_DT[dtype], device="cuda")
+    k[0, 0, 3, 0, 0], k[0, 1, 3, 0, 0] = 2.0 ** 40, -(2.0 ** 57)
+    k[0, :, 1, 0, 1], k[0, :, 1, 0, 2], k[0, :, :, 0, 3] = 2.0 ** -133, -(2.0 ** -133), 2.0 ** -133
+    x = PageIndex(KVCacheView(k, torch.zeros_like(k)))
+    ops.page_index(x, 0, torch.arange(3, dtype=torch.int32, device="cuda"))
+    for b in range(3):
+        bounds, exps = index_page(k[0, b].double().cpu().numpy())
+        np.testing.assert_array_equal(x.bounds[0, b].cpu().numpy(), bounds)
+        np.testing.assert_array_equal(x.exps[0, b].cpu().numpy(), exps)
