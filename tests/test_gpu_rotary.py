@@ -248,3 +248,32 @@ def test_rotary_passes_gradients_on():
         ops.rotary(q.clone().requires_grad_(), None, pos, rot, q_out=torch.empty_like(q))
     with torch.no_grad():
         assert torch.equal(ops.rotary(q.clone().requires_grad_(), None, pos, rot, q_out=torch.empty_like(q))[0], plain[0])
+
+
+def test_gradients_in_a_graph():
+    """Forward and backward pass captured together, beside an eager graph of the same leaves that is still alive, and
+    replayed over new values."""
+    from mentat_b200 import Rotary, ops
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rot, pos = Rotary(64), torch.arange(5, device="cuda") * 1001
+    q, k = (torch.randn((5, h, 64), generator=g, device="cuda").requires_grad_() for h in (4, 2))
+    up = [torch.randn((5, h, 64), generator=g, device="cuda") for h in (4, 2)]
+
+    def step():
+        return torch.autograd.grad(ops.rotary(q, k, pos, rot), (q, k), up)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        alive = ops.rotary(q, k, pos, rot)
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = step()
+    for _ in range(2):
+        for t in up:
+            t.normal_(generator=g)
+        graph.replay()
+        for a, b, name in zip(got, up, "qk"):
+            _near(a, b, pos, rot, inverse=True, what=name)
+    assert torch.equal(torch.autograd.grad(alive, (q, k), up)[0], got[0])
