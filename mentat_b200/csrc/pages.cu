@@ -19,7 +19,7 @@
 // of CTAs takes them all, with cluster barriers between them; else each step is a launch.
 //
 // Forks and frees are bound by latency: chains of dependent loads and barriers.  Fork and free of 64 x 3 children of 130
-// to 160 pages in 32 layers: 8 + 23 us, against 1 us of bytes; of 6 of 30 pages: 4 + 11 us.  A compaction is bound by the
+// to 160 pages in 32 layers: 32 us, against 1 us of bytes; of 6 of 30 pages: 17 us.  A compaction is bound by the
 // rows that it moves.
 
 #include <cooperative_groups.h>
@@ -113,8 +113,9 @@ __global__ void __launch_bounds__(PAGES_THREADS) k_fork_check(mentat_kv_cache c,
     }
 }
 
-// A warp takes one (layer, run of children of one parent that follow one another): the parent's table is read once
-// and each page's count rises by the run's length in one atomic.
+// A warp takes one (layer, child) and every gridDim.z-th group of 128 pages.  Of a run of children of one parent that
+// follow one another, the first one's warp raises each page's count by the run's length in one atomic.  (One warp for
+// a whole run and table: 3 children of 2,048 pages in 32 layers took 43 us, 3 single forks 14.)
 __global__ void __launch_bounds__(PAGES_THREADS) k_fork_batched(mentat_kv_cache c, const int32_t* parents,
                                                                 const int32_t* children, int n) {
     __shared__ int s_stop;
@@ -125,32 +126,38 @@ __global__ void __launch_bounds__(PAGES_THREADS) k_fork_batched(mentat_kv_cache 
     if (s_stop) return;
     const int lane = threadIdx.x & 31, l = blockIdx.y, i = blockIdx.x * PAGES_WARPS + (threadIdx.x >> 5);
     if (i >= n) return;
-    const int parent = parents[i];
-    if (i > 0 && parents[i - 1] == parent) return;  // in an earlier warp's run
-    int run = 1;
-    while (i + run < n && parents[i + run] == parent) ++run;
-    const int64_t ps = seq_index(c, l, parent);
+    const int parent = parents[i], child = children[i];
+    const int64_t ps = seq_index(c, l, parent), cs = seq_index(c, l, child);
     const int nb = c.nblocks[ps], ntok = c.ntok[ps], tail = c.tail[ps];
+    int run = 0;  // of the children that this one is the first of
+    if (i == 0 || parents[i - 1] != parent) {
+        uint32_t same = 0xffffffffu;
+        for (run = 1; same == 0xffffffffu; run += same == 0xffffffffu ? 32 : __ffs(~same) - 1)
+            same = __ballot_sync(0xffffffffu, i + run + lane < n && parents[i + run + lane] == parent);
+    }
     const int32_t* src = table_row(c, l, parent);
-    for (int j0 = 0; j0 < nb; j0 += 128) {
-        int b[4];  // four entries of a lane on the way
+    int32_t* dst = table_row(c, l, child);
+    for (int j0 = blockIdx.z * 128 + lane; j0 < nb; j0 += gridDim.z * 128) {
+        int b[4], old[4];  // four entries of a lane on the way
 #pragma unroll
-        for (int u = 0; u < 4; ++u) b[u] = j0 + 32 * u + lane < nb ? src[j0 + 32 * u + lane] : -1;
+        for (int u = 0; u < 4; ++u) b[u] = j0 + 32 * u < nb ? src[j0 + 32 * u] : -1;
+        if (run) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (j0 + 32 * u + lane >= nb) continue;
-            if ((unsigned)b[u] >= (unsigned)c.num_blocks) set_error(c, MENTAT_DEV_BAD_BLOCK, b[u]);
-            else if (atomicAdd(&c.refcounts[b[u]], run) <= 0) set_error(c, MENTAT_DEV_REF_FREE, b[u]);
+            for (int u = 0; u < 4; ++u) old[u] = (unsigned)b[u] < (unsigned)c.num_blocks ? atomicAdd(&c.refcounts[b[u]], run) : 1;
         }
-        for (int k = 0; k < run; ++k) {
-            int32_t* dst = table_row(c, l, children[i + k]) + j0 + lane;
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (j0 + 32 * u + lane < nb) dst[32 * u] = b[u];
+        for (int u = 0; u < 4; ++u)
+            if (j0 + 32 * u < nb) dst[j0 + 32 * u] = b[u];
+        if (run) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (j0 + 32 * u >= nb) continue;
+                if ((unsigned)b[u] >= (unsigned)c.num_blocks) set_error(c, MENTAT_DEV_BAD_BLOCK, b[u]);
+                else if (old[u] <= 0) set_error(c, MENTAT_DEV_REF_FREE, b[u]);
+            }
         }
     }
-    for (int k = lane; k < run; k += 32) {
-        const int64_t cs = seq_index(c, l, children[i + k]);
+    if (blockIdx.z == 0 && lane == 0) {
         c.nblocks[cs] = nb;
         c.ntok[cs] = ntok;
         c.tail[cs] = tail;
@@ -979,7 +986,10 @@ int mentat_kv_fork_batched(const mentat_kv_cache* c, const int32_t* parents, con
     if (bad_pages(c, n) || (n > 0 && (!parents || !children))) return MENTAT_ERR_ARG;
     if (n == 0) return MENTAT_OK;
     if (!slots_fit(c)) return MENTAT_ERR_UNSUPPORTED;
-    const dim3 grid((n + PAGES_WARPS - 1) / PAGES_WARPS, c->num_layers);
+    // two CTAs an SM at least, if the tables may be long enough (how long they are, only the device knows)
+    const int by_child = (n + PAGES_WARPS - 1) / PAGES_WARPS;
+    const int parts = 2 * 148 / (by_child * c->num_layers);
+    const dim3 grid(by_child, c->num_layers, parts < 2 ? 1 : chunks_of(c->max_blocks_per_seq, 128, parts));
     MENTAT_LAUNCH(k_fork_check, dim3(chunks_of((int64_t)n * c->num_layers, PAGES_THREADS, 148)), dim3(PAGES_THREADS),
                   bitmap_bytes(c), s, *c, parents, children, n);
     MENTAT_LAUNCH(k_fork_batched, grid, dim3(PAGES_THREADS), 0, s, *c, parents, children, n);

@@ -604,3 +604,28 @@ def test_rotated_appends_to_no_layer_change_nothing():
         with pytest.raises(ValueError, match="layer"):
             m.append_rotated_batched([a], layer, x, x, x, rot)
     same(m, o)
+
+
+@pytest.mark.parametrize("capacity", [1001, 20000])  # pages of a table shared out over a few CTAs and over many
+def test_forks_of_runs_and_long_tables(capacity):
+    """Parents of no page to a thousand, in runs of children around a warp's width, in one batch and by the manager."""
+    from mentat_b200 import ops
+    rng = np.random.default_rng(25)
+    m, o = pair(L=2, hkv=1, d=8, pool=20000, bs=1, max_seqs=400, max_blocks_per_seq=capacity, strict=False)
+    ids = start(m, o, [0, 1, 127, 128, 129, 513, 1000], rng)
+    parents = [p for p, run in zip([6, 4, 0, 3, 5, 2, 1, 6, 4], [33, 1, 5, 32, 65, 31, 64, 3, 1]) for _ in range(run)]
+    slots = m._free_slots[::-1][: len(parents)]
+    ops.fork_pages(m, torch.tensor([m._sequences[ids[p]].slot for p in parents], dtype=torch.int32, device="cuda"),
+                   torch.tensor(slots, dtype=torch.int32, device="cuda"))
+    m.check()
+    for p, s in zip(parents, slots):
+        own = m._sequences[ids[p]].slot
+        assert torch.equal(m._nblocks[:, s], m._nblocks[:, own]) and torch.equal(m._ntok[:, s], m._ntok[:, own])
+        nb = int(m._nblocks[0, own])
+        assert torch.equal(m._tables[:, s, :nb], m._tables[:, own, :nb])
+    ops.free_pages(m, torch.tensor(slots, dtype=torch.int32, device="cuda"))
+    same(m, o)
+    for n in (1, 3, 4, 70):
+        some = [ids[p] for p in parents[:n]]
+        assert m.fork_sequences(some) == [o.fork_sequence(s) for s in some]
+    same(m, o)
