@@ -482,7 +482,8 @@ struct CompactArgs {
 constexpr int PLAN_CHUNK = 512;  // kept positions of a warp's step; the last chunk goes on to the end of a list
 // The plan, in one cluster, a warp a range of rows: the batch is checked, the kept positions are inside their
 // sequences; how many pages at the front stay, and the fresh blocks of the others.  Bound by latency (the lists
-// are a thousandth of the bytes that are moved): 12 us for 8 sequences in 4 layers, 21 for 12 of 16,000 tokens in 2.
+// are a thousandth of the bytes that are moved): 12 us for 8 sequences in 4 layers, 21 for 12 of 16,000 tokens in 2;
+// alone with cold caches 16 and 26.
 __global__ void __launch_bounds__(CLUSTER_THREADS) k_compact_plan(mentat_kv_cache c, CompactArgs a, int chunks,
                                                                   PagesWs w) {
     extern __shared__ uint32_t bits[];
@@ -734,8 +735,8 @@ __device__ __forceinline__ void turn_row(T* row, int H, int D, const mentat_rota
 // through a ring of stages.  A producer warp looks up where the rows come from and copies them in with bulk
 // copies, K and V, a stage ahead or more; eight warps turn K in place; the stage, which is contiguous in the
 // fresh page, leaves as two bulk copies.  So the bytes pass through registers only where they change, and the
-// next rows are always on the way.  Bound by memory: 1.3 GB in 223 us, 5.9 TB/s (through registers, a CTA a page: 3.0);
-// 75 MB in 19 us, of which the first and last stages, which nothing covers, are 6.
+// next rows are always on the way.  Bound by memory: 1.3 GB in 229 us alone, 5.7 TB/s (through registers, a CTA a page: 3.0);
+// 75 MB in 23 us with cold caches, 19 among other calls, of which the first and last stages, which nothing covers, are 6.
 constexpr int STREAM_WORKERS = 256, STREAM_THREADS = STREAM_WORKERS + 32, STREAM_MAX_STAGES = 4;
 template <typename T, int VEC, bool IL>
 __global__ void __launch_bounds__(STREAM_THREADS) k_compact_stream(mentat_kv_cache c, CompactArgs a, mentat_rotary r,

@@ -124,9 +124,10 @@ template <> struct Extreme<__half> {
 };
 
 // The index of all heads of one block by one CTA, 16 bytes of a row to a thread (head_dim / VEC threads to a
-// head, a power of two within a warp, every thread of which takes part); the page is read once, 8 rows of a
-// thread on the way at a time.  Bound by memory: 8,192 pages of 16 x 8 heads of 128 (285 MB) in 55 us, 5.2 TB/s (15
-// rows at a time 58; a ring of bulk copies in one CTA on an SM 61).
+// head, a power of two within a warp, every thread of which takes part); the page is read once, 8 rows asked
+// for at a time, of which the 32 registers that the compiler takes hold about half.  Bound by memory: 8,192 pages of 16 x
+// 8 heads of 128 (285 MB) in 50 us alone with cold caches, 5.7 TB/s; among other calls 55 (15 rows at a time 58; a ring of
+// bulk copies in one CTA on an SM 61).
 template <typename T>
 __device__ __forceinline__ void index_block(const mentat_kv_cache& c, int layer, int b, const mentat_page_index& x) {
     using E = Extreme<T>;
@@ -237,7 +238,7 @@ __global__ void k_index_seqs(mentat_kv_cache c, int layer0, const int32_t* slots
 }
 
 // Four pages to a CTA, each thread one piece of each of them on the way.  Bound by the stores: 8,192 pages of 8 heads
-// of 128 (84 MB) take 15 us, with stores that stay in L2 22.
+// of 128 (84 MB) take 20 us alone with cold caches; with stores that stay in L2 the index and this take 80 us, not 74.
 constexpr int BOUNDS_PAGES = 4;
 __global__ void __launch_bounds__(256) k_page_bounds(mentat_kv_cache c, int layer, const int32_t* blocks, int n,
                                                      mentat_page_index x, float* low, float* high, int8_t* exps) {
@@ -295,7 +296,8 @@ __global__ void __launch_bounds__(256) k_page_bounds(mentat_kv_cache c, int laye
 // The cluster's CTAs score a slice of the pages each and write the keys to all of their
 // shared memories; each then makes the whole choice for itself, attends to an equal share
 // of the chosen pages, and they merge their partials: one launch, and no workspace.  Bound by latency: one sequence of
-// 4,000 tokens takes 10 us (slots, lengths, table, bounds, the choice and the pages wait for one another).
+// 4,000 tokens takes 10 us, 16 alone with cold caches (slots, lengths, table, bounds, the choice and the pages wait for
+// one another).
 // warps of a CTA: with the tensor-core path's rings two CTAs of four fit on an SM; the other path is bound by
 // latency and takes eight
 __host__ __device__ constexpr int sparse_warps(bool mma) { return mma ? 4 : 8; }
@@ -822,7 +824,7 @@ __device__ __forceinline__ void attend_simple(const mentat_kv_cache& c, const Sp
 // time for the batch below, and an error against 64 bits 3 to 5 % above that of the output's rounding alone.)
 //
 // Bound by memory: 64 sequences with 128 pages each for 8 KV heads of 128 (540 MB of different rows, 1.07 GB with
-// those that several sequences chose) take 80 us, 6.7 TB/s of the former.  A tile of the larger tensor-core
+// those that several sequences chose) take 88 us alone with cold caches, 6.1 TB/s of the former.  A tile of the larger tensor-core
 // instruction has 128 rows, of which a KV head's group would fill at most 16.
 template <typename T, int D, int GM>
 __device__ __forceinline__ void attend_mma(const mentat_kv_cache& c, const SparseArgs& a, const CUtensorMap* mk,
@@ -1130,8 +1132,8 @@ __global__ void __launch_bounds__(32 * sparse_warps(MMA)) k_sparse(const __grid_
 // where all of them have the same 16 blocks the bounds are read once.  Two warps take 16 pages, half of the
 // columns each.  Pages that are not shared are put aside, and then shared out by sequence among all warps of the
 // CTA.  A warp has the next pages' bounds and the blocks of those after them on the way while it works.
-// Bound by latency and issue: 64 sequences of 2,050 to 2,300 pages, 2,048 in common, 8 KV heads of 4 query heads: 19 us
-// (the bounds are 4 MB, the byte products 3 us); 24 where each warp pair scored its own unshared tiles.
+// Bound by latency and issue: 64 sequences of 2,050 to 2,300 pages, 2,048 in common, 8 KV heads of 4 query heads: 19 us,
+// 21 alone with cold caches (the bounds are 4 MB, the byte products 3 us); 24 where each warp pair scored its own unshared tiles.
 constexpr int SCORE_THREADS = 256, SCORE_WARPS = SCORE_THREADS / 32;
 constexpr int SCORE_TILES = SCORE_WARPS / 2;  // tiles of 16 pages at a time
 constexpr int SCORE_ASIDE = 1024;             // tiles between two looks at those put aside
@@ -1395,7 +1397,7 @@ __global__ void __launch_bounds__(SCORE_THREADS, 2) k_score(mentat_kv_cache c, m
 }
 
 // The chosen pages from the keys (12 us for 512 of 2,200 pages; made by the attention's CTAs instead, the same batch
-// takes 126 us in all, not 121): one CTA per (sequence, KV head), or a cluster where a sequence may have
+// took 126 us in all where this took 121): one CTA per (sequence, KV head), or a cluster where a sequence may have
 // more than HELD_PAGES pages.
 constexpr int CHOOSE_THREADS = 256, HELD_PAGES = 16384;
 template <bool CL>
