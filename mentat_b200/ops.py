@@ -414,7 +414,9 @@ class _Turn(torch.autograd.Function):
         ctx.save_for_backward(positions)
         ctx.rot, ctx.inverse = rot, inverse
         ctx.set_materialize_grads(False)
-        return rotary(q, k, positions, rot, inverse=inverse)
+        out = rotary(q, k, positions, rot, inverse=inverse)
+        ctx.mark_non_differentiable(*(o for o, need in zip(out, ctx.needs_input_grad) if o is not None and not need))
+        return out
 
     @staticmethod
     def backward(ctx, gq, gk):

@@ -35,8 +35,8 @@ from . import _lib, ops
 _DTYPES = {torch.float32: _lib.MENTAT_F32, torch.bfloat16: _lib.MENTAT_BF16, torch.float16: _lib.MENTAT_F16}
 
 # Sequences that fork_sequences forks one by one.  A batch's slots are uploaded and checked first, which takes as long as
-# three or four single calls: 3 children 37 us singly and 53 as a batch, from the call to the device's end; on the
-# device 14 and 12.
+# four single calls: 3 children take 31 us singly and 53 as a batch, from the call to the device's end (4 children 45 and
+# 54), and 14 and 12 us on the device.
 FEW_FORKS = 3
 
 OUT_OF_BLOCKS_MSG = ("PagedKVCache: out of blocks (pool size={n}).  "

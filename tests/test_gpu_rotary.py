@@ -277,3 +277,11 @@ def test_gradients_in_a_graph():
         for a, b, name in zip(got, up, "qk"):
             _near(a, b, pos, rot, inverse=True, what=name)
     assert torch.equal(torch.autograd.grad(alive, (q, k), up)[0], got[0])
+
+
+def test_outputs_require_gradients_as_their_inputs_do():
+    from mentat_b200 import Rotary, ops
+    rot, pos = Rotary(64), torch.arange(3, device="cuda")
+    for need in ((True, False), (False, True), (True, True), (False, False)):
+        q, k = (torch.ones((3, 2, 64), device="cuda").requires_grad_(n) for n in need)
+        assert tuple(t.requires_grad for t in ops.rotary(q, k, pos, rot)) == need
